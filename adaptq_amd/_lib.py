@@ -18,6 +18,15 @@ _f = C.POINTER(C.c_float)
 _u8 = C.POINTER(C.c_uint8)
 _ip = C.POINTER(C.c_int)
 
+class Rows(C.Structure):
+    """adaptq_rows_t"""
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("n_heads", C.c_int),
+                ("in_nb1", C.c_size_t), ("in_nb2", C.c_size_t), ("in_nb3", C.c_size_t),
+                ("out_nb1", C.c_size_t), ("out_nb2", C.c_size_t), ("out_nb3", C.c_size_t)]
+
+
+_v, _i, _z = C.c_void_p, C.c_int, C.c_size_t
+
 # name -> (restype, argtypes); every symbol declared in include/adaptq.h.
 SIGNATURES = {
     "adaptq_last_error": (C.c_char_p, []),
@@ -77,6 +86,19 @@ SIGNATURES = {
                                                        C.c_void_p, C.c_void_p, C.c_void_p]),
     "adaptq_mha_step_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                          C.c_int, C.c_int, C.c_void_p]),
+    # rotary positions and the paged cache
+    "adaptq_rotary_create": (_v, [_i, _i, C.c_double, _i, C.c_double, _i, C.c_double, C.c_double,
+                                  C.c_double]),
+    "adaptq_rotary_destroy": (None, [_v]),
+    "adaptq_rotary_device": (_i, [_v, C.POINTER(Rows), _i, _i, _i, _v, _z, _i, _i, _i, _v]),
+    "adaptq_paged_create": (_v, [_v, _v, _i, _i, _i, _i, _i, _v]),
+    "adaptq_paged_destroy": (None, [_v]),
+    "adaptq_paged_append_device": (_i, [_v, _v, _v, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i, _v,
+                                        _v]),
+    "adaptq_paged_attend_device": (_i, [_v, _v, _v, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i,
+                                        C.c_float, _i, _v]),
+    "adaptq_paged_step_device": (_i, [_v, _v, _v, _z, _z, _z, _z, _v, _v, _i, _z, _z, _z, _z, _v,
+                                      _i, _i, _v, _i, C.c_float, _i, _v]),
 }
 
 FEAT_AVX2, FEAT_HYBRID, FEAT_SPARSE_V, FEAT_HIP = 1, 2, 4, 8

@@ -112,6 +112,80 @@ class PyMHAContext {
   int head_dim_, n_heads_;
 };
 
+// Handles of the rotary positions and the paged cache; addresses are device
+// pointers (torch-ROCm tensors' data_ptr()), strides bytes.
+using addr = uintptr_t;
+
+void *ptr(addr a) { return reinterpret_cast<void *>(a); }
+const int *ints(addr a) { return reinterpret_cast<const int *>(a); }
+void check(int rc) {
+  if (rc != 0) throw std::runtime_error(adaptq_last_error());
+}
+
+class PyRotary {
+ public:
+  PyRotary(int dim, bool interleaved, double base, int scaling, double factor, int context,
+           double slow, double fast, double amplitude)
+      : h_(adaptq_rotary_create(dim, interleaved, base, scaling, factor, context, slow, fast,
+                                amplitude)) {
+    if (!h_) throw std::runtime_error(adaptq_last_error());
+  }
+  ~PyRotary() { adaptq_rotary_destroy(h_); }
+  PyRotary(const PyRotary &) = delete;
+  PyRotary &operator=(const PyRotary &) = delete;
+  adaptq_rotary_t handle() const { return h_; }
+
+  void rotate(addr positions, size_t pos_stride, int n_batch, int n_tokens, int dim, int io,
+              bool backward, addr stream, addr q, addr q_out, int q_heads, size_t q1, size_t q2,
+              size_t q3, size_t qo1, size_t qo2, size_t qo3, addr k, addr k_out, int k_heads,
+              size_t k1, size_t k2, size_t k3, size_t ko1, size_t ko2, size_t ko3) {
+    const adaptq_rows_t rows[2] = {{ptr(q), ptr(q_out), q_heads, q1, q2, q3, qo1, qo2, qo3},
+                                   {ptr(k), ptr(k_out), k_heads, k1, k2, k3, ko1, ko2, ko3}};
+    check(adaptq_rotary_device(h_, rows, k ? 2 : 1, dim, io, ints(positions), pos_stride, n_batch,
+                               n_tokens, backward, ptr(stream)));
+  }
+
+ private:
+  adaptq_rotary_t h_;
+};
+
+class PyPagedCache {
+ public:
+  PyPagedCache(addr k_pages, addr v_pages, int n_pages, int page_size, int n_heads, int dim,
+               int io, const PyRotary *rotary)
+      : h_(adaptq_paged_create(ptr(k_pages), ptr(v_pages), n_pages, page_size, n_heads, dim, io,
+                               rotary ? rotary->handle() : nullptr)) {
+    if (!h_) throw std::runtime_error(adaptq_last_error());
+  }
+  ~PyPagedCache() { adaptq_paged_destroy(h_); }
+  PyPagedCache(const PyPagedCache &) = delete;
+  PyPagedCache &operator=(const PyPagedCache &) = delete;
+
+  void append(addr k, addr v, int n_tokens, size_t k1, size_t k2, size_t v1, size_t v2, addr table,
+              int width, int stride, addr lengths, int n_seqs, addr offsets, addr stream) {
+    check(adaptq_paged_append_device(h_, ptr(k), ptr(v), n_tokens, k1, k2, v1, v2, ints(table),
+                                     width, stride, ints(lengths), n_seqs, ints(offsets),
+                                     ptr(stream)));
+  }
+  void attend(addr q, addr out, int q_heads, size_t q1, size_t q2, size_t o1, size_t o2,
+              addr table, int width, int stride, addr lengths, int n_seqs, float scale, int window,
+              addr stream) {
+    check(adaptq_paged_attend_device(h_, ptr(q), ptr(out), q_heads, q1, q2, o1, o2, ints(table),
+                                     width, stride, ints(lengths), n_seqs, scale, window,
+                                     ptr(stream)));
+  }
+  void step(addr k, addr v, size_t k1, size_t k2, size_t v1, size_t v2, addr q, addr out,
+            int q_heads, size_t q1, size_t q2, size_t o1, size_t o2, addr table, int width,
+            int stride, addr lengths, int n_seqs, float scale, int window, addr stream) {
+    check(adaptq_paged_step_device(h_, ptr(k), ptr(v), k1, k2, v1, v2, ptr(q), ptr(out), q_heads,
+                                   q1, q2, o1, o2, ints(table), width, stride, ints(lengths),
+                                   n_seqs, scale, window, ptr(stream)));
+  }
+
+ private:
+  adaptq_paged_t h_;
+};
+
 }  // namespace
 
 PYBIND11_MODULE(adaptq_py, m) {
@@ -138,4 +212,21 @@ PYBIND11_MODULE(adaptq_py, m) {
       .def("kv_bytes", &PyMHAContext::kv_bytes)
       .def_property_readonly("n_heads", &PyMHAContext::n_heads)
       .def_property_readonly("head_dim", &PyMHAContext::head_dim);
+
+  // what adaptq_amd.rotary and adaptq_amd.paged call, in the order of their arguments
+  py::class_<PyRotary>(m, "Rotary")
+      .def(py::init<int, bool, double, int, double, int, double, double, double>())
+      .def("rotate", &PyRotary::rotate)
+      .def("rotate", [](PyRotary &r, addr positions, size_t pos_stride, int n_batch, int n_tokens,
+                        int dim, int io, bool backward, addr stream, addr q, addr q_out,
+                        int q_heads, size_t q1, size_t q2, size_t q3, size_t qo1, size_t qo2,
+                        size_t qo3) {
+        r.rotate(positions, pos_stride, n_batch, n_tokens, dim, io, backward, stream, q, q_out,
+                 q_heads, q1, q2, q3, qo1, qo2, qo3, 0, 0, 0, 0, 0, 0, 0, 0, 0);
+      });
+  py::class_<PyPagedCache>(m, "PagedCache")
+      .def(py::init<addr, addr, int, int, int, int, int, const PyRotary *>())
+      .def("append", &PyPagedCache::append)
+      .def("attend", &PyPagedCache::attend)
+      .def("step", &PyPagedCache::step);
 }

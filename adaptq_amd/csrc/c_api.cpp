@@ -25,6 +25,7 @@
 #include "../../include/adaptq.h"
 #include "device.hpp"
 #include "device_buffer.hpp"
+#include "host.hpp"
 #include "launch.hpp"
 
 // Workspace of the allocation-free decode (adaptq_plan_compute_device_static):
@@ -35,42 +36,29 @@
 constexpr size_t kScratchBytes = (size_t)8 << 20;
 static __device__ __align__(256) uint8_t scratch[kScratchBytes];
 
+namespace aq {
+
+namespace {
+thread_local char tl_error[256] = "";
+}
+
+void set_error(const char *msg) { std::snprintf(tl_error, sizeof(tl_error), "%s", msg); }
+void clear_error() { tl_error[0] = '\0'; }
+
+}  // namespace aq
+
 namespace {
 
 using aq::DevBuf;
 using aq::KeptBuf;
 
-thread_local char tl_error[256] = "";
-
-void set_error(const char *msg) { std::snprintf(tl_error, sizeof(tl_error), "%s", msg); }
-
-void set_errorf(const char *fn, const char *what) {
-  std::snprintf(tl_error, sizeof(tl_error), "%s: %s", fn, what);
-}
-
-void clear_error() { tl_error[0] = '\0'; }
-
-bool require_handle(const void *h, const char *fn) {
-  if (h) return true;
-  set_errorf(fn, "null handle");
-  return false;
-}
-
-bool require_pointer(const void *p, const char *fn, const char *param) {
-  if (p) return true;
-  char msg[256];
-  std::snprintf(msg, sizeof(msg), "%s: null %s", fn, param);
-  set_error(msg);
-  return false;
-}
-
-bool hip_fail(hipError_t e, const char *fn) {
-  if (e == hipSuccess) return false;
-  char msg[256];
-  std::snprintf(msg, sizeof(msg), "%s: HIP error: %s", fn, hipGetErrorString(e));
-  set_error(msg);
-  return true;
-}
+using aq::clear_error;
+using aq::DeviceGuard;
+using aq::hip_fail;
+using aq::require_handle;
+using aq::require_pointer;
+using aq::set_error;
+using aq::set_errorf;
 
 int next_pow2(int n) {
   if (n <= 1) return 1;
@@ -425,19 +413,6 @@ bool any_mirror(const std::vector<Ctx *> &cs, int n) {
     if (aq::mirror_count(c->st, n, c->cap, c->hyb) > 0) return true;
   return false;
 }
-
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    if (prev != dev) (void)hipSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    (void)hipGetDevice(&cur);
-    if (prev >= 0 && cur != prev) (void)hipSetDevice(prev);
-  }
-};
 
 void free_ctx(Ctx *c) {
   if (!c) return;
@@ -1063,7 +1038,7 @@ int step_device(Mha *m, const void *dk, const void *dv, const void *dq, void *do
 
 extern "C" {
 
-const char *adaptq_last_error(void) { return tl_error; }
+const char *adaptq_last_error(void) { return aq::tl_error; }
 
 adaptq_ctx_t adaptq_create(int dim, int k_bits, int v_bits, int capacity, uint64_t seed,
                            float v_mass, int hybrid_thresh) {

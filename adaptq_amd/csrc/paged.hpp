@@ -1,0 +1,78 @@
+// paged.hpp -- host-side launchers of the rotary and paged-cache kernels
+// (rotary.hip, paged.hip).  All are asynchronous on the given stream and return
+// the HIP launch status.
+#pragma once
+
+#include "launch.hpp"
+
+namespace aq {
+
+// A rotation, its per-pair steps (see rotary.hpp) in device memory.
+struct RotaryTable {
+  const uint64_t *steps;  // [pairs]; pairs 0: no rotation
+  int pairs;
+  bool interleaved;
+  float amplitude;
+};
+
+struct RotaryRows {
+  const void *in;
+  void *out;
+  int n_heads;
+  size_t in_nb[3], out_nb[3];  // byte strides between heads, tokens, batches
+};
+
+struct RotaryCall {
+  RotaryRows rows[2];
+  int n_rows;
+  const int *positions;
+  size_t pos_stride;
+  int n_batch, n_tokens, dim;
+  IoType io;
+  bool backward;
+};
+
+hipError_t launch_rotary(const RotaryTable &t, const RotaryCall &c, hipStream_t s);
+
+// The pages of a cache: [n_pages][n_heads][page_size][dim] of io, keys and values.
+struct PagedShape {
+  void *k_pages, *v_pages;
+  int n_pages, page_size, n_heads, dim;
+  IoType io;
+  RotaryTable rotary;
+};
+
+// Which pages a sequence's tokens lie in, and how many it holds.
+struct PagedSeqs {
+  const int *table;  // [n_seqs] rows of `width` page numbers, `stride` apart
+  int width, stride;
+  const int *lengths;
+  int n_seqs;
+};
+
+struct PagedAppend {
+  const void *k, *v;
+  size_t k_nb[2], v_nb[2];  // byte strides between heads, tokens
+  int n_tokens;
+  const int *offsets;  // [n_seqs + 1], or null: one token a sequence
+};
+
+hipError_t launch_paged_append(const PagedShape &p, const PagedSeqs &q, const PagedAppend &a,
+                               hipStream_t s);
+
+struct PagedAttend {
+  const void *q;
+  void *out;
+  size_t q_nb[2], out_nb[2];
+  int q_heads;
+  float scale;
+  int window;  // 0: all tokens
+  int extra;   // tokens beyond `lengths` that a sequence holds by now
+};
+
+// Bytes of workspace an attention of this shape may need, zeroed once when it is made.
+size_t paged_workspace_bytes(const PagedShape &p);
+hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
+                               void *workspace, hipStream_t s);
+
+}  // namespace aq

@@ -1,0 +1,152 @@
+"""``Rotary``: rotary positions on queries and keys (adaptq_rotary_* of adaptq.h).
+
+    rotary = Rotary(128, base=500000.0)
+    q, k = rotary(positions, q, k)         # [tokens, heads, dim] or [batch, tokens, heads, dim]
+
+Device tensors of fp32, fp16 or bf16, rotated in one launch on torch's current
+stream, in fp32 and rounded once.  Differentiable in q and k.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import adaptq_py
+
+# ADAPTQ_IO_* and ADAPTQ_ROTARY_* in adaptq.h
+IO_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+def stream_of(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class Rotary:
+    """Rotation of the first ``dim`` channels of a row: pairs (i, i + dim/2), or
+    (2i, 2i + 1) with ``interleaved``, by position * base^(-2i/dim).
+
+    scaling, for contexts longer than a model was trained on:
+
+    - "linear": every angle divided by ``factor``;
+    - "ntk": base * factor^(dim/(dim-2)) in place of base;
+    - "bands": pairs that turn more than ``fast`` (4) times over ``context``
+      positions stay, those below ``slow`` (1) are divided by factor, linear between;
+    - "yarn": the same with the ramp over the pairs' numbers and ``fast`` 32, and
+      cosine and sine times 0.1 ln(factor) + 1.
+
+    ``amplitude`` replaces the factor on cosine and sine (1, but for "yarn").  The
+    object lives on ``device`` (the current one).
+    """
+
+    def __init__(self, dim: int, *, base: float = 10000.0, interleaved: bool = False,
+                 scaling: str | None = None, factor: float = 1.0, context: int = 0,
+                 slow: float | None = None, fast: float | None = None,
+                 amplitude: float | None = None, device=None):
+        if scaling not in SCALINGS:
+            raise ValueError(f"scaling must be one of {list(SCALINGS)}, got {scaling!r}")
+        for name, x in (("slow", slow), ("fast", fast), ("amplitude", amplitude)):
+            if x is not None and not x > 0:
+                raise ValueError(f"{name} must be positive, got {x}")
+        self.dim = dim
+        self.device = torch.device("cuda" if device is None else device)
+        if self.device.type != "cuda":
+            raise ValueError(f"Rotary lives on a GPU, got device {self.device}")
+        with torch.cuda.device(self.device):
+            self.device = torch.device("cuda", torch.cuda.current_device())
+            self._handle = adaptq_py.Rotary(dim, interleaved, base, SCALINGS[scaling], factor,
+                                            context, slow or 0.0, fast or 0.0, amplitude or 0.0)
+
+    def __call__(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, *,
+                 inplace: bool = False):
+        """Rotated q, or (q, k).  positions: int32 [tokens] or [batch, tokens]; q, k: [tokens,
+        heads, dim] or [batch, tokens, heads, dim] of one type, any strides with rows side by
+        side.  inplace: writes into q and k (not where they need gradients)."""
+        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+            if inplace:
+                raise ValueError("inplace rotation of tensors that need gradients")
+            out = _Rotate.apply(self, positions, False, q, k)
+            return out if k is not None else out[0]
+        out = self._rotate(positions, q, k, inplace, False)
+        return out if k is not None else out[0]
+
+    def _rotate(self, positions, q, k, inplace, backward):
+        if positions.dtype != torch.int32:
+            raise TypeError(f"positions must be int32, got {positions.dtype}")
+        io = IO_TYPES.get(q.dtype)
+        if io is None:
+            raise TypeError(f"rows must be float32, float16 or bfloat16, got {q.dtype}")
+        n = q.dim()
+        if n != 3 and n != 4:
+            raise ValueError("rows must be [tokens, heads, dim] or [batch, tokens, heads, dim], "
+                             f"got {tuple(q.shape)}")
+        shape = q.shape
+        batch, tokens, dim = (shape[0] if n == 4 else 1), shape[-3], shape[-1]
+        if positions.dim() == 1:
+            ok, stride = positions.shape[0] == tokens, 0
+        else:
+            ok = n == 4 and positions.shape in ((batch, tokens), (1, tokens))
+            stride = positions.stride(0) if ok and positions.shape[0] > 1 else 0
+        if not ok:
+            raise ValueError(f"positions of shape {tuple(positions.shape)} do not fit rows of "
+                             f"shape {tuple(shape)}")
+        if tokens > 1 and positions.stride(-1) != 1 or stride and stride < tokens:
+            positions, stride = positions.contiguous(), tokens if stride else 0
+        if q.device != self.device or positions.device != self.device:
+            raise ValueError(f"tensors must be on {self.device}")
+        args = []
+        outs = []
+        for x in (q, k):
+            if x is None:
+                outs.append(None)
+                continue
+            if x is k and (x.dtype != q.dtype or x.device != q.device or x.dim() != n or
+                           x.shape[:-2] != shape[:-2] or x.shape[-1] != dim):
+                raise ValueError(f"k {tuple(x.shape)} {x.dtype} does not go with q "
+                                 f"{tuple(shape)} {q.dtype}")
+            if x.numel() and x.stride(-1) != 1:
+                if inplace:
+                    raise ValueError("inplace needs rows whose values lie side by side")
+                x = x.contiguous()
+            y = x if inplace else torch.empty_like(x)
+            if y is not x and y.numel() and y.stride(-1) != 1:
+                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            outs.append(y)
+            size = x.element_size()
+            s, t = x.stride(), y.stride()
+            args += (x.data_ptr(), y.data_ptr(), x.shape[-2], s[-2] * size, s[-3] * size,
+                     s[0] * size if n == 4 else 0, t[-2] * size, t[-3] * size,
+                     t[0] * size if n == 4 else 0)
+        if q.numel() == 0 or k is not None and k.numel() == 0:
+            if q.numel() or k is not None and k.numel():
+                raise ValueError("q and k must both have heads")
+            return tuple(outs)
+        self._handle.rotate(positions.data_ptr(), stride, batch, tokens, dim, io, backward,
+                            stream_of(self.device), *args)
+        return tuple(outs)
+
+
+class _Rotate(torch.autograd.Function):
+    """The rotation, whose gradient is the transposed rotation of the outputs' gradients
+    (itself differentiable)."""
+
+    @staticmethod
+    def forward(ctx, rotary, positions, backward, q, k):
+        ctx.rotary, ctx.backward_ = rotary, backward
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        out = rotary._rotate(positions, q, k, False, backward)
+        ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad[3:])
+                                      if y is not None and not need))
+        return out
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        (positions,) = ctx.saved_tensors
+        want = [g if need else None
+                for g, need in zip((dq, dk), ctx.needs_input_grad[3:])]
+        have = [g for g in want if g is not None]
+        if have:
+            got = iter(_Rotate.apply(ctx.rotary, positions, not ctx.backward_, have[0],
+                                     have[1] if len(have) > 1 else None))
+            want = [next(got) if g is not None else None for g in want]
+        return (None, None, None, *want)

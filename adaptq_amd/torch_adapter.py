@@ -7,6 +7,9 @@ Same constructor, ``forward(q, k, v)`` on (1, heads, dim) tensors and
 step appends k, v and decodes q in one call on torch's current stream, in
 their own element type (fp32, fp16 or bf16), so nothing is copied to the host.
 CPU tensors take the Engine's host path.
+
+With ``rotary`` (adaptq_amd.rotary.Rotary), q and k are rotated by the token's
+position before the step, where the reference leaves that to its caller.
 """
 from __future__ import annotations
 
@@ -22,7 +25,7 @@ _IO_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 class AdaptQAttention(nn.Module):
     def __init__(self, dim: int, heads: int, k_bits: int = 4, v_bits: int = 4,
-                 capacity: int = 4096, seed: int = 42):
+                 capacity: int = 4096, seed: int = 42, rotary=None):
         super().__init__()
         self.dim = dim
         self.heads = heads
@@ -30,6 +33,18 @@ class AdaptQAttention(nn.Module):
         self.v_bits = v_bits
         self.engine = Engine(dim=dim, heads=heads, k_bits=k_bits, v_bits=v_bits,
                              capacity=capacity, seed=seed)
+        self.rotary = rotary
+        # the positions first, first + 1, ... on the rotary's device: a token's call takes
+        # one of them and uploads nothing
+        self._positions, self._first = None, 0
+
+    def _position(self) -> torch.Tensor:
+        at = self.engine.pos - self._first
+        if self._positions is None or not 0 <= at < self._positions.shape[0]:
+            self._first, at = self.engine.pos, 0
+            self._positions = torch.arange(self._first, self._first + 4096, dtype=torch.int32,
+                                           device=self.rotary.device)
+        return self._positions[at:at + 1]
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """q, k, v: (1, heads, dim).  Appends k, v, then returns the attention
@@ -49,6 +64,12 @@ class AdaptQAttention(nn.Module):
             raise ValueError(f"Expected k shape {tuple(q.shape)}, got {tuple(k.shape)}.")
         if v.shape != q.shape:
             raise ValueError(f"Expected v shape {tuple(q.shape)}, got {tuple(v.shape)}.")
+
+        if self.rotary is not None:
+            if not q.is_cuda:
+                raise ValueError("AdaptQAttention with rotary takes tensors on the GPU.")
+            with torch.no_grad():
+                q, k = self.rotary(self._position(), q, k)
 
         if q.is_cuda:
             # a token's call is bound by the host: nothing here makes a tensor

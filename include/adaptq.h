@@ -7,7 +7,8 @@
  * are quantised by a HIP kernel and attention is computed by HIP kernels.
  *
  * Part 2 lists extensions that have no counterpart in the reference; each
- * says which callers it is for.
+ * says which callers it is for.  Part 3 adds rotary positions and a paged cache of
+ * exact rows.
  *
  * Threading: each handle is independent (reference adaptq.h:12).  Calls on
  * one handle are serialised by a per-handle lock.  The last-error string is
@@ -343,6 +344,129 @@ int adaptq_plan_compute_device_static(adaptq_plan_t plan, const float *d_queries
  * Returns -1 on error (a null handle, or a context with staged host
  * appends). */
 long long adaptq_plan_workspace_bytes(adaptq_plan_t plan);
+
+/* ================= Part 3: rotary positions and the paged cache =================
+ *
+ * Extensions, no counterpart in the reference.  For serving loops beside the
+ * packed rings: keys and queries rotated by their positions, and a cache of exact
+ * rows (fp32, fp16 or bf16) in pages that sequences of any length share, with
+ * several query heads per key head.
+ *
+ * All data is device memory, and every call is asynchronous on `stream` (a
+ * hipStream_t of the handle's device; NULL = the HIP null stream), allocates
+ * nothing and waits for nothing; all may be captured into a HIP graph (creations
+ * and destructions may not).  What a call reads on the device (positions, tables,
+ * lengths, offsets) is read when it runs, so a captured call follows what these
+ * hold at each replay.  Handles live on the HIP device current at their creation.
+ * Byte strides: nb1 between heads, nb2 between tokens (or sequences), nb3 between
+ * batches, multiples of the element size; a row's `dim` values lie side by side.
+ * Rows aligned to 16 bytes are read fastest. */
+
+/* A rotation: for the pairs i < rotary_dim / 2 of a row, channels (i, i +
+ * rotary_dim/2), or (2i, 2i + 1) when interleaved,
+ *   y1 = a (x1 cos - x2 sin), y2 = a (x2 cos + x1 sin), angle = position * f_i;
+ * channels from rotary_dim on pass through.  f_i = base^(-2i / rotary_dim), scaled
+ * for contexts longer than a model was trained on:
+ *   LINEAR  f_i / factor
+ *   NTK     base * factor^(rotary_dim / (rotary_dim - 2)) in place of base
+ *   BANDS   pairs that turn more than `fast` times over `context` positions keep
+ *           f_i, those below `slow` take f_i / factor, linear between in the turns
+ *   YARN    the same with the ramp linear in i, between the floor of the pair that
+ *           turns `fast` times and the ceiling of the one that turns `slow` times
+ *           (kept within 0 and rotary_dim - 1)
+ * slow, fast: 0 = 1 and 4 (YARN: 1 and 32).  amplitude a: 0 = 1 (YARN:
+ * 0.1 ln(factor) + 1).  Angles are exact to 2^-33 of a turn at every position.
+ * Returns NULL and sets the last error on invalid arguments. */
+typedef void *adaptq_rotary_t;
+enum {
+  ADAPTQ_ROTARY_PLAIN = 0,
+  ADAPTQ_ROTARY_LINEAR = 1,
+  ADAPTQ_ROTARY_NTK = 2,
+  ADAPTQ_ROTARY_YARN = 3,
+  ADAPTQ_ROTARY_BANDS = 4
+};
+adaptq_rotary_t adaptq_rotary_create(int rotary_dim, int interleaved, double base, int scaling,
+                                     double factor, int context, double slow, double fast,
+                                     double amplitude);
+/* Waits for the device's work.  NULL is a no-op. */
+void adaptq_rotary_destroy(adaptq_rotary_t rotary);
+
+/* Rows [n_batch][n_tokens][n_heads][dim], read from `in` and written to `out`, which
+ * may be `in` itself with the same strides. */
+typedef struct {
+  const void *in;
+  void *out;
+  int n_heads;
+  size_t in_nb1, in_nb2, in_nb3;
+  size_t out_nb1, out_nb2, out_nb3;
+} adaptq_rows_t;
+
+/* Rotates one or two sets of rows (queries and keys) in one launch.  d_positions:
+ * [n_batch] rows of n_tokens, pos_stride values apart (0: one row for every batch);
+ * any int, negative ones turn backwards.  backward: the transposed rotation, which
+ * takes the gradient of the outputs to that of the inputs.  dim from rotary_dim to
+ * 1024.  Arithmetic in fp32, rounded once to io_type (ADAPTQ_IO_*).  Outputs that
+ * overlap each other or another set's input are refused.  Returns 0/-1. */
+int adaptq_rotary_device(adaptq_rotary_t rotary, const adaptq_rows_t *rows, int n_rows, int dim,
+                         int io_type, const int *d_positions, size_t pos_stride, int n_batch,
+                         int n_tokens, int backward, void *stream);
+
+/* A cache over two pools of pages that the caller holds, [n_pages][n_heads]
+ * [page_size][dim] of io_type, 16-byte aligned: page_size a multiple of 16 up to
+ * 65536, dim a multiple of 8 up to 256.  The handle keeps the pools' addresses and
+ * the few MB of workspace that its attention needs; it copies `rotary` (NULL: rows
+ * are taken as they are), by which appended keys and the queries of attention are
+ * rotated.  Several handles may share pools.  Calls on one handle from different
+ * streams (graph replays too) must be ordered by the caller. */
+typedef void *adaptq_paged_t;
+adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
+                                   int n_heads, int dim, int io_type, adaptq_rotary_t rotary);
+/* Waits for the device's work; the pools stay the caller's.  NULL is a no-op. */
+void adaptq_paged_destroy(adaptq_paged_t cache);
+
+/* The arguments that name a call's sequences: d_table [n_seqs] rows of table_width
+ * page numbers, table_stride ints apart: token p of sequence b lies in page
+ * d_table[b][p / page_size], slot p % page_size.  d_lengths [n_seqs]: the tokens
+ * each sequence holds before the call.  The library changes neither; entries behind
+ * a sequence's last page may hold anything.
+ *
+ * append: writes n_tokens rows, d_k and d_v [n_tokens][n_heads][dim].  d_offsets
+ * [n_seqs + 1], ascending: tokens d_offsets[b] to d_offsets[b + 1] - 1 go to sequence
+ * b at positions d_lengths[b], d_lengths[b] + 1, ...; tokens outside all of them are
+ * left out.  d_offsets NULL: token b goes to sequence b (n_tokens = n_seqs).  A token
+ * whose position has no page (beyond table_width, a page number outside the pool, a
+ * negative length) is left out; all else in the pools stays as it was.  Two tokens
+ * of one call must not share a slot (a page that two sequences write, a sequence
+ * twice): either's values may end up there.  Returns 0/-1. */
+int adaptq_paged_append_device(adaptq_paged_t cache, const void *d_k, const void *d_v,
+                               int n_tokens, size_t k_nb1, size_t k_nb2, size_t v_nb1,
+                               size_t v_nb2, const int *d_table, int table_width,
+                               int table_stride, const int *d_lengths, int n_seqs,
+                               const int *d_offsets, void *stream);
+
+/* attend: one query per sequence and query head, d_q and d_out [n_seqs][n_q_heads]
+ * [dim]; query heads h * g to h * g + g - 1 (g = n_q_heads / n_heads) attend over key
+ * head h's tokens [max(0, n - window), n), n = d_lengths[b]; window 0: all.  The query
+ * is the token n - 1 (its rotation).  scale: of the scores, 0 = 1 / sqrt(dim).
+ * Products and sums in fp32 or closer, rounded once.  Tokens without a page are left
+ * out, as above; a sequence with no tokens gets zeros.  The order of the sums depends
+ * on the lengths alone, so equal calls give equal bits.  d_out may not overlap d_q.
+ * Returns 0/-1. */
+int adaptq_paged_attend_device(adaptq_paged_t cache, const void *d_q, void *d_out, int n_q_heads,
+                               size_t q_nb1, size_t q_nb2, size_t out_nb1, size_t out_nb2,
+                               const int *d_table, int table_width, int table_stride,
+                               const int *d_lengths, int n_seqs, float scale, int window,
+                               void *stream);
+
+/* step: append with one token a sequence, then attend over d_lengths[b] + 1 tokens;
+ * same pages and outputs as those two calls.  A sequence of negative length is empty
+ * and stays so. */
+int adaptq_paged_step_device(adaptq_paged_t cache, const void *d_k, const void *d_v, size_t k_nb1,
+                             size_t k_nb2, size_t v_nb1, size_t v_nb2, const void *d_q,
+                             void *d_out, int n_q_heads, size_t q_nb1, size_t q_nb2,
+                             size_t out_nb1, size_t out_nb2, const int *d_table, int table_width,
+                             int table_stride, const int *d_lengths, int n_seqs, float scale,
+                             int window, void *stream);
 
 #ifdef __cplusplus
 }
