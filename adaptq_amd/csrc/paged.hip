@@ -1,7 +1,5 @@
-// paged.hip -- a cache of exact key and value rows in pages: rows written into the
-// pages of their sequences, keys rotated on the way, and the attention of one new
-// token per sequence.
-#include <float.h>
+// paged.hip -- rows written into the pages of their sequences, keys rotated on the
+// way.
 #include <limits.h>
 
 #include "paged.hpp"
@@ -13,10 +11,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ RotaryShape rotary_shape(const RotaryTable &t) {
-  return {t.steps, t.pairs, t.interleaved, t.amplitude};
-}
-
 // Page of token `at` of sequence `seq`, or -1 where the table has none for it.
 __device__ __forceinline__ int page_of(const PagedSeqs &q, const PagedShape &p, int seq, int at) {
   const int col = at / p.page_size;
@@ -25,8 +19,6 @@ __device__ __forceinline__ int page_of(const PagedSeqs &q, const PagedShape &p, 
   return page >= 0 && page < p.n_pages ? page : -1;
 }
 
-// ---- append ----
-//
 // A block takes a few tokens; their sequence, position and page, and the cosines
 // and sines of their pairs, go to LDS once for every head.  A thread takes one item
 // of a (token, head): a chunk of N pairs of the key, N channels of it that pass
@@ -124,88 +116,6 @@ hipError_t append_type(const PagedShape &p, const PagedSeqs &q, const PagedAppen
   return append_n<T, 1>(p, q, a, s);
 }
 
-// ---- attention ----
-//
-// o = sum_t p_t v_t / sum_t p_t, p_t = exp(scale <q, k_t> - max), over the tokens
-// [lo, n) of a sequence.  A block takes one (sequence, query head); its waves take
-// every fourth token with a running maximum and sum each, and join in LDS.
-
-constexpr int kMaxDim = 256;
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attend_kernel(PagedShape p, PagedSeqs q,
-                                                          PagedAttend a) {
-  constexpr int E = kMaxDim / 64;
-  __shared__ float s_q[kMaxDim];
-  __shared__ float s_acc[4][kMaxDim], s_m[4], s_l[4];
-  const int seq = blockIdx.x / a.q_heads, qh = blockIdx.x % a.q_heads;
-  const int head = qh / (a.q_heads / p.n_heads);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t cap = (int64_t)q.width * p.page_size;
-  const int64_t held = q.lengths[seq] < 0 ? 0 : (int64_t)q.lengths[seq] + a.extra;
-  const int at_q = (int)(held - 1);  // the query's position
-  const int n = (int)min(min(held, cap), (int64_t)INT_MAX);
-  const int lo = a.window > 0 && n > a.window ? n - a.window : 0;
-  const T *qr = reinterpret_cast<const T *>(static_cast<const char *>(a.q) +
-                                            (size_t)seq * a.q_nb[1] + (size_t)qh * a.q_nb[0]);
-  const RotaryTable &r = p.rotary;
-  for (int i = tid; i < r.pairs; i += kThreads) {
-    const float2 cs = rotary_cos_sin(r.steps[i], at_q, r.amplitude);
-    const int2 at = chunk_at<1>(i, r.pairs, r.interleaved);
-    const float u = row_get(qr[at.x]), v = row_get(qr[at.y]);
-    s_q[at.x] = fmaf(u, cs.x, -(v * cs.y));
-    s_q[at.y] = fmaf(v, cs.x, u * cs.y);
-  }
-  for (int i = 2 * r.pairs + tid; i < p.dim; i += kThreads) s_q[i] = row_get(qr[i]);
-  __syncthreads();
-  float acc[E] = {}, m = -INFINITY, l = 0.0f;
-  for (int t = lo + wave; t < n; t += 4) {
-    const int page = page_of(q, p, seq, t);
-    if (page < 0) continue;
-    const int64_t row =
-        (((int64_t)page * p.n_heads + head) * p.page_size + t % p.page_size) * p.dim;
-    const T *k = static_cast<const T *>(p.k_pages) + row, *v = static_cast<const T *>(p.v_pages) + row;
-    float x = 0.0f;
-    for (int i = lane; i < p.dim; i += 64) x = fmaf(row_get(k[i]), s_q[i], x);
-#pragma unroll
-    for (int k2 = 32; k2 >= 1; k2 >>= 1) x += __shfl_xor(x, k2, 64);
-    x *= a.scale;
-    const float top = fmaxf(fmaxf(m, x), -FLT_MAX);  // finite: a token was there
-    const float keep = expf(m - top), w = expf(x - top);
-    m = top;
-    l = l * keep + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = lane + 64 * e;
-      if (i < p.dim) acc[e] = fmaf(w, row_get(v[i]), acc[e] * keep);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_acc[wave][lane + 64 * e] = acc[e];
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_l[wave] = l;
-  }
-  __syncthreads();
-  float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  const bool none = top == -INFINITY;
-  if (none) top = 0.0f;
-  float w[4], sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    w[k] = expf(s_m[k] - top);
-    sum += w[k] * s_l[k];
-  }
-  T *out = reinterpret_cast<T *>(static_cast<char *>(a.out) + (size_t)seq * a.out_nb[1] +
-                                 (size_t)qh * a.out_nb[0]);
-  for (int i = tid; i < p.dim; i += kThreads) {
-    float y = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) y = fmaf(w[k], s_acc[k][i], y);
-    row_put(out[i], none ? 0.0f : y / sum);
-  }
-}
-
 }  // namespace
 
 hipError_t launch_paged_append(const PagedShape &p, const PagedSeqs &q, const PagedAppend &a,
@@ -215,19 +125,6 @@ hipError_t launch_paged_append(const PagedShape &p, const PagedSeqs &q, const Pa
     case IoType::F16: return append_type<_Float16>(p, q, a, s);
     default: return append_type<Bf16>(p, q, a, s);
   }
-}
-
-size_t paged_workspace_bytes(const PagedShape &) { return 0; }
-
-hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
-                               void *, hipStream_t s) {
-  const unsigned grid = (unsigned)q.n_seqs * a.q_heads;
-  switch (p.io) {
-    case IoType::F32: attend_kernel<float><<<grid, kThreads, 0, s>>>(p, q, a); break;
-    case IoType::F16: attend_kernel<_Float16><<<grid, kThreads, 0, s>>>(p, q, a); break;
-    default: attend_kernel<Bf16><<<grid, kThreads, 0, s>>>(p, q, a); break;
-  }
-  return hipGetLastError();
 }
 
 }  // namespace aq

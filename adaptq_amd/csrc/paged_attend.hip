@@ -1,0 +1,682 @@
+// paged_attend.hip -- attention of one new token per sequence over its pages.
+//
+// For the g query heads of a key head and the tokens t of [lo, n):
+//   s_t = scale <q, k_t>,  o = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),
+// with m the running maximum, in one pass over the rows.  Bound: the rows' bytes
+// (2 * dim values a token and key head, used once by g heads), so everything else
+// stays out of the way of the loads:
+//
+// * A wave takes a unit of 32 tokens (16 in fp32) for up to 16 query heads.  Both
+//   products run on the matrix cores as 16 x 16 tiles straight from the registers
+//   that the rows were loaded into, with no LDS and no exchange of lanes:
+//   - S = K q^T: the operand K wants lane (row r, group g) to hold 8 channels of
+//     token r, which is one 16-byte load; which 8 is free as long as q agrees.
+//   - O^T = V^T P^T: P^T comes out of the first product in the layout that the
+//     second wants (lane = query head, its registers = tokens) if token t of the
+//     operand is the token whose score sits there; so group g loads the rows of
+//     tokens 4g..4g+3 of each 16, 8 channels a lane, whole rows a load, and
+//     transposes the 8 x 8 values of its tokens and channels in its own registers.
+//   Both tiles have the query head in the lane, so the running maximum, the sum and
+//   the rescaling are lane-local but for one maximum over the four groups.
+// * The rows of the next unit are loaded before this one's are used, and the page
+//   numbers of the one behind it before that.
+// * Work is cut evenly over the resident blocks whatever the lengths (paged_split.hpp).
+//
+// Precision: scores, statistics and sums in fp32.  Rotated queries and weights enter
+// the half-precision products as the sum of two numbers of that type, which leaves
+// 2^-16 of them (bf16) or 2^-20 (fp16), so the output's own rounding is the only one
+// of its size; fp32 rows use the fp32 matrix instructions.
+#include <float.h>
+
+#include <algorithm>
+
+#include "paged.hpp"
+#include "paged_split.hpp"
+#include "rotary.hpp"
+
+namespace aq {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 16;  // query heads of a segment
+constexpr int kMaxBlocks = 1024;
+constexpr int kBeyond = 1 << 30;  // an offset behind every buffer
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef const __attribute__((address_space(4))) int cint;  // uniform loads
+
+struct Args {
+  PagedShape p;
+  PagedSeqs q;
+  PagedAttend a;
+  float scale2;        // of the scores, to base 2
+  int group, q_tiles;  // query heads of a key head, and their tiles of 16
+  int segs;            // segments of a sequence
+  int64_t cap;         // tokens that the table has columns for
+  uint64_t page_mul;   // blocks of 16 tokens -> pages: x * page_mul >> page_shift
+  int page_shift, page_blocks, row_bytes;
+  bool out_vec;
+  float *partial;
+  int *counters;
+};
+
+// What differs between the types of the rows.
+template <typename T, int DP>
+struct Kind {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kUnit = kHalf ? 32 : 16;
+  static constexpr int kSubs = kUnit / 16;
+  static constexpr int kVec = 16 / (int)sizeof(T);  // values of a K load
+  static constexpr int kChunks = DP / (4 * kVec);   // K loads of a row
+  // channels of a V load: a row over 16 lanes, at most 16 bytes each
+  static constexpr int kVVec = DP / 16 < kVec ? DP / 16 : kVec;
+  static constexpr int kVChunks = DP / (16 * kVVec);
+  static constexpr int kVRows = kUnit / 4;  // rows of V that a lane loads
+};
+
+template <int BYTES>
+struct VecOf {
+  typedef u32x4 type;
+};
+template <>
+struct VecOf<8> {
+  typedef u32x2 type;
+};
+
+// A unit's rows as they were loaded.
+template <typename T, int DP>
+struct Rows {
+  typedef Kind<T, DP> K;
+  typedef typename VecOf<K::kVVec * sizeof(T)>::type V;
+  u32x4 k[K::kSubs][K::kChunks];
+  V v[K::kVRows][K::kVChunks];
+};
+
+// Where a unit's blocks of 16 tokens lie: the page (-1: nowhere) and the first slot.
+template <int SUBS>
+struct Where {
+  int page[SUBS], slot[SUBS];
+};
+
+__device__ __forceinline__ float cross_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const uint32_t a = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const float y = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const uint32_t b = __float_as_uint(y);
+  const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+__device__ __forceinline__ float cross_sum(float x) {
+  const uint32_t a = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const float y = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const uint32_t b = __float_as_uint(y);
+  const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, Bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Two values as hi + lo: hi the largest number of the type that is below (in magnitude),
+// lo the rest, rounded.  lo is never 0 for a value that is not, and has its sign: a product
+// with an infinity stays that infinity.
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, _Float16) {
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  const float a = __uint_as_float(__float_as_uint(x) - (x != 0.0f));
+  const float b = __uint_as_float(__float_as_uint(y) - (y != 0.0f));
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  const v2 h = __builtin_bit_cast(v2, hi);
+  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
+}
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, Bf16) {
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  const uint32_t a = __float_as_uint(x) - (x != 0.0f), b = __float_as_uint(y) - (y != 0.0f);
+  hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  lo = __builtin_bit_cast(uint32_t, v2{(__bf16)(x - __uint_as_float(a & 0xFFFF0000u)),
+                                       (__bf16)(y - __uint_as_float(b & 0xFFFF0000u))});
+}
+
+template <typename T>
+__device__ __forceinline__ void split8(const float *x, u32x4 &hi, u32x4 &lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h, l;
+    split2(x[2 * i], x[2 * i + 1], h, l, T());
+    hi[i] = h;
+    lo[i] = l;
+  }
+}
+
+// A wave's running state over its units.
+template <int DP>
+struct State {
+  float m, l;        // of query head lane & 15; l of this lane's tokens only
+  f32x4 acc[DP / 16];
+};
+
+// DP: dim padded to 64, 128 or 256; EXACT: dim is DP.
+template <typename T, int DP, bool EXACT>
+struct Attend {
+  typedef Kind<T, DP> K;
+  typedef aq::Rows<T, DP> Rows;
+  typedef aq::Where<K::kSubs> Where;
+  static constexpr int kQ = K::kHalf ? K::kChunks : DP / 4;  // operand registers of q
+  // fp16 weights are taken times 2^15 (so is their sum): small ones stay normal numbers
+  static constexpr float kLift = __is_same(T, _Float16) ? 15.0f : 0.0f;
+
+  // this wave's view of a segment
+  const Args &g;
+  const int lane, row16, group4;
+  int k_off[EXACT ? 1 : K::kChunks], v_off[EXACT ? 1 : 4 * K::kVChunks];  // bytes in 16 rows
+  TokenSpan span;
+  const int *table;
+  int head, u_end;
+  u32x4 qh[K::kHalf ? kQ : 1], ql[K::kHalf ? kQ : 1];
+  float qf[K::kHalf ? 1 : kQ];
+
+  __device__ Attend(const Args &args, int lane_)
+      : g(args), lane(lane_), row16(lane_ & 15), group4(lane_ >> 4) {
+    const int row = g.row_bytes, size = (int)sizeof(T);
+    if (EXACT) {  // the rest of the offsets are constants
+      k_off[0] = row16 * DP * size + K::kVec * group4 * size;
+      v_off[0] = 4 * group4 * DP * size + K::kVVec * row16 * size;
+    } else {  // channels past dim lie beyond every buffer: they load as 0
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c)
+        k_off[c] = k_channel(c) < g.p.dim ? row16 * row + k_channel(c) * size : kBeyond;
+#pragma unroll
+      for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int d = K::kVVec * (row16 + 16 * c);
+          v_off[4 * c + j] = d < g.p.dim ? (4 * group4 + j) * row + d * size : kBeyond;
+        }
+    }
+  }
+
+  __device__ int k_channel(int chunk) const {  // first of the 8 (4) channels of a K load
+    return K::kVec * (group4 + 4 * chunk);
+  }
+
+  __device__ Where locate(int unit) const {
+    Where w;
+#pragma unroll
+    for (int s = 0; s < K::kSubs; ++s) {
+      const int b = unit * K::kSubs + s;  // block of 16 tokens
+      w.page[s] = -1;
+      w.slot[s] = 0;
+      if (unit < u_end && b * 16 < span.n) {
+        const int col = (int)((uint64_t)(uint32_t)b * g.page_mul >> g.page_shift);
+        const int page = ((cint *)(uint64_t)table)[col];
+        w.page[s] = page < g.p.n_pages ? page : -1;
+        w.slot[s] = (b - col * g.page_blocks) * 16;
+      }
+    }
+    return w;
+  }
+
+  // Rows of 16 tokens as a buffer that ends behind the last token (and is empty where
+  // there is no page): whatever lies behind it loads as 0, without a branch.
+  __device__ __amdgpu_buffer_rsrc_t rows16(const void *pool, const Where &w, int s, int t0) const {
+    const int64_t page = max(w.page[s], 0);
+    const char *at = static_cast<const char *>(pool) +
+                     ((page * g.p.n_heads + head) * g.p.page_size + w.slot[s]) * g.row_bytes;
+    const int rows = w.page[s] < 0 ? 0 : max(0, min(16, span.n - (t0 + 16 * s)));
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, rows * g.row_bytes,
+                                             0x00020000);
+  }
+
+  __device__ void load(Rows &r, const Where &w, int unit) const {
+    const int t0 = unit * K::kUnit;
+#pragma unroll
+    for (int s = 0; s < K::kSubs; ++s) {
+      const auto k = rows16(g.p.k_pages, w, s, t0);
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c)
+        r.k[s][c] = __builtin_amdgcn_raw_buffer_load_b128(
+            k, EXACT ? k_off[0] + c * 64 : k_off[EXACT ? 0 : c], 0, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < K::kSubs; ++s) {
+      const auto v = rows16(g.p.v_pages, w, s, t0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < K::kVChunks; ++c) {
+          constexpr int size = (int)sizeof(T);
+          const int off = EXACT ? v_off[0] + (j * DP + 16 * c * K::kVVec) * size
+                                : v_off[EXACT ? 0 : 4 * c + j];
+          if constexpr (K::kVVec * sizeof(T) == 8)
+            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b64(v, off, 0, 0);
+          else
+            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b128(v, off, 0, 0);
+        }
+    }
+  }
+
+  __device__ void use(State<DP> &st, Rows &r, const Where &w, int unit) const {
+    const int t0 = unit * K::kUnit;
+    bool full = t0 >= span.lo && t0 + K::kUnit <= span.n, any = false;
+#pragma unroll
+    for (int s = 0; s < K::kSubs; ++s) {
+      full = full && w.page[s] >= 0;
+      any = any || (w.page[s] >= 0 && t0 + 16 * s + 16 > span.lo);
+    }
+    if (!any) return;  // (uniform)
+
+    f32x4 s[K::kSubs];
+#pragma unroll
+    for (int i = 0; i < K::kSubs; ++i) s[i] = f32x4{0, 0, 0, 0};
+    if constexpr (K::kHalf) {
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < K::kSubs; ++i) s[i] = mfma(r.k[i][c], qh[c], s[i], T());
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < K::kSubs; ++i) s[i] = mfma(r.k[i][c], ql[c], s[i], T());
+    } else {
+      f32x4 s2 = s[0];
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(r.k[0][c][i]), qf[4 * c + i],
+                                                      s[0], 0, 0, 0);
+          s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(r.k[0][c][i + 1]),
+                                                    qf[4 * c + i + 1], s2, 0, 0, 0);
+        }
+      s[0] += s2;
+    }
+#pragma unroll
+    for (int i = 0; i < K::kSubs; ++i) s[i] *= g.scale2;
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < K::kSubs; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = t0 + 16 * i + 4 * group4 + j;
+          if (!(w.page[i] >= 0 && t >= span.lo && t < span.n)) s[i][j] = -INFINITY;
+          // rows behind the last token were loaded as 0; those before the window are there
+          if (t < span.lo)
+#pragma unroll
+            for (int c = 0; c < K::kVChunks; ++c) r.v[4 * i + j][c] = typename Rows::V(0u);
+        }
+    }
+    // at least one token is here, so the maximum is finite from now on
+    float top = fmaxf(st.m, -FLT_MAX);
+    {
+      float x = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < K::kSubs; ++i)
+        x = fmaxf(x, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
+      top = fmaxf(top, cross_max(x));
+    }
+    if (__any(top > st.m)) {
+      const float keep = __builtin_amdgcn_exp2f(st.m - top);
+      st.l *= keep;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) st.acc[i] *= keep;
+      st.m = top;
+    }
+    float p[K::kUnit / 4];
+#pragma unroll
+    for (int i = 0; i < K::kSubs; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[4 * i + j] = __builtin_amdgcn_exp2f(s[i][j] - (top - kLift));
+        st.l += p[4 * i + j];
+      }
+    if constexpr (K::kHalf) {
+      u32x4 ph, pl;
+      split8<T>(p, ph, pl);
+#pragma unroll
+      for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+        for (int w2 = 0; w2 < K::kVVec / 2; ++w2) {
+          u32x4 a, b;  // the 8 tokens of channels 2 w2 and 2 w2 + 1
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            a[x] = __builtin_amdgcn_perm(r.v[2 * x + 1][c][w2], r.v[2 * x][c][w2], 0x05040100u);
+            b[x] = __builtin_amdgcn_perm(r.v[2 * x + 1][c][w2], r.v[2 * x][c][w2], 0x07060302u);
+          }
+          f32x4 &y = st.acc[c * K::kVVec + 2 * w2], &z = st.acc[c * K::kVVec + 2 * w2 + 1];
+          y = mfma(a, ph, y, T());
+          z = mfma(b, ph, z, T());
+          y = mfma(a, pl, y, T());
+          z = mfma(b, pl, z, T());
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st.acc[4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                __uint_as_float(r.v[j][c][i]), p[j], st.acc[4 * c + i], 0, 0, 0);
+    }
+  }
+};
+
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// First unit and segment base of the sequence that unit `at` of the whole belongs to.
+// All lanes; lengths of 64 sequences a round.
+struct Found {
+  int seq;
+  int64_t base;
+};
+
+__device__ __forceinline__ int64_t units_of(const Args &g, int seq, int unit) {
+  if (seq >= g.q.n_seqs) return 0;
+  return (int64_t)token_span(g.q.lengths[seq], g.a.extra, g.a.window, g.cap, unit).units * g.segs;
+}
+
+__device__ __forceinline__ int64_t total_units(const Args &g, int lane, int unit) {
+  int64_t x = 0;
+  for (int b = lane; b < g.q.n_seqs; b += 64) x += units_of(g, b, unit);
+  if (g.q.n_seqs == 1) return uniform(x);
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) x += __shfl_xor(x, k, 64);
+  return uniform(x);
+}
+
+__device__ __forceinline__ Found find_unit(const Args &g, int lane, int unit, int64_t at) {
+  if (g.q.n_seqs == 1) return {0, 0};
+  int64_t base = 0;
+  for (int b0 = 0;; b0 += 64) {
+    int64_t x = units_of(g, b0 + lane, unit), sum = x;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const int64_t y = __shfl_up(sum, k, 64);
+      if (lane >= k) sum += y;
+    }
+    const uint64_t past = __ballot(base + sum > at);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      return {b0 + l, base + __shfl(sum - x, l, 64)};
+    }
+    base += __shfl(sum, 63, 64);
+  }
+}
+
+template <typename T, int DP, bool EXACT>
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(const Args g) {
+  typedef Kind<T, DP> K;
+  typedef Attend<T, DP, EXACT> A;
+  constexpr int S = DP + 4;
+  __shared__ __align__(16) float s_acc[kWaves][kTile][S];  // first: the queries, in [0]
+  __shared__ float s_m[kWaves][kTile], s_l[kWaves][kTile];
+  __shared__ float2 s_cs[DP / 2];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int dim = g.p.dim;
+
+  const int64_t total = total_units(g, lane, K::kUnit);
+  const int64_t share = share_of(total, (int)gridDim.x, kWaves);
+  int64_t at = blockIdx.x * share;
+  const int64_t end = min(at + share, total);
+  if (at >= end) return;
+  Found f = find_unit(g, lane, K::kUnit, at);
+  int seq = __builtin_amdgcn_readfirstlane(f.seq);
+  int64_t base = uniform(f.base);
+  int turned = -1;  // the sequence whose query position s_cs holds
+
+  A w(g, lane);
+  while (at < end) {
+    const int length = __builtin_amdgcn_readfirstlane(g.q.lengths[seq]);
+    w.span = token_span(length, g.a.extra, g.a.window, g.cap, K::kUnit);
+    const Piece pc = piece_at(at, end, base, w.span.units, share);
+    const int head = pc.seg / g.q_tiles, q0 = (pc.seg - head * g.q_tiles) * kTile;
+    const int rows = min(kTile, g.group - q0);
+    w.head = head;
+    w.table = g.q.table + (int64_t)seq * g.q.stride;
+    w.u_end = w.span.first_unit + pc.u1;
+    int u = w.span.first_unit + pc.u0 + wave;
+
+    typename A::Rows r0, r1;
+    typename A::Where w0 = w.locate(u), w1 = w.locate(u + kWaves);
+    w.load(r0, w0, u);
+
+    // the queries, rotated, into LDS and from there into operands
+    const RotaryTable &rt = g.p.rotary;
+    const int64_t qh0 = (int64_t)head * g.group + q0;
+    const char *q_at = static_cast<const char *>(g.a.q) + (int64_t)seq * g.a.q_nb[1];
+    if (rt.pairs && turned != seq) {
+      for (int i = tid; i < rt.pairs; i += kThreads)
+        s_cs[i] = rotary_cos_sin(rt.steps[i], length < 0 ? 0 : length + g.a.extra - 1, rt.amplitude);
+      turned = seq;
+      __syncthreads();
+    }
+    for (int i = tid; i < kTile * DP; i += kThreads) {
+      const int row = i / DP, d = i % DP;
+      float x = 0.0f;
+      if (row < rows && d < dim) {
+        const T *q = reinterpret_cast<const T *>(q_at + (qh0 + row) * (int64_t)g.a.q_nb[0]);
+        x = row_get(q[d]);
+        if (d < 2 * rt.pairs) {
+          const bool second = rt.interleaved ? d & 1 : d >= rt.pairs;
+          const int pair = rt.interleaved ? d >> 1 : second ? d - rt.pairs : d;
+          const int other = rt.interleaved ? d ^ 1 : second ? d - rt.pairs : d + rt.pairs;
+          const float2 cs = s_cs[pair];
+          const float y = row_get(q[other]);
+          x = second ? fmaf(x, cs.x, y * cs.y) : fmaf(x, cs.x, -(y * cs.y));
+        }
+      }
+      s_acc[0][row][d] = x;
+    }
+    __syncthreads();
+    if constexpr (K::kHalf) {
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = s_acc[0][w.row16][w.k_channel(c) + i];
+        split8<T>(x, w.qh[c], w.ql[c]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < K::kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.qf[4 * c + i] = s_acc[0][w.row16][w.k_channel(c) + i];
+    }
+    __syncthreads();  // before s_acc is written again
+
+    State<DP> st;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) st.acc[i] = f32x4{0, 0, 0, 0};
+    while (u < w.u_end) {
+      w.load(r1, w1, u + kWaves);
+      typename A::Where next = w.locate(u + 2 * kWaves);
+      w.use(st, r0, w0, u);
+      u += kWaves;
+      if (u >= w.u_end) break;
+      w0 = next;
+      w.load(r0, w0, u + kWaves);
+      next = w.locate(u + 2 * kWaves);
+      w.use(st, r1, w1, u);
+      u += kWaves;
+      w1 = next;
+    }
+
+    // the waves' parts together
+    st.l = cross_sum(st.l);
+    if (w.row16 < rows) {
+#pragma unroll
+      for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d = K::kVVec * (16 * c + 4 * w.group4 + r);
+#pragma unroll
+          for (int i = 0; i < K::kVVec; ++i)
+            s_acc[wave][w.row16][d + i] = st.acc[c * K::kVVec + i][r];
+        }
+      if (w.group4 == 0) {
+        s_m[wave][w.row16] = st.m;
+        s_l[wave][w.row16] = st.l;
+      }
+    }
+    __syncthreads();
+    char *o_at = static_cast<char *>(g.a.out) + (int64_t)seq * g.a.out_nb[1];
+    auto put = [&](int row, int d, f32x4 y) {
+      T *o = reinterpret_cast<T *>(o_at + (qh0 + row) * (int64_t)g.a.out_nb[0]) + d;
+      if (d >= dim) return;
+      RowVec<T, 4> v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) row_put(v.x[i], y[i]);
+      if (g.out_vec) {
+        *reinterpret_cast<RowVec<T, 4> *>(o) = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = v.x[i];
+      }
+    };
+    constexpr int kPart = kTile * (DP + 2);  // floats of a partial result
+    for (int i = tid; i < rows * (DP / 4); i += kThreads) {
+      const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) m = fmaxf(m, s_m[k][row]);
+      f32x4 y = {0, 0, 0, 0};
+      if (m != -INFINITY) {
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+          const float e = __builtin_amdgcn_exp2f(s_m[k][row] - m);
+          l = fmaf(e, s_l[k][row], l);
+          y += e * *reinterpret_cast<const f32x4 *>(&s_acc[k][row][d]);
+        }
+      }
+      if (pc.whole) {
+        put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
+      } else {
+        float *part = g.partial + (int64_t)(2 * blockIdx.x + pc.slot) * kPart;
+        *reinterpret_cast<f32x4 *>(part + row * DP + d) = y;
+        if (d == 0) {
+          part[kTile * DP + row] = m;
+          part[kTile * DP + kTile + row] = l;
+        }
+      }
+    }
+    if (!pc.whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0)
+        s_last = atomicAdd(g.counters + pc.first, 1) == pc.pieces - 1;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int i = tid; i < rows * (DP / 4); i += kThreads) {
+          const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+          // the first piece began the segment (slot 1), the others go on with it
+          const float *p0 = g.partial + (2 * pc.first + 1) * kPart;
+          float m = p0[kTile * DP + row];
+          for (int k = 1; k < pc.pieces; ++k)
+            m = fmaxf(m, p0[(int64_t)(2 * k - 1) * kPart + kTile * DP + row]);
+          float l = 0.0f;
+          f32x4 y = {0, 0, 0, 0};
+          if (m != -INFINITY)
+            for (int k = 0; k < pc.pieces; ++k) {
+              const float *part = p0 + (int64_t)(k ? 2 * k - 1 : 0) * kPart;
+              const float e = __builtin_amdgcn_exp2f(part[kTile * DP + row] - m);
+              l = fmaf(e, part[kTile * DP + kTile + row], l);
+              y += e * *reinterpret_cast<const f32x4 *>(part + row * DP + d);
+            }
+          put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
+        }
+        if (tid == 0) g.counters[pc.first] = 0;  // for the next call
+      }
+    }
+    __syncthreads();
+    at += pc.u1 - pc.u0;
+    if (at - base == (int64_t)w.span.units * g.segs) {
+      base = at;
+      ++seq;
+    }
+  }
+}
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <typename T, int DP>
+hipError_t launch(const Args &g, hipStream_t s) {
+  // as many blocks as the card holds at once, or as there may be work for
+  constexpr int unit = Kind<T, DP>::kUnit;
+  const int64_t longest = token_span(0x7FFFFFFF, 0, g.a.window, g.cap, unit).units + 1;
+  const int64_t most = g.q.n_seqs * (int64_t)g.segs * longest;
+  const int blocks = (int)std::min((most + kWaves - 1) / kWaves, (int64_t)(DP == 256 ? 256 : 512));
+  if (g.p.dim == DP) attend_kernel<T, DP, true><<<blocks, kThreads, 0, s>>>(g);
+  else attend_kernel<T, DP, false><<<blocks, kThreads, 0, s>>>(g);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_type(const Args &g, hipStream_t s) {
+  switch (padded_dim(g.p.dim)) {
+    case 64: return launch<T, 64>(g, s);
+    case 128: return launch<T, 128>(g, s);
+    default: return launch<T, 256>(g, s);
+  }
+}
+
+}  // namespace
+
+size_t paged_workspace_bytes(const PagedShape &p) {
+  return kMaxBlocks * (2 * sizeof(float) * kTile * (padded_dim(p.dim) + 2) + sizeof(int));
+}
+
+hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
+                               void *workspace, hipStream_t s) {
+  Args g{};
+  g.p = p;
+  g.q = q;
+  g.a = a;
+  const float log2e = 1.44269504088896340736f;
+  g.scale2 = a.scale * log2e;
+  g.group = a.q_heads / p.n_heads;
+  g.q_tiles = (g.group + kTile - 1) / kTile;
+  g.segs = p.n_heads * g.q_tiles;
+  g.cap = (int64_t)q.width * p.page_size;
+  // x / page_blocks for x < 2^27: the multiplier is rounded up by less than page_blocks
+  // parts of 2^page_shift, so the quotient is off by less than 2^27 / 2^page_shift * ... < 1
+  // part of page_blocks
+  g.page_blocks = p.page_size / 16;
+  g.row_bytes = p.dim * (p.io == IoType::F32 ? 4 : 2);
+  int bits = 0;
+  while ((1 << bits) < g.page_blocks) ++bits;
+  g.page_shift = 27 + bits;
+  g.page_mul = (((uint64_t)1 << g.page_shift) + g.page_blocks - 1) / g.page_blocks;
+  size_t x = reinterpret_cast<uintptr_t>(a.out) | a.out_nb[0] | a.out_nb[1];
+  g.out_vec = x % (p.io == IoType::F32 ? 16 : 8) == 0;
+  g.counters = static_cast<int *>(workspace);
+  g.partial = reinterpret_cast<float *>(g.counters + kMaxBlocks);
+  switch (p.io) {
+    case IoType::F32: return launch_type<float>(g, s);
+    case IoType::F16: return launch_type<_Float16>(g, s);
+    default: return launch_type<Bf16>(g, s);
+  }
+}
+
+}  // namespace aq

@@ -1,0 +1,104 @@
+// The cut of the paged attention's work, on the CPU: every unit of every segment is
+// in exactly one piece, a cut segment's pieces are those its blocks count and use
+// different slots, and token spans are what window, capacity and lengths leave.
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <set>
+#include <tuple>
+#include <vector>
+
+#include "../../adaptq_amd/csrc/paged_split.hpp"
+
+using namespace aq;
+
+static void fail(const char *what) {
+  std::fprintf(stderr, "%s\n", what);
+  std::exit(1);
+}
+
+static void check_span(int length, int extra, int window, int64_t cap, int unit) {
+  const TokenSpan s = token_span(length, extra, window, cap, unit);
+  const int64_t held = length < 0 ? 0 : (int64_t)length + extra;
+  int64_t n = held < cap ? held : cap;
+  if (n > 0x7FFFFFE0) n = 0x7FFFFFE0;
+  int64_t lo = window > 0 && held > window ? held - window : 0;
+  if (lo > n) lo = n;
+  if (s.n != n || s.lo != lo || s.units < 1) fail("span");
+  if (lo < n) {
+    if ((int64_t)s.first_unit * unit > lo) fail("span starts late");
+    if ((int64_t)(s.first_unit + 1) * unit <= lo) fail("span starts early");
+    if ((int64_t)(s.first_unit + s.units) * unit < n) fail("span ends early");
+    if ((int64_t)(s.first_unit + s.units - 1) * unit >= n) fail("span ends late");
+  }
+}
+
+static void check_cut(const std::vector<int> &units, int segs, int blocks, int waves) {
+  int64_t total = 0;
+  std::vector<int64_t> base;
+  for (int u : units) {
+    base.push_back(total);
+    total += (int64_t)u * segs;
+  }
+  const int64_t share = share_of(total, blocks, waves);
+  if (share % waves || share * blocks < total) fail("share");
+  std::map<std::pair<int, int>, std::vector<char>> seen;     // (sequence, segment) -> units
+  std::map<std::pair<int, int>, int> pieces, expected;
+  std::map<std::pair<int, int>, int64_t> firsts;
+  std::set<std::pair<int64_t, int>> slots;
+  std::set<int64_t> counters;
+  for (int64_t b = 0; b < blocks; ++b) {
+    int64_t at = b * share, end = at + share < total ? at + share : total;
+    size_t q = 0;
+    while (at < end) {
+      while (q + 1 < base.size() && base[q + 1] <= at) ++q;
+      const Piece p = piece_at(at, end, base[q], units[q], share);
+      if (p.seg < 0 || p.seg >= segs || p.u0 < 0 || p.u1 <= p.u0 || p.u1 > units[q]) fail("piece");
+      const auto key = std::make_pair((int)q, p.seg);
+      auto &v = seen[key];
+      v.resize(units[q]);
+      for (int u = p.u0; u < p.u1; ++u)
+        if (v[u]++) fail("unit twice");
+      if (p.whole != (p.pieces == 1)) fail("whole");
+      if (!p.whole) {
+        if (!slots.insert({b, p.slot}).second) fail("slot twice");
+        ++pieces[key];
+        expected[key] = p.pieces;
+        if (pieces[key] == 1) {
+          firsts[key] = p.first;
+          if (p.first != b || p.slot != 1 || !counters.insert(b).second) fail("first");
+        } else {
+          if (firsts[key] != p.first || p.slot != 0) fail("later piece");
+          if (b != p.first + pieces[key] - 1) fail("pieces are consecutive blocks");
+        }
+      }
+      at += p.u1 - p.u0;
+    }
+  }
+  for (size_t q = 0; q < units.size(); ++q)
+    for (int s = 0; s < segs; ++s) {
+      const auto key = std::make_pair((int)q, s);
+      if ((int)seen[key].size() != units[q]) fail("segment missing");
+      for (char c : seen[key])
+        if (c != 1) fail("unit missing");
+      if (pieces[key] != expected[key]) fail("piece count");
+    }
+}
+
+int main() {
+  const int edge[] = {-2147483647 - 1, -1, 0, 1, 15, 16, 17, 31, 32, 33, 1000, 2147483615, 2147483647};
+  for (int n : edge)
+    for (int extra : {0, 1})
+      for (int window : {0, 1, 16, 31, 32, 33, 500, 2147483647})
+        for (int64_t cap : {(int64_t)0, (int64_t)16, (int64_t)48, (int64_t)1008, (int64_t)1 << 40})
+          for (int unit : {16, 32}) check_span(n, extra, window, cap, unit);
+  std::mt19937 g(1);
+  for (int i = 0; i < 3000; ++i) {
+    std::vector<int> units(1 + g() % 20);
+    const int top = 1 << (g() % 9);
+    for (int &u : units) u = 1 + g() % top;
+    check_cut(units, 1 + g() % 9, 1 + g() % 300, 1 << (g() % 4));
+  }
+  std::puts("ok");
+}

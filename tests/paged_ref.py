@@ -85,8 +85,10 @@ def attend(q, k, v, scale, dtype, q_err=0.0):
     the rotated query's own error; that is a relative error of 2 d in a weight over its sum.
     The exponential, the product with v, the quotient and the joins of the parts round a few
     times each (32), the sum over n tokens as a random walk (4 sqrt(n)).  Weights and queries
-    enter the matrix cores as two half-precision numbers: 2^-17 of their size (bf16).  Then
-    the rounding to the type."""
+    enter the matrix cores as two half-precision numbers, the largest below and the rest: the
+    rest is up to 2^-7 of it (bf16) and rounds by 2^-9 of that, 2^-16 of the value; fp16 2^-10
+    and 2^-10, 2^-20 (the rounding of a rest below its normal numbers is 2^-40 of the largest
+    weight, nothing).  Then the rounding to the type."""
     q, k, v = q.double(), k.double(), v.double()
     n, d = k.shape[1], k.shape[2]
     if n == 0:
@@ -96,7 +98,7 @@ def attend(q, k, v, scale, dtype, q_err=0.0):
     w = torch.softmax(s, -1)
     out = torch.matmul(w, v)
     size = torch.matmul(q.abs(), k.abs().transpose(1, 2)) * abs(scale)
-    split = 0.0 if dtype == torch.float32 else 2.0 ** -17
+    split = {torch.float32: 0.0, torch.float16: 2.0 ** -20, torch.bfloat16: 2.0 ** -16}[dtype]
     ds = size * (U32 * (8 + 4 * math.sqrt(d)) + split) + 16 * U32 * s.abs()
     if not isinstance(q_err, float):
         ds = ds + torch.matmul(q_err, k.abs().transpose(1, 2)) * abs(scale)
