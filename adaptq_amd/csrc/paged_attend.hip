@@ -42,6 +42,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kTile = 16;  // query heads of a segment
 constexpr int kMaxBlocks = 1024;
+constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
 constexpr int kBeyond = 1 << 30;  // an offset behind every buffer
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -161,6 +162,25 @@ __device__ __forceinline__ void split8(const float *x, u32x4 &hi, u32x4 &lo) {
   }
 }
 
+// Partial results pass between blocks that may sit on different dies, whose L2 caches do not
+// see each other's lines: they are stored past them and read past them (relaxed atomics of
+// the device's scope).  A fence of that scope instead writes back and drops a whole L2: it
+// cost tens of microseconds a call.
+__device__ __forceinline__ void put_shared(float *p, float x, float y) {
+  const uint64_t w = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), w, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_shared(const float *p) {
+  const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
+}
+// Every store of this wave has reached the memory that all dies see.
+__device__ __forceinline__ void stores_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 // A wave's running state over its units.
 template <int DP>
 struct State {
@@ -236,19 +256,23 @@ struct Attend {
     const char *at = static_cast<const char *>(pool) +
                      ((page * g.p.n_heads + head) * g.p.page_size + w.slot[s]) * g.row_bytes;
     const int rows = w.page[s] < 0 ? 0 : max(0, min(16, span.n - (t0 + 16 * s)));
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, rows * g.row_bytes,
-                                             0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char *>(at), 0, __builtin_amdgcn_readfirstlane(rows * g.row_bytes), 0x00020000);
   }
 
   __device__ void load(Rows &r, const Where &w, int unit) const {
     const int t0 = unit * K::kUnit;
+    // (opaque here, so that what is added stays part of the loads instead of taking a
+    // register each outside the loop)
+    int k0 = k_off[0], v0 = v_off[0];
+    asm volatile("" : "+v"(k0), "+v"(v0));
 #pragma unroll
     for (int s = 0; s < K::kSubs; ++s) {
       const auto k = rows16(g.p.k_pages, w, s, t0);
 #pragma unroll
       for (int c = 0; c < K::kChunks; ++c)
         r.k[s][c] = __builtin_amdgcn_raw_buffer_load_b128(
-            k, EXACT ? k_off[0] + c * 64 : k_off[EXACT ? 0 : c], 0, 0);
+            k, EXACT ? k0 + c * 64 : k_off[EXACT ? 0 : c], 0, 0);
     }
 #pragma unroll
     for (int s = 0; s < K::kSubs; ++s) {
@@ -258,7 +282,7 @@ struct Attend {
 #pragma unroll
         for (int c = 0; c < K::kVChunks; ++c) {
           constexpr int size = (int)sizeof(T);
-          const int off = EXACT ? v_off[0] + (j * DP + 16 * c * K::kVVec) * size
+          const int off = EXACT ? v0 + (j * DP + 16 * c * K::kVVec) * size
                                 : v_off[EXACT ? 0 : 4 * c + j];
           if constexpr (K::kVVec * sizeof(T) == 8)
             r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b64(v, off, 0, 0);
@@ -435,25 +459,32 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(con
 
   const int64_t total = total_units(g, lane, K::kUnit);
   const int64_t share = share_of(total, (int)gridDim.x, kWaves);
-  int64_t at = blockIdx.x * share;
-  const int64_t end = min(at + share, total);
-  if (at >= end) return;
+  const int64_t start = blockIdx.x * share, end = min(start + share, total);
+  if (start >= end) return;
+  int64_t at = start;
   Found f = find_unit(g, lane, K::kUnit, at);
   int seq = __builtin_amdgcn_readfirstlane(f.seq);
-  int64_t base = uniform(f.base);
+  const int64_t base = uniform(f.base);
   int turned = -1;  // the sequence whose query position s_cs holds
 
   A w(g, lane);
+  int seg = -1, u0 = 0;
   while (at < end) {
-    const int length = __builtin_amdgcn_readfirstlane(g.q.lengths[seq]);
+    const int length = ((cint *)(uint64_t)g.q.lengths)[seq];
     w.span = token_span(length, g.a.extra, g.a.window, g.cap, K::kUnit);
-    const Piece pc = piece_at(at, end, base, w.span.units, share);
-    const int head = pc.seg / g.q_tiles, q0 = (pc.seg - head * g.q_tiles) * kTile;
+    if (seg < 0) {
+      const Start s = start_at(at, base, w.span.units);
+      seg = __builtin_amdgcn_readfirstlane(s.seg);
+      u0 = __builtin_amdgcn_readfirstlane(s.u0);
+    }
+    const Piece pc = piece_at(blockIdx.x, start, end, at, u0, w.span.units, share);
+    const int head = __builtin_amdgcn_readfirstlane(seg / g.q_tiles);
+    const int q0 = (seg - head * g.q_tiles) * kTile;
     const int rows = min(kTile, g.group - q0);
     w.head = head;
     w.table = g.q.table + (int64_t)seq * g.q.stride;
     w.u_end = w.span.first_unit + pc.u1;
-    int u = w.span.first_unit + pc.u0 + wave;
+    int u = w.span.first_unit + u0 + wave;
 
     typename A::Rows r0, r1;
     typename A::Where w0 = w.locate(u), w1 = w.locate(u + kWaves);
@@ -573,46 +604,97 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(con
         put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
       } else {
         float *part = g.partial + (int64_t)(2 * blockIdx.x + pc.slot) * kPart;
-        *reinterpret_cast<f32x4 *>(part + row * DP + d) = y;
-        if (d == 0) {
-          part[kTile * DP + row] = m;
-          part[kTile * DP + kTile + row] = l;
-        }
+        put_shared(part + row * DP + d, y[0], y[1]);
+        put_shared(part + row * DP + d + 2, y[2], y[3]);
+        if (d == 0) put_shared(part + kTile * DP + 2 * row, m, l);
       }
     }
     if (!pc.whole) {
-      __threadfence();
+      stores_done();
       __syncthreads();
       if (tid == 0)
-        s_last = atomicAdd(g.counters + pc.first, 1) == pc.pieces - 1;
+        s_last = __hip_atomic_fetch_add(g.counters + pc.first, 1, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT) == pc.pieces - 1;
       __syncthreads();
       if (s_last) {
-        __threadfence();
-        for (int i = tid; i < rows * (DP / 4); i += kThreads) {
-          const int row = i / (DP / 4), d = i % (DP / 4) * 4;
-          // the first piece began the segment (slot 1), the others go on with it
-          const float *p0 = g.partial + (2 * pc.first + 1) * kPart;
-          float m = p0[kTile * DP + row];
-          for (int k = 1; k < pc.pieces; ++k)
-            m = fmaxf(m, p0[(int64_t)(2 * k - 1) * kPart + kTile * DP + row]);
-          float l = 0.0f;
+        // Threads beyond one per 4 channels of a row share the pieces; a thread has the loads
+        // of kBatch pieces in flight at once.
+        const float *p0 = g.partial + (2 * (int64_t)pc.first + 1) * kPart;  // the first one's slot 1
+        const int items = rows * (DP / 4), parts = max(1, kThreads / items);
+        for (int i0 = 0; i0 < items; i0 += kThreads) {
+          const int part = parts > 1 ? tid / items : 0;
+          const int item = parts > 1 ? tid - part * items : i0 + tid;
+          const bool mine = part < parts && item < items;
+          const int row = item / (DP / 4), d = item % (DP / 4) * 4;
+          float m = -INFINITY, l = 0.0f;
           f32x4 y = {0, 0, 0, 0};
-          if (m != -INFINITY)
-            for (int k = 0; k < pc.pieces; ++k) {
-              const float *part = p0 + (int64_t)(k ? 2 * k - 1 : 0) * kPart;
-              const float e = __builtin_amdgcn_exp2f(part[kTile * DP + row] - m);
-              l = fmaf(e, part[kTile * DP + kTile + row], l);
-              y += e * *reinterpret_cast<const f32x4 *>(part + row * DP + d);
+          if (mine)
+            for (int k0 = part; k0 < pc.pieces; k0 += parts * kBatch) {
+              float2 ml[kBatch], lo[kBatch], hi[kBatch];
+#pragma unroll
+              for (int j = 0; j < kBatch; ++j) {
+                const int k = min(k0 + j * parts, pc.pieces - 1);  // (the last again: no weight)
+                const float *from = p0 + (k ? 2 * k - 1 : 0) * (int64_t)kPart;
+                ml[j] = get_shared(from + kTile * DP + 2 * row);
+                lo[j] = get_shared(from + row * DP + d);
+                hi[j] = get_shared(from + row * DP + d + 2);
+              }
+              float top = m;
+#pragma unroll
+              for (int j = 0; j < kBatch; ++j) {
+                if (k0 + j * parts >= pc.pieces) ml[j].x = -INFINITY;
+                top = fmaxf(top, ml[j].x);
+              }
+              if (top == -INFINITY) continue;
+              const float keep = __builtin_amdgcn_exp2f(m - top);
+              l *= keep;
+              y *= keep;
+              m = top;
+#pragma unroll
+              for (int j = 0; j < kBatch; ++j) {
+                if (ml[j].x == -INFINITY) continue;
+                const float e = __builtin_amdgcn_exp2f(ml[j].x - top);
+                l = fmaf(e, ml[j].y, l);
+                y += e * f32x4{lo[j].x, lo[j].y, hi[j].x, hi[j].y};
+              }
             }
-          put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
+          if (parts > 1) {
+            float *mine_at = &s_acc[0][0][0] + 8 * tid;
+            if (mine) {
+              *reinterpret_cast<f32x4 *>(mine_at) = y;
+              mine_at[4] = m;
+              mine_at[5] = l;
+            }
+            __syncthreads();
+            if (mine && part == 0) {
+              float top = m;
+              for (int k = 1; k < parts; ++k) top = fmaxf(top, mine_at[8 * k * items + 4]);
+              if (top != -INFINITY) {
+                const float keep = __builtin_amdgcn_exp2f(m - top);
+                l *= keep;
+                y *= keep;
+                for (int k = 1; k < parts; ++k) {
+                  const float *from = mine_at + 8 * k * items;
+                  if (from[4] == -INFINITY) continue;
+                  const float e = __builtin_amdgcn_exp2f(from[4] - top);
+                  l = fmaf(e, from[5], l);
+                  y += e * *reinterpret_cast<const f32x4 *>(from);
+                }
+                m = top;
+              }
+            }
+          }
+          if (mine && part == 0) put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
         }
-        if (tid == 0) g.counters[pc.first] = 0;  // for the next call
+        if (tid == 0)  // for the next call
+          __hip_atomic_store(g.counters + pc.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
     __syncthreads();
-    at += pc.u1 - pc.u0;
-    if (at - base == (int64_t)w.span.units * g.segs) {
-      base = at;
+    at += pc.u1 - u0;
+    u0 = 0;
+    if (++seg == g.segs) {
+      seg = 0;
       ++seq;
     }
   }
@@ -624,7 +706,9 @@ template <typename T, int DP>
 hipError_t launch(const Args &g, hipStream_t s) {
   // as many blocks as the card holds at once, or as there may be work for
   constexpr int unit = Kind<T, DP>::kUnit;
-  const int64_t longest = token_span(0x7FFFFFFF, 0, g.a.window, g.cap, unit).units + 1;
+  int64_t longest = (g.cap + unit - 1) / unit;
+  if (g.a.window > 0) longest = std::min(longest, (int64_t)g.a.window / unit + 2);
+  longest = std::max(longest, (int64_t)1);
   const int64_t most = g.q.n_seqs * (int64_t)g.segs * longest;
   const int blocks = (int)std::min((most + kWaves - 1) / kWaves, (int64_t)(DP == 256 ? 256 : 512));
   if (g.p.dim == DP) attend_kernel<T, DP, true><<<blocks, kThreads, 0, s>>>(g);

@@ -51,28 +51,40 @@ AQ_SPLIT_HD int64_t share_of(int64_t total, int blocks, int waves) {
   return s > waves ? s : waves;
 }
 
-// A block's next piece of work: units [u0, u1) of segment `seg` of a sequence whose
-// segments begin at unit `base` and have `units` units each.
+// A block's piece of a segment of `units` units: [u0, u1).  The block has units
+// [start, end) of the whole, of which `at` is the piece's first.
 struct Piece {
-  int seg, u0, u1;
-  bool whole;       // the whole segment
-  int slot;         // where its partial result goes (not whole)
-  int64_t first;    // the first block with a piece of the segment, and how many have one
-  int pieces;
+  int u1;
+  bool whole;         // the whole segment
+  int slot;           // where its partial result goes (not whole)
+  int first, pieces;  // the first block with a piece of the segment, and how many have one
 };
 
-AQ_SPLIT_HD Piece piece_at(int64_t at, int64_t end, int64_t base, int units, int64_t share) {
+AQ_SPLIT_HD Piece piece_at(int block, int64_t start, int64_t end, int64_t at, int u0, int units,
+                           int64_t share) {
   Piece p;
-  const int64_t off = at - base;
-  p.seg = (int)(off / units);
-  p.u0 = (int)(off - (int64_t)p.seg * units);
-  p.u1 = end - at < units - p.u0 ? p.u0 + (int)(end - at) : units;
-  p.whole = p.u0 == 0 && p.u1 == units;
-  p.slot = p.u0 == 0 ? 1 : 0;
-  const int64_t begin = base + (int64_t)p.seg * units;
-  p.first = begin / share;
-  p.pieces = (int)((begin + units - 1) / share - p.first) + 1;
+  p.u1 = end - at < units - u0 ? u0 + (int)(end - at) : units;
+  p.whole = u0 == 0 && p.u1 == units;
+  p.slot = u0 == 0 ? 1 : 0;
+  // of the segment's units, those before this block and up to the last (both below 2^28, so
+  // a larger share divides them as 2^31 does)
+  const uint32_t s = share < 0x80000000 ? (uint32_t)share : 0x80000000u;
+  const int64_t before = start - (at - u0);
+  p.first = before > 0 ? block - (int)(((uint32_t)before + s - 1) / s) : block;
+  p.pieces = block + (int)((uint32_t)(units - 1 - before) / s) - p.first + 1;
   return p;
+}
+
+// Where a block begins: segment and unit within it, of a sequence whose segments begin at
+// unit `base` of the whole.
+struct Start {
+  int seg, u0;
+};
+
+AQ_SPLIT_HD Start start_at(int64_t at, int64_t base, int units) {
+  const int64_t off = at - base;
+  const int seg = off >> 32 ? (int)(off / units) : (int)((uint32_t)off / (uint32_t)units);
+  return {seg, (int)(off - (int64_t)seg * units)};
 }
 
 }  // namespace aq

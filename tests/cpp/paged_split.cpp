@@ -49,16 +49,20 @@ static void check_cut(const std::vector<int> &units, int segs, int blocks, int w
   std::set<std::pair<int64_t, int>> slots;
   std::set<int64_t> counters;
   for (int64_t b = 0; b < blocks; ++b) {
-    int64_t at = b * share, end = at + share < total ? at + share : total;
+    const int64_t start = b * share, end = start + share < total ? start + share : total;
+    if (start >= end) continue;
+    int64_t at = start;
     size_t q = 0;
+    while (q + 1 < base.size() && base[q + 1] <= at) ++q;
+    Start s = start_at(at, base[q], units[q]);
     while (at < end) {
-      while (q + 1 < base.size() && base[q + 1] <= at) ++q;
-      const Piece p = piece_at(at, end, base[q], units[q], share);
-      if (p.seg < 0 || p.seg >= segs || p.u0 < 0 || p.u1 <= p.u0 || p.u1 > units[q]) fail("piece");
-      const auto key = std::make_pair((int)q, p.seg);
+      if (s.seg < 0 || s.seg >= segs || s.u0 < 0 || s.u0 >= units[q]) fail("start");
+      const Piece p = piece_at((int)b, start, end, at, s.u0, units[q], share);
+      if (p.u1 <= s.u0 || p.u1 > units[q]) fail("piece");
+      const auto key = std::make_pair((int)q, s.seg);
       auto &v = seen[key];
       v.resize(units[q]);
-      for (int u = p.u0; u < p.u1; ++u)
+      for (int u = s.u0; u < p.u1; ++u)
         if (v[u]++) fail("unit twice");
       if (p.whole != (p.pieces == 1)) fail("whole");
       if (!p.whole) {
@@ -73,7 +77,12 @@ static void check_cut(const std::vector<int> &units, int segs, int blocks, int w
           if (b != p.first + pieces[key] - 1) fail("pieces are consecutive blocks");
         }
       }
-      at += p.u1 - p.u0;
+      at += p.u1 - s.u0;
+      s.u0 = 0;
+      if (++s.seg == segs) {
+        s.seg = 0;
+        ++q;
+      }
     }
   }
   for (size_t q = 0; q < units.size(); ++q)
@@ -86,7 +95,23 @@ static void check_cut(const std::vector<int> &units, int segs, int blocks, int w
     }
 }
 
+static void check_large() {
+  // beyond 32 bits of units: a block inside the last of many long segments
+  const int units = (1 << 27) - 1, segs = 700, blocks = 512;
+  const int64_t total = (int64_t)units * segs, share = share_of(total, blocks, 4);
+  for (int64_t b : {0, 1, 255, 510, 511}) {
+    const int64_t start = b * share, end = start + share < total ? start + share : total;
+    const Start s = start_at(start, 0, units);
+    if ((int64_t)s.seg * units + s.u0 != start || s.u0 >= units) fail("large start");
+    const Piece p = piece_at((int)b, start, end, start, s.u0, units, share);
+    const int64_t begin = (int64_t)s.seg * units;
+    if (p.first != begin / share || p.first + p.pieces - 1 != (begin + units - 1) / share)
+      fail("large piece");
+  }
+}
+
 int main() {
+  check_large();
   const int edge[] = {-2147483647 - 1, -1, 0, 1, 15, 16, 17, 31, 32, 33, 1000, 2147483615, 2147483647};
   for (int n : edge)
     for (int extra : {0, 1})
