@@ -40,6 +40,7 @@ struct PagedShape {
   int n_pages, page_size, n_heads, dim;
   IoType io;
   RotaryTable rotary;
+  int cus;  // compute units of the device
 };
 
 // Which pages a sequence's tokens lie in, and how many it holds.
@@ -72,7 +73,8 @@ struct PagedAttend {
 
 // Bytes of workspace an attention of this shape may need, zeroed once when it is made.
 size_t paged_workspace_bytes(const PagedShape &p);
+// step: one token a sequence, written into its page by the same launch (a.extra 1), or null.
 hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
-                               void *workspace, hipStream_t s);
+                               const PagedAppend *step, void *workspace, hipStream_t s);
 
 }  // namespace aq

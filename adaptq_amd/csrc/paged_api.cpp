@@ -2,7 +2,7 @@
 // (include/adaptq.h, part 3): argument checks, handles, launches.
 //
 // Nothing here synchronises or allocates after a handle's creation: every call is
-// one or two launches on the caller's stream and may be captured into a graph.
+// one launch on the caller's stream and may be captured into a graph.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -464,8 +464,10 @@ adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages
     set_errorf(fn, "the rotary's rotary_dim is larger than dim");
     return nullptr;
   }
-  int device = 0;
-  if (hip_fail(hipGetDevice(&device), fn)) return nullptr;
+  int device = 0, cus = 0;
+  if (hip_fail(hipGetDevice(&device), fn) ||
+      hip_fail(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device), fn))
+    return nullptr;
   Paged *p = new (std::nothrow) Paged();
   if (!p) {
     set_errorf(fn, "host allocation failed");
@@ -473,7 +475,7 @@ adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages
   }
   p->device = device;
   p->shape = {d_k_pages, d_v_pages, n_pages, page_size, n_heads, dim,
-              static_cast<aq::IoType>(io_type), {}};
+              static_cast<aq::IoType>(io_type), {}, cus};
   hipError_t e = hipSuccess;
   if (r) {
     p->shape.rotary = r->table();
@@ -559,7 +561,7 @@ int adaptq_paged_attend_device(adaptq_paged_t h, const void *d_q, void *d_out, i
   const aq::PagedAttend a =
       attend_args(p, d_q, d_out, n_q_heads, q_nb1, q_nb2, out_nb1, out_nb2, scale, window, 0);
   DeviceGuard g(p->device);
-  if (hip_fail(aq::launch_paged_attend(p->shape, q, a, p->ws, static_cast<hipStream_t>(stream)),
+  if (hip_fail(aq::launch_paged_attend(p->shape, q, a, nullptr, p->ws, static_cast<hipStream_t>(stream)),
                fn))
     return -1;
   aq::clear_error();
@@ -595,9 +597,7 @@ int adaptq_paged_step_device(adaptq_paged_t h, const void *d_k, const void *d_v,
       attend_args(p, d_q, d_out, n_q_heads, q_nb1, q_nb2, out_nb1, out_nb2, scale, window, 1);
   DeviceGuard g(p->device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t e = aq::launch_paged_append(p->shape, q, ap, s);
-  if (e == hipSuccess) e = aq::launch_paged_attend(p->shape, q, a, p->ws, s);
-  if (hip_fail(e, fn)) return -1;
+  if (hip_fail(aq::launch_paged_attend(p->shape, q, a, &ap, p->ws, s), fn)) return -1;
   aq::clear_error();
   return 0;
 }

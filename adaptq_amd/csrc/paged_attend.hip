@@ -38,10 +38,10 @@ namespace aq {
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kTile = 16;  // query heads of a segment
 constexpr int kMaxBlocks = 1024;
+constexpr int kLoadAux = 2;
+constexpr int kMinUnits = 16;
 constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
 constexpr int kBeyond = 1 << 30;  // an offset behind every buffer
 
@@ -56,6 +56,7 @@ struct Args {
   PagedShape p;
   PagedSeqs q;
   PagedAttend a;
+  PagedAppend n;       // a step's rows (n.k null: attention alone)
   float scale2;        // of the scores, to base 2
   int group, q_tiles;  // query heads of a key head, and their tiles of 16
   int segs;            // segments of a sequence
@@ -63,6 +64,7 @@ struct Args {
   uint64_t page_mul;   // blocks of 16 tokens -> pages: x * page_mul >> page_shift
   int page_shift, page_blocks, row_bytes;
   bool out_vec;
+  int cus;
   float *partial;
   int *counters;
 };
@@ -79,6 +81,9 @@ struct Kind {
   static constexpr int kVVec = DP / 16 < kVec ? DP / 16 : kVec;
   static constexpr int kVChunks = DP / (16 * kVVec);
   static constexpr int kVRows = kUnit / 4;  // rows of V that a lane loads
+  static constexpr int kWaves = 4;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kBlocksPerCu = DP == 256 ? 1 : 2;
 };
 
 template <int BYTES>
@@ -260,7 +265,37 @@ struct Attend {
         const_cast<char *>(at), 0, __builtin_amdgcn_readfirstlane(rows * g.row_bytes), 0x00020000);
   }
 
+  // A step's token: its rows, the key rotated, into its slot, by the wave that will load it.
+  __device__ void append(int seq, int at) const {
+    const int col = (int)((uint64_t)(uint32_t)(at >> 4) * g.page_mul >> g.page_shift);
+    const int page = ((cint *)(uint64_t)table)[col];
+    if (page < 0 || page >= g.p.n_pages) return;
+    const int slot = at - col * g.p.page_size;
+    const int64_t row = ((int64_t)page * g.p.n_heads + head) * g.p.page_size + slot;
+    T *k = reinterpret_cast<T *>(static_cast<char *>(g.p.k_pages) + row * g.row_bytes);
+    T *v = reinterpret_cast<T *>(static_cast<char *>(g.p.v_pages) + row * g.row_bytes);
+    const T *kin = reinterpret_cast<const T *>(static_cast<const char *>(g.n.k) +
+                                               seq * (int64_t)g.n.k_nb[1] + head * (int64_t)g.n.k_nb[0]);
+    const T *vin = reinterpret_cast<const T *>(static_cast<const char *>(g.n.v) +
+                                               seq * (int64_t)g.n.v_nb[1] + head * (int64_t)g.n.v_nb[0]);
+    const RotaryTable &rt = g.p.rotary;
+    for (int i = lane; i < g.p.dim / 2; i += 64) {
+      const bool turns = i < rt.pairs;
+      const int2 c = turns ? chunk_at<1>(i, rt.pairs, rt.interleaved) : make_int2(2 * i, 2 * i + 1);
+      RowVec<T, 1> x{{kin[c.x]}}, y{{kin[c.y]}};
+      if (turns) {
+        const float2 cs = rotary_cos_sin(rt.steps[i], at, rt.amplitude);
+        rotate_pairs<T, 1>(x, y, &cs, rt.interleaved, false);
+      }
+      k[c.x] = x.x[0];
+      k[c.y] = y.x[0];
+      v[2 * i] = vin[2 * i];
+      v[2 * i + 1] = vin[2 * i + 1];
+    }
+  }
+
   __device__ void load(Rows &r, const Where &w, int unit) const {
+
     const int t0 = unit * K::kUnit;
     // (opaque here, so that what is added stays part of the loads instead of taking a
     // register each outside the loop)
@@ -272,7 +307,7 @@ struct Attend {
 #pragma unroll
       for (int c = 0; c < K::kChunks; ++c)
         r.k[s][c] = __builtin_amdgcn_raw_buffer_load_b128(
-            k, EXACT ? k0 + c * 64 : k_off[EXACT ? 0 : c], 0, 0);
+            k, EXACT ? k0 + c * 64 : k_off[EXACT ? 0 : c], 0, kLoadAux);
     }
 #pragma unroll
     for (int s = 0; s < K::kSubs; ++s) {
@@ -285,9 +320,9 @@ struct Attend {
           const int off = EXACT ? v0 + (j * DP + 16 * c * K::kVVec) * size
                                 : v_off[EXACT ? 0 : 4 * c + j];
           if constexpr (K::kVVec * sizeof(T) == 8)
-            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b64(v, off, 0, 0);
+            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b64(v, off, 0, kLoadAux);
           else
-            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b128(v, off, 0, 0);
+            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b128(v, off, 0, kLoadAux);
         }
     }
   }
@@ -404,32 +439,34 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// First unit and segment base of the sequence that unit `at` of the whole belongs to.
-// All lanes; lengths of 64 sequences a round.
+// All units of a call, and the sequence that unit `at` of them belongs to: its length, and
+// the unit that its segments begin at.  All lanes; 64 sequences a round.
 struct Found {
-  int seq;
+  int seq, length;
   int64_t base;
 };
 
-__device__ __forceinline__ int64_t units_of(const Args &g, int seq, int unit) {
-  if (seq >= g.q.n_seqs) return 0;
-  return (int64_t)token_span(g.q.lengths[seq], g.a.extra, g.a.window, g.cap, unit).units * g.segs;
+__device__ __forceinline__ int64_t units_of(const Args &g, int length, int unit) {
+  return (int64_t)token_span(length, g.a.extra, g.a.window, g.cap, unit, kMinUnits).units * g.segs;
 }
 
 __device__ __forceinline__ int64_t total_units(const Args &g, int lane, int unit) {
+  if (g.q.n_seqs == 1) return units_of(g, g.q.lengths[0], unit);
   int64_t x = 0;
-  for (int b = lane; b < g.q.n_seqs; b += 64) x += units_of(g, b, unit);
-  if (g.q.n_seqs == 1) return uniform(x);
+  for (int b = lane; b < g.q.n_seqs; b += 64) x += units_of(g, g.q.lengths[b], unit);
 #pragma unroll
   for (int k = 32; k >= 1; k >>= 1) x += __shfl_xor(x, k, 64);
-  return uniform(x);
+  return x;
 }
 
 __device__ __forceinline__ Found find_unit(const Args &g, int lane, int unit, int64_t at) {
-  if (g.q.n_seqs == 1) return {0, 0};
+  if (g.q.n_seqs == 1) return {0, g.q.lengths[0], 0};
   int64_t base = 0;
   for (int b0 = 0;; b0 += 64) {
-    int64_t x = units_of(g, b0 + lane, unit), sum = x;
+    const int b = b0 + lane;
+    const int length = g.q.lengths[min(b, g.q.n_seqs - 1)];
+    const int64_t x = b < g.q.n_seqs ? units_of(g, length, unit) : 0;
+    int64_t sum = x;
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) {
       const int64_t y = __shfl_up(sum, k, 64);
@@ -438,40 +475,48 @@ __device__ __forceinline__ Found find_unit(const Args &g, int lane, int unit, in
     const uint64_t past = __ballot(base + sum > at);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      return {b0 + l, base + __shfl(sum - x, l, 64)};
+      return {b0 + l, __shfl(length, l, 64), base + __shfl(sum - x, l, 64)};
     }
     base += __shfl(sum, 63, 64);
   }
 }
 
-template <typename T, int DP, bool EXACT>
-__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(const Args g) {
+template <typename T, int DP, bool EXACT, bool STEP>
+__global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void attend_kernel(
+    const Args g) {
   typedef Kind<T, DP> K;
   typedef Attend<T, DP, EXACT> A;
+  constexpr int kWaves = K::kWaves, kThreads = K::kThreads;
   constexpr int S = DP + 4;
   __shared__ __align__(16) float s_acc[kWaves][kTile][S];  // first: the queries, in [0]
   __shared__ float s_m[kWaves][kTile], s_l[kWaves][kTile];
-  __shared__ float2 s_cs[DP / 2];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dim = g.p.dim;
 
-  const int64_t total = total_units(g, lane, K::kUnit);
+  const int64_t total = uniform(total_units(g, lane, K::kUnit));
   const int64_t share = share_of(total, (int)gridDim.x, kWaves);
   const int64_t start = blockIdx.x * share, end = min(start + share, total);
   if (start >= end) return;
-  int64_t at = start;
-  Found f = find_unit(g, lane, K::kUnit, at);
+  const Found f = find_unit(g, lane, K::kUnit, start);
   int seq = __builtin_amdgcn_readfirstlane(f.seq);
+  int length = __builtin_amdgcn_readfirstlane(f.length);
+  int64_t at = start;
   const int64_t base = uniform(f.base);
-  int turned = -1;  // the sequence whose query position s_cs holds
+
+  // this thread's pair of channels of the queries: a pair of the rotation, or two side by side
+  const RotaryTable &rt = g.p.rotary;
+  const int pair = tid % (DP / 2);
+  const bool turns = pair < rt.pairs;
+  const int c0 = !turns || rt.interleaved ? 2 * pair : pair;
+  const int c1 = !turns || rt.interleaved ? 2 * pair + 1 : pair + rt.pairs;
+  const uint64_t step = turns ? rt.steps[pair] : 0;
 
   A w(g, lane);
   int seg = -1, u0 = 0;
   while (at < end) {
-    const int length = ((cint *)(uint64_t)g.q.lengths)[seq];
-    w.span = token_span(length, g.a.extra, g.a.window, g.cap, K::kUnit);
+    w.span = token_span(length, g.a.extra, g.a.window, g.cap, K::kUnit, kMinUnits);
     if (seg < 0) {
       const Start s = start_at(at, base, w.span.units);
       seg = __builtin_amdgcn_readfirstlane(s.seg);
@@ -481,43 +526,39 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(con
     const int head = __builtin_amdgcn_readfirstlane(seg / g.q_tiles);
     const int q0 = (seg - head * g.q_tiles) * kTile;
     const int rows = min(kTile, g.group - q0);
+    const int64_t qh0 = (int64_t)head * g.group + q0;
     w.head = head;
     w.table = g.q.table + (int64_t)seq * g.q.stride;
     w.u_end = w.span.first_unit + pc.u1;
     int u = w.span.first_unit + u0 + wave;
 
+    if (STEP && length >= 0 && length < g.cap) {
+      // the token goes into its page by the wave whose units hold it
+      const int last = length / K::kUnit, off = last - (w.span.first_unit + u0);
+      if (last < w.u_end && off >= 0 && off % kWaves == wave) {
+        w.append(seq, length);
+        stores_done();
+      }
+    }
     typename A::Rows r0, r1;
     typename A::Where w0 = w.locate(u), w1 = w.locate(u + kWaves);
     w.load(r0, w0, u);
 
     // the queries, rotated, into LDS and from there into operands
-    const RotaryTable &rt = g.p.rotary;
-    const int64_t qh0 = (int64_t)head * g.group + q0;
-    const char *q_at = static_cast<const char *>(g.a.q) + (int64_t)seq * g.a.q_nb[1];
-    if (rt.pairs && turned != seq) {
-      for (int i = tid; i < rt.pairs; i += kThreads)
-        s_cs[i] = rotary_cos_sin(rt.steps[i], length < 0 ? 0 : length + g.a.extra - 1, rt.amplitude);
-      turned = seq;
-      __syncthreads();
-    }
-    for (int i = tid; i < kTile * DP; i += kThreads) {
-      const int row = i / DP, d = i % DP;
-      float x = 0.0f;
-      if (row < rows && d < dim) {
-        const T *q = reinterpret_cast<const T *>(q_at + (qh0 + row) * (int64_t)g.a.q_nb[0]);
-        x = row_get(q[d]);
-        if (d < 2 * rt.pairs) {
-          const bool second = rt.interleaved ? d & 1 : d >= rt.pairs;
-          const int pair = rt.interleaved ? d >> 1 : second ? d - rt.pairs : d;
-          const int other = rt.interleaved ? d ^ 1 : second ? d - rt.pairs : d + rt.pairs;
-          const float2 cs = s_cs[pair];
-          const float y = row_get(q[other]);
-          x = second ? fmaf(x, cs.x, y * cs.y) : fmaf(x, cs.x, -(y * cs.y));
-        }
+    const char *q_at = static_cast<const char *>(g.a.q) + (int64_t)seq * g.a.q_nb[1] +
+                       qh0 * (int64_t)g.a.q_nb[0];
+    {
+      float2 cs = make_float2(1.0f, 0.0f);
+      if (turns) cs = rotary_cos_sin(step, length < 0 ? 0 : length + g.a.extra - 1, rt.amplitude);
+      for (int row = tid / (DP / 2); row < rows; row += 2 * kThreads / DP) {
+        const T *q = reinterpret_cast<const T *>(q_at + row * (int64_t)g.a.q_nb[0]);
+        const float x = c0 < dim ? row_get(q[c0]) : 0.0f, y = c1 < dim ? row_get(q[c1]) : 0.0f;
+        s_acc[0][row][c0] = turns ? fmaf(x, cs.x, -(y * cs.y)) : x;
+        s_acc[0][row][c1] = turns ? fmaf(y, cs.x, x * cs.y) : y;
       }
-      s_acc[0][row][d] = x;
     }
     __syncthreads();
+    // (rows that are no query's hold anything: their columns of the products go nowhere)
     if constexpr (K::kHalf) {
 #pragma unroll
       for (int c = 0; c < K::kChunks; ++c) {
@@ -693,9 +734,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(con
     __syncthreads();
     at += pc.u1 - u0;
     u0 = 0;
-    if (++seg == g.segs) {
+    if (++seg == g.segs && at < end) {
       seg = 0;
-      ++seq;
+      length = ((cint *)(uint64_t)g.q.lengths)[++seq];
     }
   }
 }
@@ -708,11 +749,16 @@ hipError_t launch(const Args &g, hipStream_t s) {
   constexpr int unit = Kind<T, DP>::kUnit;
   int64_t longest = (g.cap + unit - 1) / unit;
   if (g.a.window > 0) longest = std::min(longest, (int64_t)g.a.window / unit + 2);
-  longest = std::max(longest, (int64_t)1);
+  typedef Kind<T, DP> K;
+  longest = std::max(longest, (int64_t)kMinUnits);
   const int64_t most = g.q.n_seqs * (int64_t)g.segs * longest;
-  const int blocks = (int)std::min((most + kWaves - 1) / kWaves, (int64_t)(DP == 256 ? 256 : 512));
-  if (g.p.dim == DP) attend_kernel<T, DP, true><<<blocks, kThreads, 0, s>>>(g);
-  else attend_kernel<T, DP, false><<<blocks, kThreads, 0, s>>>(g);
+  const int blocks = (int)std::min((most + K::kWaves - 1) / K::kWaves,
+                                   (int64_t)std::min(kMaxBlocks, g.cus * K::kBlocksPerCu));
+  auto *kernel = g.p.dim == DP ? (g.n.k ? attend_kernel<T, DP, true, true>
+                                        : attend_kernel<T, DP, true, false>)
+                               : (g.n.k ? attend_kernel<T, DP, false, true>
+                                        : attend_kernel<T, DP, false, false>);
+  kernel<<<blocks, K::kThreads, 0, s>>>(g);
   return hipGetLastError();
 }
 
@@ -732,8 +778,9 @@ size_t paged_workspace_bytes(const PagedShape &p) {
 }
 
 hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
-                               void *workspace, hipStream_t s) {
+                               const PagedAppend *step, void *workspace, hipStream_t s) {
   Args g{};
+  if (step) g.n = *step;
   g.p = p;
   g.q = q;
   g.a = a;
@@ -754,6 +801,7 @@ hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const Pa
   g.page_mul = (((uint64_t)1 << g.page_shift) + g.page_blocks - 1) / g.page_blocks;
   size_t x = reinterpret_cast<uintptr_t>(a.out) | a.out_nb[0] | a.out_nb[1];
   g.out_vec = x % (p.io == IoType::F32 ? 16 : 8) == 0;
+  g.cus = p.cus;
   g.counters = static_cast<int *>(workspace);
   g.partial = reinterpret_cast<float *>(g.counters + kMaxBlocks);
   switch (p.io) {

@@ -24,12 +24,14 @@ namespace aq {
 // The tokens that a sequence's attention is over: [lo, n), and their units.
 struct TokenSpan {
   int lo, n;
-  int first_unit, units;  // at least one unit, so that an empty sequence has a segment
+  int first_unit, units;  // units: at least `least`, those behind the last token empty
 };
 
 // length: tokens held (negative: none), extra: more by now; cap: tokens that the table
-// has columns for.
-AQ_SPLIT_HD TokenSpan token_span(int length, int extra, int window, int64_t cap, int unit) {
+// has columns for.  least: what a segment costs at the least, in units, so that a share
+// does not fill with many short ones; 1 or more, for an empty sequence has segments too.
+AQ_SPLIT_HD TokenSpan token_span(int length, int extra, int window, int64_t cap, int unit,
+                                 int least) {
   int64_t held = length < 0 ? 0 : (int64_t)length + extra;
   TokenSpan s;
   const int64_t lo = window > 0 && held > window ? held - window : 0;
@@ -40,7 +42,7 @@ AQ_SPLIT_HD TokenSpan token_span(int length, int extra, int window, int64_t cap,
   s.lo = (int)(lo < held ? lo : held);
   s.first_unit = s.lo / unit;
   s.units = s.n > 0 ? (s.n - 1) / unit + 1 - s.first_unit : 1;
-  if (s.units < 1) s.units = 1;
+  if (s.units < least) s.units = least;
   return s;
 }
 

@@ -19,7 +19,11 @@ static void fail(const char *what) {
 }
 
 static void check_span(int length, int extra, int window, int64_t cap, int unit) {
-  const TokenSpan s = token_span(length, extra, window, cap, unit);
+  const TokenSpan s = token_span(length, extra, window, cap, unit, 1);
+  const TokenSpan t = token_span(length, extra, window, cap, unit, 8);
+  if (t.lo != s.lo || t.n != s.n || t.first_unit != s.first_unit ||
+      t.units != (s.units < 8 ? 8 : s.units))
+    fail("least");
   const int64_t held = length < 0 ? 0 : (int64_t)length + extra;
   int64_t n = held < cap ? held : cap;
   if (n > 0x7FFFFFE0) n = 0x7FFFFFE0;
