@@ -38,9 +38,13 @@ namespace aq {
 
 namespace {
 
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
 constexpr int kTile = 16;  // query heads of a segment
 constexpr int kMaxBlocks = 1024;
-constexpr int kLoadAux = 2;
+constexpr int kStreaming = 2;  // nt: rows are read once
+// What a segment counts at the least, and what is never cut: its start and end cost a block
+// about as much as the rows of 16 units (5 us).
 constexpr int kMinUnits = 16;
 constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
 constexpr int kBeyond = 1 << 30;  // an offset behind every buffer
@@ -81,9 +85,6 @@ struct Kind {
   static constexpr int kVVec = DP / 16 < kVec ? DP / 16 : kVec;
   static constexpr int kVChunks = DP / (16 * kVVec);
   static constexpr int kVRows = kUnit / 4;  // rows of V that a lane loads
-  static constexpr int kWaves = 4;
-  static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kBlocksPerCu = DP == 256 ? 1 : 2;
 };
 
 template <int BYTES>
@@ -168,22 +169,106 @@ __device__ __forceinline__ void split8(const float *x, u32x4 &hi, u32x4 &lo) {
 }
 
 // Partial results pass between blocks that may sit on different dies, whose L2 caches do not
-// see each other's lines: they are stored past them and read past them (relaxed atomics of
-// the device's scope).  A fence of that scope instead writes back and drops a whole L2: it
-// cost tens of microseconds a call.
+// see each other's lines: they are stored past them and read past them (the device's scope,
+// as its relaxed atomics are).  A fence of that scope instead writes back and drops a whole
+// L2: it cost tens of microseconds a call.
 __device__ __forceinline__ void put_shared(float *p, float x, float y) {
-  const uint64_t w = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
-  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), w, __ATOMIC_RELAXED,
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p),
+                     (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float2 get_shared(const float *p) {
+__device__ __forceinline__ float2 get_shared2(const float *p) {
   const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED,
                                        __HIP_MEMORY_SCOPE_AGENT);
   return make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
 }
+__device__ __forceinline__ f32x4 get_shared4(const float *p) {
+  const float2 a = get_shared2(p), b = get_shared2(p + 2);
+  return {a.x, a.y, b.x, b.y};
+}
 // Every store of this wave has reached the memory that all dies see.
 __device__ __forceinline__ void stores_done() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// A partial result: the rows' sums [16][DP], then (m, l) of each row.
+constexpr int part_floats(int dp) { return kTile * (dp + 2); }
+
+// The pieces of a cut segment together, by the block that finished last, in their order.
+// Threads beyond one per 4 channels of a row share the pieces; a thread has the loads of
+// kBatch pieces in flight at once.
+template <int DP, typename Put>
+__device__ __forceinline__ void join(const Args &g, const Piece &pc, int rows, int tid, float *lds,
+                                     Put put) {
+  constexpr int kPart = part_floats(DP);
+  // the first piece began the segment (slot 1 of its block), the others go on with it (slot 0)
+  const float *p0 = g.partial + (2 * (int64_t)pc.first + 1) * kPart;
+  const int items = rows * (DP / 4), parts = max(1, kThreads / items);
+  for (int i0 = 0; i0 < items; i0 += kThreads) {
+    const int part = parts > 1 ? tid / items : 0;
+    const int item = parts > 1 ? tid - part * items : i0 + tid;
+    const bool mine = part < parts && item < items;
+    const int row = item / (DP / 4), d = item % (DP / 4) * 4;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 y = {0, 0, 0, 0};
+    if (mine)
+      for (int k0 = part; k0 < pc.pieces; k0 += parts * kBatch) {
+        float2 ml[kBatch];
+        f32x4 x[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int k = min(k0 + j * parts, pc.pieces - 1);  // (the last again: no weight)
+          const float *from = p0 + (k ? 2 * k - 1 : 0) * (int64_t)kPart;
+          ml[j] = get_shared2(from + kTile * DP + 2 * row);
+          x[j] = get_shared4(from + row * DP + d);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          if (k0 + j * parts >= pc.pieces) ml[j].x = -INFINITY;
+          top = fmaxf(top, ml[j].x);
+        }
+        if (top == -INFINITY) continue;
+        const float keep = __builtin_amdgcn_exp2f(m - top);
+        l *= keep;
+        y *= keep;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          if (ml[j].x == -INFINITY) continue;
+          const float e = __builtin_amdgcn_exp2f(ml[j].x - top);
+          l = fmaf(e, ml[j].y, l);
+          y += e * x[j];
+        }
+      }
+    if (parts > 1) {
+      float *at = lds + 8 * tid;
+      if (mine) {
+        *reinterpret_cast<f32x4 *>(at) = y;
+        at[4] = m;
+        at[5] = l;
+      }
+      __syncthreads();
+      if (mine && part == 0) {
+        float top = m;
+        for (int k = 1; k < parts; ++k) top = fmaxf(top, at[8 * k * items + 4]);
+        if (top != -INFINITY) {
+          const float keep = __builtin_amdgcn_exp2f(m - top);
+          l *= keep;
+          y *= keep;
+          for (int k = 1; k < parts; ++k) {
+            const float *from = at + 8 * k * items;
+            if (from[4] == -INFINITY) continue;
+            const float e = __builtin_amdgcn_exp2f(from[4] - top);
+            l = fmaf(e, from[5], l);
+            y += e * *reinterpret_cast<const f32x4 *>(from);
+          }
+          m = top;
+        }
+      }
+    }
+    if (mine && part == 0) put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
+  }
 }
 
 // A wave's running state over its units.
@@ -307,7 +392,7 @@ struct Attend {
 #pragma unroll
       for (int c = 0; c < K::kChunks; ++c)
         r.k[s][c] = __builtin_amdgcn_raw_buffer_load_b128(
-            k, EXACT ? k0 + c * 64 : k_off[EXACT ? 0 : c], 0, kLoadAux);
+            k, EXACT ? k0 + c * 64 : k_off[EXACT ? 0 : c], 0, kStreaming);
     }
 #pragma unroll
     for (int s = 0; s < K::kSubs; ++s) {
@@ -320,9 +405,9 @@ struct Attend {
           const int off = EXACT ? v0 + (j * DP + 16 * c * K::kVVec) * size
                                 : v_off[EXACT ? 0 : 4 * c + j];
           if constexpr (K::kVVec * sizeof(T) == 8)
-            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b64(v, off, 0, kLoadAux);
+            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b64(v, off, 0, kStreaming);
           else
-            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b128(v, off, 0, kLoadAux);
+            r.v[4 * s + j][c] = __builtin_amdgcn_raw_buffer_load_b128(v, off, 0, kStreaming);
         }
     }
   }
@@ -433,60 +518,42 @@ struct Attend {
   }
 };
 
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+// The lengths of up to 64 sequences, one a lane, and where their units end among the units
+// of all of them.
+struct Ends {
+  int length;
+  int64_t end, units;
+};
+
+__device__ __forceinline__ Ends ends_of(const Args &g, int lane, int unit, int b0) {
+  const int b = b0 + lane;
+  Ends e;
+  e.length = g.q.lengths[min(b, g.q.n_seqs - 1)];
+  e.units = 0;
+  if (b < g.q.n_seqs)
+    e.units = (int64_t)token_span(e.length, g.a.extra, g.a.window, g.cap, unit, kMinUnits).units *
+              g.segs;
+  e.end = e.units;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    if (k >= g.q.n_seqs) break;  // (uniform)
+    const int64_t y = __shfl_up(e.end, k, 64);
+    if (lane >= k) e.end += y;
+  }
+  return e;
+}
+
+__device__ __forceinline__ int64_t uniform(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), lane);
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// All units of a call, and the sequence that unit `at` of them belongs to: its length, and
-// the unit that its segments begin at.  All lanes; 64 sequences a round.
-struct Found {
-  int seq, length;
-  int64_t base;
-};
-
-__device__ __forceinline__ int64_t units_of(const Args &g, int length, int unit) {
-  return (int64_t)token_span(length, g.a.extra, g.a.window, g.cap, unit, kMinUnits).units * g.segs;
-}
-
-__device__ __forceinline__ int64_t total_units(const Args &g, int lane, int unit) {
-  if (g.q.n_seqs == 1) return units_of(g, g.q.lengths[0], unit);
-  int64_t x = 0;
-  for (int b = lane; b < g.q.n_seqs; b += 64) x += units_of(g, g.q.lengths[b], unit);
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) x += __shfl_xor(x, k, 64);
-  return x;
-}
-
-__device__ __forceinline__ Found find_unit(const Args &g, int lane, int unit, int64_t at) {
-  if (g.q.n_seqs == 1) return {0, g.q.lengths[0], 0};
-  int64_t base = 0;
-  for (int b0 = 0;; b0 += 64) {
-    const int b = b0 + lane;
-    const int length = g.q.lengths[min(b, g.q.n_seqs - 1)];
-    const int64_t x = b < g.q.n_seqs ? units_of(g, length, unit) : 0;
-    int64_t sum = x;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const int64_t y = __shfl_up(sum, k, 64);
-      if (lane >= k) sum += y;
-    }
-    const uint64_t past = __ballot(base + sum > at);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      return {b0 + l, __shfl(length, l, 64), base + __shfl(sum - x, l, 64)};
-    }
-    base += __shfl(sum, 63, 64);
-  }
-}
-
 template <typename T, int DP, bool EXACT, bool STEP>
-__global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void attend_kernel(
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
     const Args g) {
   typedef Kind<T, DP> K;
   typedef Attend<T, DP, EXACT> A;
-  constexpr int kWaves = K::kWaves, kThreads = K::kThreads;
   constexpr int S = DP + 4;
   __shared__ __align__(16) float s_acc[kWaves][kTile][S];  // first: the queries, in [0]
   __shared__ float s_m[kWaves][kTile], s_l[kWaves][kTile];
@@ -495,15 +562,29 @@ __global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void at
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dim = g.p.dim;
 
-  const int64_t total = uniform(total_units(g, lane, K::kUnit));
+  // the block's share of the units, and the sequence that it begins in
+  Ends e = ends_of(g, lane, K::kUnit, 0);
+  const int n_seqs = g.q.n_seqs;
+  int64_t total = uniform(e.end, min(n_seqs, 64) - 1);
+  for (int b0 = 64; b0 < n_seqs; b0 += 64)
+    total += uniform(ends_of(g, lane, K::kUnit, b0).end, min(n_seqs - b0, 64) - 1);
   const int64_t share = share_of(total, (int)gridDim.x, kWaves);
   const int64_t start = blockIdx.x * share, end = min(start + share, total);
   if (start >= end) return;
-  const Found f = find_unit(g, lane, K::kUnit, start);
-  int seq = __builtin_amdgcn_readfirstlane(f.seq);
-  int length = __builtin_amdgcn_readfirstlane(f.length);
+  int64_t base = 0;
+  uint64_t past = __ballot(e.end > start);
+  int seq = 0;
+  while (!past) {  // (ends: start < total)
+    base += uniform(e.end, 63);
+    seq += 64;
+    e = ends_of(g, lane, K::kUnit, seq);
+    past = __ballot(base + e.end > start && seq + lane < n_seqs);
+  }
+  const int first = __ffsll((unsigned long long)past) - 1;
+  seq += first;
+  int length = __builtin_amdgcn_readlane(e.length, first);
+  base += uniform(e.end, first) - uniform(e.units, first);
   int64_t at = start;
-  const int64_t base = uniform(f.base);
 
   // this thread's pair of channels of the queries: a pair of the rotation, or two side by side
   const RotaryTable &rt = g.p.rotary;
@@ -515,6 +596,14 @@ __global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void at
 
   A w(g, lane);
   int seg = -1, u0 = 0;
+  const auto next = [&](const Piece &pc) {
+    at += pc.u1 - u0;
+    u0 = 0;
+    if (++seg == g.segs && at < end) {
+      seg = 0;
+      length = ((cint *)(uint64_t)g.q.lengths)[++seq];
+    }
+  };
   while (at < end) {
     w.span = token_span(length, g.a.extra, g.a.window, g.cap, K::kUnit, kMinUnits);
     if (seg < 0) {
@@ -522,7 +611,12 @@ __global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void at
       seg = __builtin_amdgcn_readfirstlane(s.seg);
       u0 = __builtin_amdgcn_readfirstlane(s.u0);
     }
-    const Piece pc = piece_at(blockIdx.x, start, end, at, u0, w.span.units, share);
+    const Piece pc =
+        piece_at(blockIdx.x, start, end, at, u0, w.span.units, w.span.short_, share);
+    if (pc.empty) {
+      next(pc);
+      continue;
+    }
     const int head = __builtin_amdgcn_readfirstlane(seg / g.q_tiles);
     const int q0 = (seg - head * g.q_tiles) * kTile;
     const int rows = min(kTile, g.group - q0);
@@ -626,7 +720,7 @@ __global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void at
         for (int i = 0; i < 4; ++i) o[i] = v.x[i];
       }
     };
-    constexpr int kPart = kTile * (DP + 2);  // floats of a partial result
+    constexpr int kPart = part_floats(DP);
     for (int i = tid; i < rows * (DP / 4); i += kThreads) {
       const int row = i / (DP / 4), d = i % (DP / 4) * 4;
       float m = -INFINITY, l = 0.0f;
@@ -658,86 +752,13 @@ __global__ __launch_bounds__((Kind<T, DP>::kThreads), DP == 256 ? 1 : 2) void at
                                         __HIP_MEMORY_SCOPE_AGENT) == pc.pieces - 1;
       __syncthreads();
       if (s_last) {
-        // Threads beyond one per 4 channels of a row share the pieces; a thread has the loads
-        // of kBatch pieces in flight at once.
-        const float *p0 = g.partial + (2 * (int64_t)pc.first + 1) * kPart;  // the first one's slot 1
-        const int items = rows * (DP / 4), parts = max(1, kThreads / items);
-        for (int i0 = 0; i0 < items; i0 += kThreads) {
-          const int part = parts > 1 ? tid / items : 0;
-          const int item = parts > 1 ? tid - part * items : i0 + tid;
-          const bool mine = part < parts && item < items;
-          const int row = item / (DP / 4), d = item % (DP / 4) * 4;
-          float m = -INFINITY, l = 0.0f;
-          f32x4 y = {0, 0, 0, 0};
-          if (mine)
-            for (int k0 = part; k0 < pc.pieces; k0 += parts * kBatch) {
-              float2 ml[kBatch], lo[kBatch], hi[kBatch];
-#pragma unroll
-              for (int j = 0; j < kBatch; ++j) {
-                const int k = min(k0 + j * parts, pc.pieces - 1);  // (the last again: no weight)
-                const float *from = p0 + (k ? 2 * k - 1 : 0) * (int64_t)kPart;
-                ml[j] = get_shared(from + kTile * DP + 2 * row);
-                lo[j] = get_shared(from + row * DP + d);
-                hi[j] = get_shared(from + row * DP + d + 2);
-              }
-              float top = m;
-#pragma unroll
-              for (int j = 0; j < kBatch; ++j) {
-                if (k0 + j * parts >= pc.pieces) ml[j].x = -INFINITY;
-                top = fmaxf(top, ml[j].x);
-              }
-              if (top == -INFINITY) continue;
-              const float keep = __builtin_amdgcn_exp2f(m - top);
-              l *= keep;
-              y *= keep;
-              m = top;
-#pragma unroll
-              for (int j = 0; j < kBatch; ++j) {
-                if (ml[j].x == -INFINITY) continue;
-                const float e = __builtin_amdgcn_exp2f(ml[j].x - top);
-                l = fmaf(e, ml[j].y, l);
-                y += e * f32x4{lo[j].x, lo[j].y, hi[j].x, hi[j].y};
-              }
-            }
-          if (parts > 1) {
-            float *mine_at = &s_acc[0][0][0] + 8 * tid;
-            if (mine) {
-              *reinterpret_cast<f32x4 *>(mine_at) = y;
-              mine_at[4] = m;
-              mine_at[5] = l;
-            }
-            __syncthreads();
-            if (mine && part == 0) {
-              float top = m;
-              for (int k = 1; k < parts; ++k) top = fmaxf(top, mine_at[8 * k * items + 4]);
-              if (top != -INFINITY) {
-                const float keep = __builtin_amdgcn_exp2f(m - top);
-                l *= keep;
-                y *= keep;
-                for (int k = 1; k < parts; ++k) {
-                  const float *from = mine_at + 8 * k * items;
-                  if (from[4] == -INFINITY) continue;
-                  const float e = __builtin_amdgcn_exp2f(from[4] - top);
-                  l = fmaf(e, from[5], l);
-                  y += e * *reinterpret_cast<const f32x4 *>(from);
-                }
-                m = top;
-              }
-            }
-          }
-          if (mine && part == 0) put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
-        }
+        join<DP>(g, pc, rows, tid, &s_acc[0][0][0], put);
         if (tid == 0)  // for the next call
           __hip_atomic_store(g.counters + pc.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
     __syncthreads();
-    at += pc.u1 - u0;
-    u0 = 0;
-    if (++seg == g.segs && at < end) {
-      seg = 0;
-      length = ((cint *)(uint64_t)g.q.lengths)[++seq];
-    }
+    next(pc);
   }
 }
 
@@ -749,16 +770,20 @@ hipError_t launch(const Args &g, hipStream_t s) {
   constexpr int unit = Kind<T, DP>::kUnit;
   int64_t longest = (g.cap + unit - 1) / unit;
   if (g.a.window > 0) longest = std::min(longest, (int64_t)g.a.window / unit + 2);
-  typedef Kind<T, DP> K;
-  longest = std::max(longest, (int64_t)kMinUnits);
-  const int64_t most = g.q.n_seqs * (int64_t)g.segs * longest;
-  const int blocks = (int)std::min((most + K::kWaves - 1) / K::kWaves,
-                                   (int64_t)std::min(kMaxBlocks, g.cus * K::kBlocksPerCu));
+  const int64_t segments = g.q.n_seqs * (int64_t)g.segs;
+  // Two blocks a CU overlap one's ends of segments with the other's rows (64 sequences x 8
+  // heads of 8,192 tokens 315 us, with one 320; 1,666 segments of a few tokens 40 and 53).
+  // Fewer segments than CUs are cut: into half as many pieces with one block a CU, and
+  // joining them is what costs (one sequence of 32,768 tokens, 8 heads, 30 us, with two 35).
+  const int per_cu = DP == 256 || segments < g.cus ? 1 : 2;
+  const int64_t most = segments * std::max(longest, (int64_t)kMinUnits);
+  const int blocks = (int)std::min((most + kWaves - 1) / kWaves,
+                                   (int64_t)std::min(kMaxBlocks, g.cus * per_cu));
   auto *kernel = g.p.dim == DP ? (g.n.k ? attend_kernel<T, DP, true, true>
                                         : attend_kernel<T, DP, true, false>)
                                : (g.n.k ? attend_kernel<T, DP, false, true>
                                         : attend_kernel<T, DP, false, false>);
-  kernel<<<blocks, K::kThreads, 0, s>>>(g);
+  kernel<<<blocks, kThreads, 0, s>>>(g);
   return hipGetLastError();
 }
 
@@ -774,7 +799,7 @@ hipError_t launch_type(const Args &g, hipStream_t s) {
 }  // namespace
 
 size_t paged_workspace_bytes(const PagedShape &p) {
-  return kMaxBlocks * (2 * sizeof(float) * kTile * (padded_dim(p.dim) + 2) + sizeof(int));
+  return kMaxBlocks * (2 * sizeof(float) * part_floats(padded_dim(p.dim)) + sizeof(int));
 }
 
 hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,

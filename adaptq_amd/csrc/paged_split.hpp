@@ -9,6 +9,7 @@
 // finishes the segments that lie inside its share and leaves a partial result for
 // the ones that its share cuts: one that began before it (slot 0) and one that goes
 // on behind it (slot 1).  A cut segment is joined by the block that finishes last.
+// Short segments are never cut: the block that one begins in has all of it.
 #pragma once
 
 #include <stdint.h>
@@ -25,6 +26,7 @@ namespace aq {
 struct TokenSpan {
   int lo, n;
   int first_unit, units;  // units: at least `least`, those behind the last token empty
+  bool short_;            // no more than `least` of them: not cut
 };
 
 // length: tokens held (negative: none), extra: more by now; cap: tokens that the table
@@ -42,29 +44,40 @@ AQ_SPLIT_HD TokenSpan token_span(int length, int extra, int window, int64_t cap,
   s.lo = (int)(lo < held ? lo : held);
   s.first_unit = s.lo / unit;
   s.units = s.n > 0 ? (s.n - 1) / unit + 1 - s.first_unit : 1;
-  if (s.units < least) s.units = least;
+  s.short_ = s.units <= least;
+  if (s.short_) s.units = least;
   return s;
 }
 
 // Units of a block: an equal share of the total, in whole passes of the block's waves.
 AQ_SPLIT_HD int64_t share_of(int64_t total, int blocks, int waves) {
-  int64_t s = (total + blocks - 1) / blocks;
-  s = (s + waves - 1) / waves * waves;
+  const int64_t s = ((total + blocks - 1) / blocks + waves - 1) / waves * waves;
   return s > waves ? s : waves;
 }
 
-// A block's piece of a segment of `units` units: [u0, u1).  The block has units
-// [start, end) of the whole, of which `at` is the piece's first.
+// A block's piece of a segment of `units` units: [u0, u1), empty if it is another block's.
+// The block has units [start, end) of the whole, of which `at` is the segment's u0.
 struct Piece {
-  int u1;
+  int u1;             // where the block goes on
+  bool empty;
   bool whole;         // the whole segment
   int slot;           // where its partial result goes (not whole)
   int first, pieces;  // the first block with a piece of the segment, and how many have one
 };
 
 AQ_SPLIT_HD Piece piece_at(int block, int64_t start, int64_t end, int64_t at, int u0, int units,
-                           int64_t share) {
+                           bool short_, int64_t share) {
   Piece p;
+  if (short_) {
+    p.u1 = units;
+    p.empty = u0 > 0;
+    p.whole = true;
+    p.slot = 0;
+    p.first = block;
+    p.pieces = 1;
+    return p;
+  }
+  p.empty = false;
   p.u1 = end - at < units - u0 ? u0 + (int)(end - at) : units;
   p.whole = u0 == 0 && p.u1 == units;
   p.slot = u0 == 0 ? 1 : 0;

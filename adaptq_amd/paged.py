@@ -146,7 +146,7 @@ class PagedCache:
         if scale is not None and scale == 0:
             raise ValueError("scale must not be 0")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q)  # its rows' values side by side, as q's are
         elif self._rows(out, "out", 0) is not out or out.shape != q.shape:
             raise ValueError("out must have q's shape, its rows' values side by side")
         size, qs, os = self._size, q.stride(), out.stride()

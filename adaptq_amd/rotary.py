@@ -17,7 +17,14 @@ IO_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
 
+# torch's current stream of a device as an address; without the Stream object around it where
+# torch has that call (0.1 us instead of 1.7, of 8 to 11 that a small call takes the host)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device: torch.device) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -22,7 +22,7 @@ static void check_span(int length, int extra, int window, int64_t cap, int unit)
   const TokenSpan s = token_span(length, extra, window, cap, unit, 1);
   const TokenSpan t = token_span(length, extra, window, cap, unit, 8);
   if (t.lo != s.lo || t.n != s.n || t.first_unit != s.first_unit ||
-      t.units != (s.units < 8 ? 8 : s.units))
+      t.units != (s.units < 8 ? 8 : s.units) || t.short_ != (s.units <= 8))
     fail("least");
   const int64_t held = length < 0 ? 0 : (int64_t)length + extra;
   int64_t n = held < cap ? held : cap;
@@ -38,7 +38,7 @@ static void check_span(int length, int extra, int window, int64_t cap, int unit)
   }
 }
 
-static void check_cut(const std::vector<int> &units, int segs, int blocks, int waves) {
+static void check_cut(const std::vector<int> &units, int segs, int blocks, int waves, int short_units) {
   int64_t total = 0;
   std::vector<int64_t> base;
   for (int u : units) {
@@ -61,8 +61,20 @@ static void check_cut(const std::vector<int> &units, int segs, int blocks, int w
     Start s = start_at(at, base[q], units[q]);
     while (at < end) {
       if (s.seg < 0 || s.seg >= segs || s.u0 < 0 || s.u0 >= units[q]) fail("start");
-      const Piece p = piece_at((int)b, start, end, at, s.u0, units[q], share);
+      const bool small = units[q] <= short_units;
+      const Piece p = piece_at((int)b, start, end, at, s.u0, units[q], small, share);
       if (p.u1 <= s.u0 || p.u1 > units[q]) fail("piece");
+      if (p.empty != (small && s.u0 > 0)) fail("empty");
+      if (small && !(p.whole && p.pieces == 1 && p.u1 == units[q])) fail("short");
+      if (p.empty) {
+        at += p.u1 - s.u0;
+        s.u0 = 0;
+        if (++s.seg == segs) {
+          s.seg = 0;
+          ++q;
+        }
+        continue;
+      }
       const auto key = std::make_pair((int)q, s.seg);
       auto &v = seen[key];
       v.resize(units[q]);
@@ -107,7 +119,7 @@ static void check_large() {
     const int64_t start = b * share, end = start + share < total ? start + share : total;
     const Start s = start_at(start, 0, units);
     if ((int64_t)s.seg * units + s.u0 != start || s.u0 >= units) fail("large start");
-    const Piece p = piece_at((int)b, start, end, start, s.u0, units, share);
+    const Piece p = piece_at((int)b, start, end, start, s.u0, units, false, share);
     const int64_t begin = (int64_t)s.seg * units;
     if (p.first != begin / share || p.first + p.pieces - 1 != (begin + units - 1) / share)
       fail("large piece");
@@ -127,7 +139,8 @@ int main() {
     std::vector<int> units(1 + g() % 20);
     const int top = 1 << (g() % 9);
     for (int &u : units) u = 1 + g() % top;
-    check_cut(units, 1 + g() % 9, 1 + g() % 300, 1 << (g() % 4));
+    check_cut(units, 1 + g() % 9, 1 + g() % 300, 1 << (g() % 4),
+              g() % 3 ? 0 : g() % 40);
   }
   std::puts("ok");
 }
