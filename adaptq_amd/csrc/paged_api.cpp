@@ -26,6 +26,7 @@ using aq::set_errorf;
 
 constexpr int kMaxRotaryDim = 1024;
 constexpr int kMaxPagedDim = 256;
+constexpr int kMaxHeads = 1 << 15;  // of one set of rows
 constexpr int kPageUnit = 16;
 constexpr int kMaxPageSize = 1 << 16;
 
@@ -226,8 +227,8 @@ bool append_ok(const Paged *p, const void *k, const void *v, int n_tokens, const
 
 bool attend_ok(const Paged *p, const void *q, const void *out, int q_heads, int n_seqs,
                const size_t *nb, float scale, int window, const char *fn) {
-  if (q_heads <= 0 || q_heads % p->shape.n_heads) {
-    set_errorf(fn, "n_q_heads must be a positive multiple of the cache's n_heads");
+  if (q_heads <= 0 || q_heads > kMaxHeads || q_heads % p->shape.n_heads) {
+    set_errorf(fn, "n_q_heads must be a multiple of the cache's n_heads, up to 32768");
     return false;
   }
   if (!std::isfinite(scale)) {
@@ -377,8 +378,8 @@ int adaptq_rotary_device(adaptq_rotary_t h, const adaptq_rows_t *rows, int n_row
     const adaptq_rows_t &x = rows[i];
     aq::RotaryRows &y = c.rows[i];
     if (!require_pointer(x.in, fn, "rows.in") || !require_pointer(x.out, fn, "rows.out")) return -1;
-    if (x.n_heads <= 0 || x.n_heads > (1 << 16)) {
-      set_errorf(fn, "n_heads must be from 1 to 65536");
+    if (x.n_heads <= 0 || x.n_heads > kMaxHeads) {
+      set_errorf(fn, "n_heads must be from 1 to 32768");
       return -1;
     }
     counts[i][0] = x.n_heads;
@@ -432,8 +433,8 @@ adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages
   if (!require_pointer(d_k_pages, fn, "d_k_pages") || !require_pointer(d_v_pages, fn, "d_v_pages") ||
       !io_ok(io_type, fn))
     return nullptr;
-  if (n_pages <= 0 || n_heads <= 0 || n_heads > (1 << 16)) {
-    set_errorf(fn, "n_pages must be positive, n_heads from 1 to 65536");
+  if (n_pages <= 0 || n_heads <= 0 || n_heads > kMaxHeads) {
+    set_errorf(fn, "n_pages must be positive, n_heads from 1 to 32768");
     return nullptr;
   }
   if (page_size <= 0 || page_size % kPageUnit || page_size > kMaxPageSize) {

@@ -41,6 +41,35 @@ struct alignas(sizeof(T) * N) RowVec {
   T x[N];
 };
 
+// The same as one access; NT: marked as not used again soon.
+template <int BYTES>
+struct Words {
+  typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4)));
+};
+template <>
+struct Words<4> {
+  typedef uint32_t type;
+};
+template <>
+struct Words<2> {
+  typedef uint16_t type;
+};
+
+template <bool NT, typename T, int N>
+__device__ __forceinline__ RowVec<T, N> load_rows(const T *p) {
+  typedef typename Words<sizeof(T) * N>::type W;
+  const W *from = reinterpret_cast<const W *>(p);
+  return __builtin_bit_cast(RowVec<T, N>, NT ? __builtin_nontemporal_load(from) : *from);
+}
+template <bool NT, typename T, int N>
+__device__ __forceinline__ void store_rows(T *p, const RowVec<T, N> &x) {
+  typedef typename Words<sizeof(T) * N>::type W;
+  W *to = reinterpret_cast<W *>(p);
+  const W w = __builtin_bit_cast(W, x);
+  if (NT) __builtin_nontemporal_store(w, to);
+  else *to = w;
+}
+
 // fp16 and fp32 as their C++ types, bf16 as its bits.
 struct Bf16 {
   uint16_t bits;

@@ -142,18 +142,23 @@ class _Rotate(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
         out = rotary._rotate(positions, q, k, False, backward)
-        ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad[3:])
-                                      if y is not None and not need))
+        needs = ctx.needs_input_grad
+        if not (needs[3] and needs[4]):
+            ctx.mark_non_differentiable(*(y for y, need in zip(out, needs[3:])
+                                          if y is not None and not need))
         return out
 
     @staticmethod
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
-        want = [g if need else None
-                for g, need in zip((dq, dk), ctx.needs_input_grad[3:])]
-        have = [g for g in want if g is not None]
-        if have:
-            got = iter(_Rotate.apply(ctx.rotary, positions, not ctx.backward_, have[0],
-                                     have[1] if len(have) > 1 else None))
-            want = [next(got) if g is not None else None for g in want]
-        return (None, None, None, *want)
+        rotate = ctx.rotary._rotate
+        if torch.is_grad_enabled():  # a graph of the gradient is asked for
+            def rotate(positions, a, b, inplace, backward):
+                return _Rotate.apply(ctx.rotary, positions, backward, a, b)
+        _, _, _, needs_q, needs_k = ctx.needs_input_grad
+        dq, dk = dq if needs_q else None, dk if needs_k else None
+        if dq is not None:
+            dq, dk = rotate(positions, dq, dk, False, not ctx.backward_)
+        elif dk is not None:
+            dk, _ = rotate(positions, dk, None, False, not ctx.backward_)
+        return None, None, None, dq, dk
