@@ -47,6 +47,8 @@ constexpr int kStreaming = 2;  // nt: rows are read once
 // about as much as the rows of 16 units (5 us).
 constexpr int kMinUnits = 16;
 constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
+constexpr int kGroup = 16;  // pieces of a group of a join, and floats that are joined at once
+constexpr int kJoinAtOnce = 1 << 14;
 constexpr int kBeyond = 1 << 30;  // an offset behind every buffer
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -70,7 +72,8 @@ struct Args {
   bool out_vec;
   int cus;
   float *partial;
-  int *counters;
+  int *counters;        // [kMaxBlocks]: parts there of the segment cut first by a block
+  int *group_counters;  // [2 * kMaxBlocks]: pieces there of the group that a slot begins
 };
 
 // What differs between the types of the rows.
@@ -194,15 +197,19 @@ __device__ __forceinline__ void stores_done() {
 // A partial result: the rows' sums [16][DP], then (m, l) of each row.
 constexpr int part_floats(int dp) { return kTile * (dp + 2); }
 
-// The pieces of a cut segment together, by the block that finished last, in their order.
-// Threads beyond one per 4 channels of a row share the pieces; a thread has the loads of
-// kBatch pieces in flight at once.
+// Where piece k of a cut segment lies: the first one began it (slot 1 of its block), the
+// others go on with it (slot 0 of the blocks behind).
+__device__ __forceinline__ int piece_slot(int first, int k) {
+  return k == 0 ? 2 * first + 1 : 2 * (first + k);
+}
+
+// Pieces k0, k0 + step, ... (n of them) of a segment together, in their order, by the block
+// that finished last.  Threads beyond one per 4 channels of a row share the pieces; a thread
+// has the loads of kBatch pieces in flight at once.  put(row, channel, sums, max, sum).
 template <int DP, typename Put>
-__device__ __forceinline__ void join(const Args &g, const Piece &pc, int rows, int tid, float *lds,
-                                     Put put) {
+__device__ __forceinline__ void join(const Args &g, int first, int piece0, int step, int n,
+                                     int rows, int tid, float *lds, Put put) {
   constexpr int kPart = part_floats(DP);
-  // the first piece began the segment (slot 1 of its block), the others go on with it (slot 0)
-  const float *p0 = g.partial + (2 * (int64_t)pc.first + 1) * kPart;
   const int items = rows * (DP / 4), parts = max(1, kThreads / items);
   for (int i0 = 0; i0 < items; i0 += kThreads) {
     const int part = parts > 1 ? tid / items : 0;
@@ -212,20 +219,20 @@ __device__ __forceinline__ void join(const Args &g, const Piece &pc, int rows, i
     float m = -INFINITY, l = 0.0f;
     f32x4 y = {0, 0, 0, 0};
     if (mine)
-      for (int k0 = part; k0 < pc.pieces; k0 += parts * kBatch) {
+      for (int k0 = part; k0 < n; k0 += parts * kBatch) {
         float2 ml[kBatch];
         f32x4 x[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          const int k = min(k0 + j * parts, pc.pieces - 1);  // (the last again: no weight)
-          const float *from = p0 + (k ? 2 * k - 1 : 0) * (int64_t)kPart;
+          const int k = min(k0 + j * parts, n - 1);  // (the last again: no weight)
+          const float *from = g.partial + (int64_t)piece_slot(first, piece0 + k * step) * kPart;
           ml[j] = get_shared2(from + kTile * DP + 2 * row);
           x[j] = get_shared4(from + row * DP + d);
         }
         float top = m;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          if (k0 + j * parts >= pc.pieces) ml[j].x = -INFINITY;
+          if (k0 + j * parts >= n) ml[j].x = -INFINITY;
           top = fmaxf(top, ml[j].x);
         }
         if (top == -INFINITY) continue;
@@ -267,7 +274,7 @@ __device__ __forceinline__ void join(const Args &g, const Piece &pc, int rows, i
         }
       }
     }
-    if (mine && part == 0) put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
+    if (mine && part == 0) put(row, d, y, m, l);
   }
 }
 
@@ -707,9 +714,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
     }
     __syncthreads();
     char *o_at = static_cast<char *>(g.a.out) + (int64_t)seq * g.a.out_nb[1];
-    auto put = [&](int row, int d, f32x4 y) {
+    const auto put = [&](int row, int d, f32x4 y, float m, float l) {
       T *o = reinterpret_cast<T *>(o_at + (qh0 + row) * (int64_t)g.a.out_nb[0]) + d;
       if (d >= dim) return;
+      y = m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l;  // no tokens: zeros
       RowVec<T, 4> v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) row_put(v.x[i], y[i]);
@@ -721,6 +729,15 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
       }
     };
     constexpr int kPart = part_floats(DP);
+    int slot = 2 * blockIdx.x + pc.slot;  // where this block's part of a cut segment goes
+    const auto put_part = [&](int row, int d, f32x4 y) {
+      float *part = g.partial + (int64_t)slot * kPart + row * DP + d;
+      put_shared(part, y[0], y[1]);
+      put_shared(part + 2, y[2], y[3]);
+    };
+    const auto put_stats = [&](int row, float m, float l) {
+      put_shared(g.partial + (int64_t)slot * kPart + kTile * DP + 2 * row, m, l);
+    };
     for (int i = tid; i < rows * (DP / 4); i += kThreads) {
       const int row = i / (DP / 4), d = i % (DP / 4) * 4;
       float m = -INFINITY, l = 0.0f;
@@ -736,25 +753,53 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
         }
       }
       if (pc.whole) {
-        put(row, d, m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l);
+        put(row, d, y, m, l);
       } else {
-        float *part = g.partial + (int64_t)(2 * blockIdx.x + pc.slot) * kPart;
-        put_shared(part + row * DP + d, y[0], y[1]);
-        put_shared(part + row * DP + d + 2, y[2], y[3]);
-        if (d == 0) put_shared(part + kTile * DP + 2 * row, m, l);
+        put_part(row, d, y);
+        if (d == 0) put_stats(row, m, l);
       }
     }
     if (!pc.whole) {
-      stores_done();
-      __syncthreads();
-      if (tid == 0)
-        s_last = __hip_atomic_fetch_add(g.counters + pc.first, 1, __ATOMIC_RELAXED,
-                                        __HIP_MEMORY_SCOPE_AGENT) == pc.pieces - 1;
-      __syncthreads();
-      if (s_last) {
-        join<DP>(g, pc, rows, tid, &s_acc[0][0][0], put);
+      // Joined by the block that finishes last: all pieces at once, or, where they are more
+      // than 64 KB, by groups whose last blocks leave the group's part each, and those then
+      // (a CU reads some 20 GB/s past the caches.  65,536 tokens, one key head of 128, 16
+      // query heads: 256 pieces at once 93 us, in groups 27; 84 pieces of one row 20 and 22).
+      const int k = blockIdx.x - pc.first;
+      const bool grouped = pc.pieces > kGroup && pc.pieces * rows * DP > kJoinAtOnce;
+      int piece0 = grouped ? k / kGroup * kGroup : 0, step = 1;
+      int n = grouped ? min(kGroup, pc.pieces - piece0) : pc.pieces;
+      int *counter = grouped ? g.group_counters + piece_slot(pc.first, piece0)
+                             : g.counters + pc.first;
+      for (bool last = !grouped;; last = true) {
+        stores_done();
+        __syncthreads();
+        if (tid == 0)
+          s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+        __syncthreads();
+        if (!s_last) break;
         if (tid == 0)  // for the next call
-          __hip_atomic_store(g.counters + pc.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        slot = piece_slot(pc.first, piece0);
+        join<DP>(g, pc.first, piece0, step, n, rows, tid, &s_acc[0][0][0],
+                 [&](int row, int d, f32x4 y, float m, float l) {
+                   if (last) {
+                     put(row, d, y, m, l);
+                   } else {
+                     put_part(row, d, y);  // read by this item's threads alone
+                     if (d == 0) {
+                       s_m[0][row] = m;
+                       s_l[0][row] = l;
+                     }
+                   }
+                 });
+        if (last) break;
+        __syncthreads();  // every thread has read the first piece's (max, sum)
+        if (tid < rows) put_stats(tid, s_m[0][tid], s_l[0][tid]);
+        piece0 = 0;
+        step = kGroup;
+        n = (pc.pieces + kGroup - 1) / kGroup;
+        counter = g.counters + pc.first;
       }
     }
     __syncthreads();
@@ -799,7 +844,7 @@ hipError_t launch_type(const Args &g, hipStream_t s) {
 }  // namespace
 
 size_t paged_workspace_bytes(const PagedShape &p) {
-  return kMaxBlocks * (2 * sizeof(float) * part_floats(padded_dim(p.dim)) + sizeof(int));
+  return kMaxBlocks * (2 * sizeof(float) * part_floats(padded_dim(p.dim)) + 4 * sizeof(int));
 }
 
 hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
@@ -828,7 +873,8 @@ hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const Pa
   g.out_vec = x % (p.io == IoType::F32 ? 16 : 8) == 0;
   g.cus = p.cus;
   g.counters = static_cast<int *>(workspace);
-  g.partial = reinterpret_cast<float *>(g.counters + kMaxBlocks);
+  g.group_counters = g.counters + kMaxBlocks;
+  g.partial = reinterpret_cast<float *>(g.counters + 4 * kMaxBlocks);
   switch (p.io) {
     case IoType::F32: return launch_type<float>(g, s);
     case IoType::F16: return launch_type<_Float16>(g, s);

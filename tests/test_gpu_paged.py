@@ -132,6 +132,20 @@ def test_long(dtype, ps, lengths):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,group,lengths", [
+    (128, 1, [40000]), (128, 16, [2176]), (128, 16, [2177]), (128, 17, [9000]), (128, 3, [33000]),
+    (64, 16, [3000, 20000]), (256, 8, [5000]), (256, 16, [30000]), (80, 5, [8000, 1, 8000]),
+])
+def test_one_key_head(dtype, dim, group, lengths):
+    """Hundreds of pieces of one segment, joined by groups first."""
+    s = Server(lengths, 1, dim, 64, dtype, seed=group)
+    q = s.queries(group)
+    first = s.attend(q)
+    R.check(first, *s.want(q))
+    assert torch.equal(s.attend(q), first)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [1, 63, 64, 65, 300, 1000])
 def test_many_sequences(dtype, n):
     rng = random.Random(n)
