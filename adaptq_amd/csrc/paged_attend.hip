@@ -67,8 +67,8 @@ struct Args {
   int group, q_tiles;  // query heads of a key head, and their tiles of 16
   int segs;            // segments of a sequence
   int64_t cap;         // tokens that the table has columns for
-  uint64_t page_mul;   // blocks of 16 tokens -> pages: x * page_mul >> page_shift
-  int page_shift, page_blocks, row_bytes;
+  PageOf page_of;
+  int row_bytes;
   bool out_vec;
   int cus;
   float *partial;
@@ -337,10 +337,10 @@ struct Attend {
       w.page[s] = -1;
       w.slot[s] = 0;
       if (unit < u_end && b * 16 < span.n) {
-        const int col = (int)((uint64_t)(uint32_t)b * g.page_mul >> g.page_shift);
+        const int col = page_column(g.page_of, b);
         const int page = ((cint *)(uint64_t)table)[col];
         w.page[s] = page < g.p.n_pages ? page : -1;
-        w.slot[s] = (b - col * g.page_blocks) * 16;
+        w.slot[s] = (b - col * g.page_of.blocks) * 16;
       }
     }
     return w;
@@ -359,7 +359,7 @@ struct Attend {
 
   // A step's token: its rows, the key rotated, into its slot, by the wave that will load it.
   __device__ void append(int seq, int at) const {
-    const int col = (int)((uint64_t)(uint32_t)(at >> 4) * g.page_mul >> g.page_shift);
+    const int col = page_column(g.page_of, at >> 4);
     const int page = ((cint *)(uint64_t)table)[col];
     if (page < 0 || page >= g.p.n_pages) return;
     const int slot = at - col * g.p.page_size;
@@ -581,12 +581,13 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
   int64_t base = 0;
   uint64_t past = __ballot(e.end > start);
   int seq = 0;
-  while (!past) {  // (ends: start < total)
+  while (!past && seq + 64 < n_seqs) {
     base += uniform(e.end, 63);
     seq += 64;
     e = ends_of(g, lane, K::kUnit, seq);
     past = __ballot(base + e.end > start && seq + lane < n_seqs);
   }
+  if (!past) return;  // (only if the lengths changed under the call)
   const int first = __ffsll((unsigned long long)past) - 1;
   seq += first;
   int length = __builtin_amdgcn_readlane(e.length, first);
@@ -606,9 +607,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
   const auto next = [&](const Piece &pc) {
     at += pc.u1 - u0;
     u0 = 0;
-    if (++seg == g.segs && at < end) {
+    if (++seg == g.segs) {
       seg = 0;
-      length = ((cint *)(uint64_t)g.q.lengths)[++seq];
+      if (++seq < n_seqs) length = ((cint *)(uint64_t)g.q.lengths)[seq];
+      else at = end;
     }
   };
   while (at < end) {
@@ -650,7 +652,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
                        qh0 * (int64_t)g.a.q_nb[0];
     {
       float2 cs = make_float2(1.0f, 0.0f);
-      if (turns) cs = rotary_cos_sin(step, length < 0 ? 0 : length + g.a.extra - 1, rt.amplitude);
+      if (turns) cs = rotary_cos_sin(step, length < 0 ? 0 : length + (g.a.extra - 1), rt.amplitude);
       for (int row = tid / (DP / 2); row < rows; row += 2 * kThreads / DP) {
         const T *q = reinterpret_cast<const T *>(q_at + row * (int64_t)g.a.q_nb[0]);
         const float x = c0 < dim ? row_get(q[c0]) : 0.0f, y = c1 < dim ? row_get(q[c1]) : 0.0f;
@@ -807,6 +809,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
   }
 }
 
+// Blocks that the card holds at once: two a CU, one at d256.
+int most_blocks(int cus, int dp) { return std::min(kMaxBlocks, dp == 256 ? cus : 2 * cus); }
+
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 template <typename T, int DP>
@@ -820,10 +825,9 @@ hipError_t launch(const Args &g, hipStream_t s) {
   // heads of 8,192 tokens 315 us, with one 320; 1,666 segments of a few tokens 40 and 53).
   // Fewer segments than CUs are cut: into half as many pieces with one block a CU, and
   // joining them is what costs (one sequence of 32,768 tokens, 8 heads, 30 us, with two 35).
-  const int per_cu = DP == 256 || segments < g.cus ? 1 : 2;
+  const int resident = std::min(most_blocks(g.cus, DP), segments < g.cus ? g.cus : 2 * g.cus);
   const int64_t most = segments * std::max(longest, (int64_t)kMinUnits);
-  const int blocks = (int)std::min((most + kWaves - 1) / kWaves,
-                                   (int64_t)std::min(kMaxBlocks, g.cus * per_cu));
+  const int blocks = (int)std::min((most + kWaves - 1) / kWaves, (int64_t)resident);
   auto *kernel = g.p.dim == DP ? (g.n.k ? attend_kernel<T, DP, true, true>
                                         : attend_kernel<T, DP, true, false>)
                                : (g.n.k ? attend_kernel<T, DP, false, true>
@@ -844,7 +848,8 @@ hipError_t launch_type(const Args &g, hipStream_t s) {
 }  // namespace
 
 size_t paged_workspace_bytes(const PagedShape &p) {
-  return kMaxBlocks * (2 * sizeof(float) * part_floats(padded_dim(p.dim)) + 4 * sizeof(int));
+  return 4 * sizeof(int) * kMaxBlocks +
+         2 * sizeof(float) * part_floats(padded_dim(p.dim)) * most_blocks(p.cus, padded_dim(p.dim));
 }
 
 hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
@@ -859,16 +864,9 @@ hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const Pa
   g.group = a.q_heads / p.n_heads;
   g.q_tiles = (g.group + kTile - 1) / kTile;
   g.segs = p.n_heads * g.q_tiles;
-  g.cap = (int64_t)q.width * p.page_size;
-  // x / page_blocks for x < 2^27: the multiplier is rounded up by less than page_blocks
-  // parts of 2^page_shift, so the quotient is off by less than 2^27 / 2^page_shift * ... < 1
-  // part of page_blocks
-  g.page_blocks = p.page_size / 16;
+  g.cap = std::min((int64_t)q.width * p.page_size, (int64_t)kMaxTokens);
+  g.page_of = page_of_blocks(p.page_size);
   g.row_bytes = p.dim * (p.io == IoType::F32 ? 4 : 2);
-  int bits = 0;
-  while ((1 << bits) < g.page_blocks) ++bits;
-  g.page_shift = 27 + bits;
-  g.page_mul = (((uint64_t)1 << g.page_shift) + g.page_blocks - 1) / g.page_blocks;
   size_t x = reinterpret_cast<uintptr_t>(a.out) | a.out_nb[0] | a.out_nb[1];
   g.out_vec = x % (p.io == IoType::F32 ? 16 : 8) == 0;
   g.cus = p.cus;

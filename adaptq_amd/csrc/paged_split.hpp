@@ -22,6 +22,32 @@
 
 namespace aq {
 
+// Tokens of a sequence: whole units of them end within an int.
+constexpr int kMaxTokens = 0x7FFFFFE0;
+
+// Pages of blocks of 16 tokens: block b lies in page b / blocks = b * mul >> shift.  mul is
+// 2^shift / blocks rounded up, by less than one, so b * mul is over 2^shift * (b / blocks) by
+// less than b < 2^27: that is less than 2^shift / blocks, the distance to the next page, as
+// shift = 27 + log2(blocks) rounded up.
+struct PageOf {
+  uint64_t mul;
+  int shift, blocks;
+};
+
+inline PageOf page_of_blocks(int page_size) {
+  PageOf p;
+  p.blocks = page_size / 16;
+  int bits = 0;
+  while ((1 << bits) < p.blocks) ++bits;
+  p.shift = 27 + bits;
+  p.mul = (((uint64_t)1 << p.shift) + p.blocks - 1) / p.blocks;
+  return p;
+}
+
+AQ_SPLIT_HD int page_column(const PageOf &p, int block) {
+  return (int)((uint64_t)(uint32_t)block * p.mul >> p.shift);
+}
+
 // The tokens that a sequence's attention is over: [lo, n), and their units.
 struct TokenSpan {
   int lo, n;
@@ -38,8 +64,7 @@ AQ_SPLIT_HD TokenSpan token_span(int length, int extra, int window, int64_t cap,
   TokenSpan s;
   const int64_t lo = window > 0 && held > window ? held - window : 0;
   if (held > cap) held = cap;
-  // (whole units of int tokens: the last one of 2^31 - 1 would end beyond)
-  if (held > 0x7FFFFFE0) held = 0x7FFFFFE0;
+  if (held > kMaxTokens) held = kMaxTokens;
   s.n = (int)held;
   s.lo = (int)(lo < held ? lo : held);
   s.first_unit = s.lo / unit;

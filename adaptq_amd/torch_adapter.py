@@ -68,6 +68,10 @@ class AdaptQAttention(nn.Module):
         if self.rotary is not None:
             if not q.is_cuda:
                 raise ValueError("AdaptQAttention with rotary takes tensors on the GPU.")
+            if torch.cuda.is_current_stream_capturing():
+                # the position is the host's: a replay would rotate by the captured one
+                raise RuntimeError("AdaptQAttention with rotary cannot be captured; capture "
+                                   "Rotary with positions that the graph advances.")
             with torch.no_grad():
                 q, k = self.rotary(self._position(), q, k)
 

@@ -126,7 +126,20 @@ static void check_large() {
   }
 }
 
+static void check_pages() {
+  for (int blocks = 1; blocks <= 4096; ++blocks) {
+    const PageOf p = page_of_blocks(16 * blocks);
+    if (p.blocks != blocks) fail("page blocks");
+    for (int64_t b : {0ll, 1ll, (1ll << 27) - 1, (1ll << 27) - 2, (1ll << 26) + 7})
+      for (int64_t x : {b, b / blocks * blocks, b / blocks * blocks - 1, b / blocks * blocks + 1})
+        if (x >= 0 && x < 1ll << 27 && page_column(p, (int)x) != x / blocks) fail("page column");
+    for (int x = 0; x < 3 * blocks; ++x)
+      if (page_column(p, x) != x / blocks) fail("page column");
+  }
+}
+
 int main() {
+  check_pages();
   check_large();
   const int edge[] = {-2147483647 - 1, -1, 0, 1, 15, 16, 17, 31, 32, 33, 1000, 2147483615, 2147483647};
   for (int n : edge)

@@ -263,6 +263,20 @@ def test_tokens_without_a_page_are_left_out(dtype):
     R.check(s.attend(q), *s.want(q))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_run_without_pages(dtype):
+    """Whole pieces of a cut sequence have no page: 4,000 tokens in the middle, or all."""
+    s = Server([6000, 6000], 1, 64, 16, dtype)
+    q = s.queries(4)
+    s.table_host[0, 50:300] = -1
+    s.table_host[1, :] = 2 ** 31 - 1
+    s.table.copy_(s.table_host[:, :s.table.shape[1]])
+    keep = [*range(800), *range(4800, 6000)]
+    s.k[0], s.v[0] = s.k[0][keep], s.v[0][keep]
+    s.k[1], s.v[1] = s.k[1][:0], s.v[1][:0]
+    R.check(s.attend(q), *s.want(q))
+
+
 def test_table_of_no_width():
     s = Server([0, 0], 1, 64, 16, torch.float32)
     q = s.queries(2)
@@ -619,6 +633,47 @@ def test_refusals():
         with pytest.raises(kind):
             call()
     R.check(s.attend(q), *s.want(q))  # refused calls left nothing behind
+
+
+def test_c_refusals():
+    """The C entries by themselves: null pointers, counts and strides that make no sense."""
+    k = torch.zeros(2, 2, 16, 64, device="cuda")
+    v = torch.zeros_like(k)
+    args = [k.data_ptr(), v.data_ptr(), 2, 16, 2, 64, 0, None]
+    for i, x in ((0, None), (1, None), (0, k.data_ptr() + 4), (2, 0), (2, -1), (3, 0), (3, 24),
+                 (3, 1 << 17), (4, 0), (4, 1 << 20), (5, 0), (5, 12), (5, 512), (6, 3),
+                 (1, k.data_ptr() + 4096)):
+        bad = list(args)
+        bad[i] = x
+        assert L.adaptq_paged_create(*bad) is None, (i, x)
+        assert _lib.last_error().startswith("adaptq_paged_create: ")
+    h = L.adaptq_paged_create(*args)
+    assert h, _lib.last_error()
+    t = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    n = torch.zeros(2, dtype=torch.int32, device="cuda")
+    q, o = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, 4, 64, device="cuda")
+    at = [h, q.data_ptr(), o.data_ptr(), 4, 256, 1024, 256, 1024, t.data_ptr(), 1, 1, n.data_ptr(),
+          2, 0.0, 0, None]
+    assert L.adaptq_paged_attend_device(*at) == 0
+    for i, x in ((0, None), (1, None), (2, None), (2, q.data_ptr()), (3, 0), (3, 3), (3, -4), (4, 2),
+                 (5, 2 ** 62), (6, 128), (7, 512), (8, None), (8, t.data_ptr() + 1), (9, -1), (9, 2),
+                 (11, None), (12, -1), (12, 2 ** 31 - 1), (13, float("inf")), (14, -1)):
+        bad = list(at)
+        bad[i] = x
+        assert L.adaptq_paged_attend_device(*bad) == -1, (i, x)
+        assert _lib.last_error().startswith("adaptq_paged_attend_device: ")
+    ap = [h, q.data_ptr(), o.data_ptr(), 2, 256, 1024, 256, 1024, t.data_ptr(), 1, 1, n.data_ptr(),
+          2, None, None]
+    assert L.adaptq_paged_append_device(*ap) == 0
+    for i, x in ((0, None), (1, None), (2, None), (1, k.data_ptr()), (3, -1), (3, 1), (4, 6),
+                 (8, None), (10, 0), (11, None), (12, 3), (13, n.data_ptr() + 2)):
+        bad = list(ap)
+        bad[i] = x
+        assert L.adaptq_paged_append_device(*bad) == -1, (i, x)
+    torch.cuda.synchronize()
+    L.adaptq_paged_destroy(h)
+    L.adaptq_paged_destroy(None)
+    L.adaptq_rotary_destroy(None)
 
 
 def test_handle_outlives_its_rotary():

@@ -273,11 +273,11 @@ def test_torch_adapter(Rotary, dtype):
     a = AdaptQAttention(D, H, seed=3, rotary=rotary)
     b = AdaptQAttention(D, H, seed=3)
     g = torch.Generator().manual_seed(1)
-    a.engine.pos = b.engine.pos = 4090
-    for t in list(range(4090, 4100)) + list(range(3)):
+    for t in [0, *range(4090, 4100), 0, 1, 2]:  # the module holds 4,096 positions at a time
         if t == 0:
             a.reset_cache()
             b.reset_cache()
+        a.engine.pos = b.engine.pos = t
         q, k, v = (torch.randn(1, H, D, generator=g).to(dtype).cuda()
                    for _ in range(3))
         q0, k0 = q.clone(), k.clone()
@@ -287,3 +287,10 @@ def test_torch_adapter(Rotary, dtype):
         assert torch.equal(q, q0) and torch.equal(k, k0)
     with pytest.raises(ValueError):
         a(q.cpu(), k.cpu(), v.cpu())
+    torch.cuda.synchronize()
+    graph, y = torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        y.add_(1)
+        with pytest.raises(RuntimeError, match="captured"):
+            a(q, k, v)
+    assert a.engine.pos == 3
