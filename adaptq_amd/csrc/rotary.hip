@@ -43,6 +43,32 @@ struct Shape {
   bool backward;
 };
 
+// Cosines and sines of a token's pairs in LDS: two pairs (16 bytes) of each chunk of N side
+// by side for all its chunks, then the next two, so that threads of neighbouring chunks read
+// neighbouring words: 29.6 us instead of 30.5 with a chunk's pairs in a row.  (The append
+// keeps them in a row: it gains nothing, and prompts over 4 heads lose 5 %.)
+template <int N>
+__device__ __forceinline__ int cos_sin_at(int pair, int chunks) {
+  if (N == 1) return pair;
+  const int j = pair % N;
+  return (j / 2 * chunks + pair / N) * 2 + j % 2;
+}
+template <int N>
+__device__ __forceinline__ void get_cos_sin(const float2 *of_token, int chunk, int chunks,
+                                            float2 (&cs)[N]) {
+  if constexpr (N == 1) {
+    cs[0] = of_token[chunk];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float4 x =
+          *reinterpret_cast<const float4 *>(of_token + (j / 2 * chunks + chunk) * 2);
+      cs[j] = make_float2(x.x, x.y);
+      cs[j + 1] = make_float2(x.z, x.w);
+    }
+  }
+}
+
 template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const Shape s) {
   typedef RowVec<T, N> Vec;
@@ -89,9 +115,11 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Shape s) {
 
   for (int i = tid; i < nt * s.r.pairs; i += kThreads) {
     const int j = i / s.r.pairs, t = t0 + j, batch = s.n_batch > 1 ? t / s.n_tokens : 0;
-    s_cs[i] = rotary_cos_sin(s.r.steps[i - j * s.r.pairs],
-                             s.positions[batch * s.pos_stride + (t - batch * s.n_tokens)],
-                             s.r.amplitude);
+    const int pair = i - j * s.r.pairs;
+    s_cs[j * s.r.pairs + cos_sin_at<N>(pair, chunks)] =
+        rotary_cos_sin(s.r.steps[pair],
+                       s.positions[batch * s.pos_stride + (t - batch * s.n_tokens)],
+                       s.r.amplitude);
   }
   __syncthreads();
 
@@ -102,8 +130,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Shape s) {
       if (row >= n_rows) break;
       if (item < chunks) {
         const int tok = (int)((uint64_t)row * s.head_mul >> 32);
-        rotate_pairs<T, N>(u[j], v[j], s_cs + tok * s.r.pairs + item * N, s.r.interleaved,
-                           s.backward);
+        float2 cs[N];
+        get_cos_sin<N>(s_cs + tok * s.r.pairs, item, chunks, cs);
+        rotate_pairs<T, N>(u[j], v[j], cs, s.r.interleaved, s.backward);
       }
       T *out = reinterpret_cast<T *>(place(row, true));
       store_rows<false>(out + at.x, u[j]);
