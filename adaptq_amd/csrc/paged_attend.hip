@@ -46,9 +46,9 @@ constexpr int kStreaming = 2;  // nt: rows are read once
 // What a segment counts at the least, and what is never cut: its start and end cost a block
 // about as much as the rows of 16 units (5 us).
 constexpr int kMinUnits = 16;
-constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
-constexpr int kGroup = 16;  // pieces of a group of a join, and floats that are joined at once
-constexpr int kJoinAtOnce = 1 << 14;
+constexpr int kBatch = 8;             // pieces of a join whose loads are in flight at once
+constexpr int kGroup = 16;            // pieces of a group of a join
+constexpr int kJoinAtOnce = 1 << 14;  // floats that are joined without groups
 constexpr int kBeyond = 1 << 30;  // an offset behind every buffer
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -142,8 +142,8 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, Bf16) {
 }
 
 // Two values as hi + lo: hi the largest number of the type that is below (in magnitude),
-// lo the rest, rounded.  lo is never 0 for a value that is not, and has its sign: a product
-// with an infinity stays that infinity.
+// lo the rest, rounded.  lo has the value's sign and is not 0 for one that is not (in fp16
+// from 2^-12 on): a product with an infinity stays that infinity.
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, _Float16) {
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   const float a = __uint_as_float(__float_as_uint(x) - (x != 0.0f));
@@ -387,7 +387,6 @@ struct Attend {
   }
 
   __device__ void load(Rows &r, const Where &w, int unit) const {
-
     const int t0 = unit * K::kUnit;
     // (opaque here, so that what is added stays part of the loads instead of taking a
     // register each outside the loop)
@@ -632,7 +631,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
     const int64_t qh0 = (int64_t)head * g.group + q0;
     w.head = head;
     w.table = g.q.table + (int64_t)seq * g.q.stride;
-    w.u_end = w.span.first_unit + pc.u1;
+    // (a short segment counts for more units than it has)
+    w.u_end = min(w.span.first_unit + pc.u1, (w.span.n + K::kUnit - 1) / K::kUnit);
     int u = w.span.first_unit + u0 + wave;
 
     if (STEP && length >= 0 && length < g.cap) {
