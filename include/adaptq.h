@@ -374,8 +374,8 @@ long long adaptq_plan_workspace_bytes(adaptq_plan_t plan);
  *   YARN    the same with the ramp linear in i, between the floor of the pair that
  *           turns `fast` times and the ceiling of the one that turns `slow` times
  *           (kept within 0 and rotary_dim - 1)
- * slow, fast: 0 = 1 and 4 (YARN: 1 and 32).  amplitude a: 0 = 1 (YARN:
- * 0.1 ln(factor) + 1).  Angles are exact to 2^-33 of a turn at every position.
+ * slow, fast: 0 = 1 and 4 (YARN: 1 and 32).  factor at least 1, base above 1,
+ * rotary_dim even, from 2 to 1024.  amplitude a: 0 = 1 (YARN: 0.1 ln(factor) + 1).  Angles are exact to 2^-33 of a turn at every position.
  * Returns NULL and sets the last error on invalid arguments. */
 typedef void *adaptq_rotary_t;
 enum {
@@ -414,10 +414,10 @@ int adaptq_rotary_device(adaptq_rotary_t rotary, const adaptq_rows_t *rows, int 
 /* A cache over two pools of pages that the caller holds, [n_pages][n_heads]
  * [page_size][dim] of io_type, 16-byte aligned: page_size a multiple of 16 up to
  * 65536, dim a multiple of 8 up to 256.  The handle keeps the pools' addresses and
- * the few MB of workspace that its attention needs; it copies `rotary` (NULL: rows
+ * the workspace that its attention needs (8.5 MB at dim 128); it copies `rotary` (NULL: rows
  * are taken as they are), by which appended keys and the queries of attention are
  * rotated.  Several handles may share pools.  Calls on one handle from different
- * streams (graph replays too) must be ordered by the caller. */
+ * streams (graph replays too) must be ordered by the caller.  n_heads up to 32768. */
 typedef void *adaptq_paged_t;
 adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
                                    int n_heads, int dim, int io_type, adaptq_rotary_t rotary);
