@@ -18,6 +18,7 @@ _f = C.POINTER(C.c_float)
 _u8 = C.POINTER(C.c_uint8)
 _ip = C.POINTER(C.c_int)
 
+
 class Rows(C.Structure):
     """adaptq_rows_t"""
     _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("n_heads", C.c_int),

@@ -8,7 +8,6 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
-#include <mutex>
 #include <new>
 #include <vector>
 

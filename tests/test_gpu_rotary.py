@@ -196,6 +196,30 @@ def test_side_stream_and_graph(Rotary):
         assert torch.equal(y, rotary(pos, q))
 
 
+def test_captured_backward(Rotary):
+    """Forward and gradient in one graph, on leaves that no eager graph holds; replays follow
+    the rows, the positions and the outputs' gradient."""
+    rotary, pos = Rotary(64), _positions(24, 3)
+    q, k = (_rows((24, h, 64), torch.float32, h).requires_grad_() for h in (4, 2))
+    gq, gk = torch.empty_like(q), torch.empty_like(k)
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        yq, yk = rotary(pos, q, k)
+        dq, dk = torch.autograd.grad((yq, yk), (q, k), (gq, gk))
+    for i in range(3):
+        with torch.no_grad():
+            for j, x in enumerate((q, k, gq, gk)):
+                x.copy_(_rows(x.shape, torch.float32, 10 * i + j))
+            pos.add_(77)
+        graph.replay()
+        torch.cuda.synchronize()
+        for y, x in ((yq, q), (yk, k)):
+            R.check(y, *R.rotate(x, pos, 64))
+        for d, g in ((dq, gq), (dk, gk)):
+            R.check(d, *R.rotate(g, pos, 64, backward=True))
+
+
 def test_empty(Rotary):
     rotary = Rotary(64)
     for shape in ((0, 4, 64), (0, 5, 4, 64), (2, 0, 4, 64)):
