@@ -821,12 +821,17 @@ hipError_t launch(const Args &g, hipStream_t s) {
   int64_t longest = (g.cap + unit - 1) / unit;
   if (g.a.window > 0) longest = std::min(longest, (int64_t)g.a.window / unit + 2);
   const int64_t segments = g.q.n_seqs * (int64_t)g.segs;
-  // Two blocks a CU overlap one's ends of segments with the other's rows (64 sequences x 8
-  // heads of 8,192 tokens 315 us, with one 320; 1,666 segments of a few tokens 40 and 53).
-  // Fewer segments than CUs are cut: into half as many pieces with one block a CU, and
-  // joining them is what costs (one sequence of 32,768 tokens, 8 heads, 30 us, with two 35).
-  const int resident = std::min(most_blocks(g.cus, DP), segments < g.cus ? g.cus : 2 * g.cus);
   const int64_t most = segments * std::max(longest, (int64_t)kMinUnits);
+  // Two blocks a CU overlap one's ends of segments with the other's rows (64 sequences x 8
+  // heads of 8,192 tokens 315 us, with one 320; 88 segments of up to 20 units 17.6 and 18.9;
+  // 1,666 of a few tokens 40 and 53), and with little work a wave of theirs has one unit
+  // where it would have two (28 segments of 63 units 16.0 and 17.5).  Few long segments are
+  // cut into twice as many pieces by them, and joining those costs more (one sequence of
+  // 32,768 tokens, 8 heads: 35 us, with one block a CU 30; 36 segments of 128 units 25 and
+  // 23.3; one segment of 2,048 units, 8 query heads 24.5 and 19.8).
+  const bool few_long = segments < g.cus / 16 ||
+                        (segments < g.cus / 4 && most > 2 * kWaves * (int64_t)g.cus);
+  const int resident = std::min(most_blocks(g.cus, DP), few_long ? g.cus : 2 * g.cus);
   const int blocks = (int)std::min((most + kWaves - 1) / kWaves, (int64_t)resident);
   auto *kernel = g.p.dim == DP ? (g.n.k ? attend_kernel<T, DP, true, true>
                                         : attend_kernel<T, DP, true, false>)

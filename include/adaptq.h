@@ -450,8 +450,8 @@ int adaptq_paged_append_device(adaptq_paged_t cache, const void *d_k, const void
  * is the token n - 1 (its rotation).  scale: of the scores, 0 = 1 / sqrt(dim).
  * Products and sums in fp32 or closer, rounded once.  Tokens without a page are left
  * out, as above; a sequence with no tokens gets zeros.  The order of the sums depends
- * on the lengths alone, so equal calls give equal bits.  d_out may not overlap d_q.
- * Returns 0/-1. */
+ * on the call's shape and the lengths alone, so equal calls give equal bits.  d_out may
+ * not overlap d_q.  Returns 0/-1. */
 int adaptq_paged_attend_device(adaptq_paged_t cache, const void *d_q, void *d_out, int n_q_heads,
                                size_t q_nb1, size_t q_nb2, size_t out_nb1, size_t out_nb2,
                                const int *d_table, int table_width, int table_stride,
