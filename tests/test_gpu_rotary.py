@@ -196,6 +196,24 @@ def test_side_stream_and_graph(Rotary):
         assert torch.equal(y, rotary(pos, q))
 
 
+def test_offsets_beyond_32_bits(Rotary):
+    """Rows more than 2^32 bytes from the first, of one token set and of a batch."""
+    tokens, heads, dim = 140000, 128, 128
+    q = torch.zeros(tokens, heads, dim, dtype=torch.bfloat16, device="cuda")
+    assert q.numel() * 2 > 2 ** 32
+    last = _rows((3, heads, dim), torch.bfloat16)
+    q[-3:] = last
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    rotary = Rotary(64, interleaved=True)
+    want = R.rotate(last, pos[-3:], 64, True)
+    y = rotary(pos, q)
+    R.check(y[-3:], *want)
+    assert not y[:-3].any()
+    del y
+    rotary(pos.view(20, -1), q.view(20, -1, heads, dim), inplace=True)
+    R.check(q[-3:], *want)
+
+
 def test_captured_backward(Rotary):
     """Forward and gradient in one graph, on leaves that no eager graph holds; replays follow
     the rows, the positions and the outputs' gradient."""
