@@ -182,8 +182,8 @@ bool attend_ok(const Paged *p, const void *q, const void *out, int q_heads, int 
     set_errorf(fn, "n_q_heads must be a multiple of the cache's n_heads, up to 32768");
     return false;
   }
-  if (!std::isfinite(scale)) {
-    set_errorf(fn, "scale must be finite");
+  if (!std::isfinite(scale * 1.5f)) {  // the kernel takes it times log2(e)
+    set_errorf(fn, "scale must be finite, up to 2.2e38");
     return false;
   }
   if (window < 0) {
@@ -243,8 +243,8 @@ adaptq_rotary_t adaptq_rotary_create(int rotary_dim, int interleaved, double bas
   }
   const bool ramp = scaling == ADAPTQ_ROTARY_YARN || scaling == ADAPTQ_ROTARY_BANDS;
   if (!(std::isfinite(base) && base > 1.0) || !(std::isfinite(factor) && factor >= 1.0) ||
-      !(std::isfinite(amplitude) && amplitude >= 0.0)) {
-    set_errorf(fn, "base must be above 1, factor at least 1, amplitude not negative");
+      !(std::isfinite((float)amplitude) && amplitude >= 0.0)) {
+    set_errorf(fn, "base must be above 1, factor at least 1, amplitude not negative (nor beyond fp32)");
     return nullptr;
   }
   if (scaling == ADAPTQ_ROTARY_NTK && rotary_dim == 2) {

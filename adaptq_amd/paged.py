@@ -143,8 +143,8 @@ class PagedCache:
             raise ValueError("q holds one query a sequence")
         if window is not None and window <= 0:
             raise ValueError(f"window must be positive, got {window}")
-        if scale is not None and scale == 0:
-            raise ValueError("scale must not be 0")
+        if scale is not None and abs(scale) < 2.0 ** -126:  # 0 in fp32 would mean 1/sqrt(dim)
+            raise ValueError(f"scale must not be 0 in fp32, got {scale}")
         if out is None:
             out = torch.empty_like(q)  # its rows' values side by side, as q's are
         elif self._rows(out, "out", 0) is not out or out.shape != q.shape:

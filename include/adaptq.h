@@ -375,8 +375,9 @@ long long adaptq_plan_workspace_bytes(adaptq_plan_t plan);
  *           turns `fast` times and the ceiling of the one that turns `slow` times
  *           (kept within 0 and rotary_dim - 1)
  * slow, fast: 0 = 1 and 4 (YARN: 1 and 32).  factor at least 1, base above 1,
- * rotary_dim even, from 2 to 1024.  amplitude a: 0 = 1 (YARN: 0.1 ln(factor) + 1).  Angles are exact to 2^-33 of a turn at every position.
- * Returns NULL and sets the last error on invalid arguments. */
+ * rotary_dim even, from 2 to 1024.  amplitude a: 0 = 1 (YARN: 0.1 ln(factor) + 1).
+ * Angles are exact to 2^-33 of a turn at every position.  Returns NULL and sets the last
+ * error on invalid arguments. */
 typedef void *adaptq_rotary_t;
 enum {
   ADAPTQ_ROTARY_PLAIN = 0,
@@ -414,9 +415,9 @@ int adaptq_rotary_device(adaptq_rotary_t rotary, const adaptq_rows_t *rows, int 
 /* A cache over two pools of pages that the caller holds, [n_pages][n_heads]
  * [page_size][dim] of io_type, 16-byte aligned: page_size a multiple of 16 up to
  * 65536, dim a multiple of 8 up to 256.  The handle keeps the pools' addresses and
- * the workspace that its attention needs (8.5 MB at dim 128); it copies `rotary` (NULL: rows
- * are taken as they are), by which appended keys and the queries of attention are
- * rotated.  Several handles may share pools.  Calls on one handle from different
+ * the workspace that its attention needs (8.5 MB at dim 128); it copies `rotary`
+ * (NULL: rows are taken as they are), by which appended keys and the queries of
+ * attention are rotated.  Several handles may share pools.  Calls on one handle from different
  * streams (graph replays too) must be ordered by the caller.  n_heads up to 32768. */
 typedef void *adaptq_paged_t;
 adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
@@ -447,7 +448,7 @@ int adaptq_paged_append_device(adaptq_paged_t cache, const void *d_k, const void
 /* attend: one query per sequence and query head, d_q and d_out [n_seqs][n_q_heads]
  * [dim]; query heads h * g to h * g + g - 1 (g = n_q_heads / n_heads) attend over key
  * head h's tokens [max(0, n - window), n), n = d_lengths[b]; window 0: all.  The query
- * is the token n - 1 (its rotation).  scale: of the scores, 0 = 1 / sqrt(dim).
+ * is the token n - 1 (its rotation).  scale: of the scores, 0 = 1 / sqrt(dim), finite.
  * Products and sums in fp32 or closer, rounded once.  Tokens without a page are left
  * out, as above; a sequence with no tokens gets zeros.  The order of the sums depends
  * on the call's shape and the lengths alone, so equal calls give equal bits.  d_out may

@@ -635,6 +635,19 @@ def test_refusals():
     R.check(s.attend(q), *s.want(q))  # refused calls left nothing behind
 
 
+@pytest.mark.parametrize("scale,kind", [
+    (1e-60, ValueError), (-1e-46, ValueError),  # 0 in fp32, which stands for 1/sqrt(dim)
+    (3e38, RuntimeError), (-3e38, RuntimeError), (1e300, (RuntimeError, TypeError))])
+def test_scales_beyond_fp32(scale, kind):
+    s = Server([4, 9], 2, 64, 16, torch.float16)
+    q, k = s.queries(4), s.normal(2, 2, 64).cuda()
+    with pytest.raises(kind):
+        s.cache.attend(q, s.table, s.lengths, scale=scale)
+    with pytest.raises(kind):
+        s.cache.step(q, k, k, s.table, s.lengths, scale=scale)
+    R.check(s.attend(q), *s.want(q))
+
+
 def test_c_refusals():
     """The C entries by themselves: null pointers, counts and strides that make no sense."""
     k = torch.zeros(2, 2, 16, 64, device="cuda")

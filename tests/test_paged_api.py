@@ -68,3 +68,10 @@ def test_python_side_rejects_the_cpu():
         PagedCache(x, torch.zeros_like(x))
     with pytest.raises(TypeError):
         PagedCache(x.double(), x.double())
+
+
+@pytest.mark.parametrize("amplitude", [1e39, 1e300])
+def test_rotary_create_rejects_an_amplitude_beyond_fp32(lib, amplitude):
+    """It would be infinite on the device, and 0 times it NaN."""
+    assert lib.adaptq_rotary_create(*{**GOOD, "amplitude": amplitude}.values()) is None
+    assert b"amplitude" in lib.adaptq_last_error() and b"HIP" not in lib.adaptq_last_error()
