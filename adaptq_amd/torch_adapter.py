@@ -41,6 +41,8 @@ class AdaptQAttention(nn.Module):
     def _position(self) -> torch.Tensor:
         at = self.engine.pos - self._first
         if self._positions is None or not 0 <= at < self._positions.shape[0]:
+            if self._positions is not None:  # calls on this stream may still read them
+                self._positions.record_stream(torch.cuda.current_stream(self.rotary.device))
             self._first, at = self.engine.pos, 0
             self._positions = torch.arange(self._first, self._first + 4096, dtype=torch.int32,
                                            device=self.rotary.device)
