@@ -4,9 +4,9 @@
     q, k = rotary(positions, q, k)         # [tokens, heads, dim] or [batch, tokens, heads, dim]
 
 Device tensors of fp32, fp16 or bf16, rotated in one launch on torch's current
-stream, in fp32 and rounded once.  Differentiable in q and k.  Calls may be captured into a graph, a backward
-pass only together with its forward, on leaves that no graph outside the capture holds (as
-torch wants it of any operator).
+stream, in fp32 and rounded once.  Differentiable in q and k.  Calls may be captured
+into a graph, a backward pass only together with its forward, on leaves that no graph
+outside the capture holds (as torch wants it of any operator).
 """
 from __future__ import annotations
 
