@@ -24,7 +24,8 @@
 //
 // Precision: scores, statistics and sums in fp32.  Rotated queries and weights enter
 // the half-precision products as the sum of two numbers of that type, which leaves
-// 2^-16 of them (bf16) or 2^-20 (fp16), so the output's own rounding is the only one
+// 2^-16 of them (bf16) or 2^-20 (fp16, scaled by a power of two a row so that none of
+// them is too large or too small for it), so the output's own rounding is the only one
 // of its size; fp32 rows use the fp32 matrix instructions.
 #include <float.h>
 
@@ -142,7 +143,8 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, Bf16) {
 
 // Two values as hi + lo: hi the largest number of the type that is below (in magnitude),
 // lo the rest, rounded.  lo has the value's sign and is not 0 for one that is not (in fp16
-// from 2^-12 on): a product with an infinity stays that infinity.
+// from 2^-12 on; queries and weights come scaled, their largest to 2^14 or more): a product
+// with an infinity stays that infinity.
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, _Float16) {
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   const float a = __uint_as_float(__float_as_uint(x) - (x != 0.0f));
@@ -304,6 +306,7 @@ struct Attend {
   int head, u_end;
   u32x4 qh[K::kHalf ? kQ : 1], ql[K::kHalf ? kQ : 1];
   float qf[K::kHalf ? 1 : kQ];
+  int q_shift = 0;  // fp16: the operands are the query times 2^-q_shift
 
   __device__ Attend(const Args &args, int lane_)
       : g(args), lane(lane_), row16(lane_ & 15), group4(lane_ >> 4) {
@@ -454,7 +457,14 @@ struct Attend {
       s[0] += s2;
     }
 #pragma unroll
-    for (int i = 0; i < K::kSubs; ++i) s[i] *= g.scale2;
+    for (int i = 0; i < K::kSubs; ++i)
+      if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[i][j] = __builtin_amdgcn_ldexpf(s[i][j], q_shift) * g.scale2;
+      } else {
+        s[i] *= g.scale2;
+      }
     if (!full) {
 #pragma unroll
       for (int i = 0; i < K::kSubs; ++i)
@@ -663,11 +673,27 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
     __syncthreads();
     // (rows that are no query's hold anything: their columns of the products go nowhere)
     if constexpr (K::kHalf) {
+      // A rotated fp16 query may lie anywhere in fp32's range (the amplitude): the row's largest
+      // value is taken to 2^14 to 2^15, where two fp16 numbers hold 2^-20 of it and of every
+      // value down to 2^-16 of it, and 2^-38 of the largest below that; exact, as the shift is a
+      // power of two.  (An infinity or NaN makes the row's scores that, whatever the rest.)
+      if constexpr (__is_same(T, _Float16)) {
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < K::kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            top = fmaxf(top, fabsf(s_acc[0][w.row16][w.k_channel(c) + i]));
+        w.q_shift = __builtin_amdgcn_frexp_expf(cross_max(top)) - 15;
+      }
 #pragma unroll
       for (int c = 0; c < K::kChunks; ++c) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s_acc[0][w.row16][w.k_channel(c) + i];
+        for (int i = 0; i < 8; ++i) {
+          x[i] = s_acc[0][w.row16][w.k_channel(c) + i];
+          if constexpr (__is_same(T, _Float16)) x[i] = __builtin_amdgcn_ldexpf(x[i], -w.q_shift);
+        }
         split8<T>(x, w.qh[c], w.ql[c]);
       }
     } else {
