@@ -22,11 +22,12 @@
 //   numbers of the one behind it before that.
 // * Work is cut evenly over the resident blocks whatever the lengths (paged_split.hpp).
 //
-// Precision: scores, statistics and sums in fp32.  Rotated queries and weights enter
-// the half-precision products as the sum of two numbers of that type, which leaves
-// 2^-16 of them (bf16) or 2^-20 (fp16, scaled by a power of two a row so that none of
-// them is too large or too small for it), so the output's own rounding is the only one
-// of its size; fp32 rows use the fp32 matrix instructions.
+// Precision: scores, statistics and sums in fp32.  Queries and weights enter the
+// half-precision products as the sum of three bf16 numbers, which holds fp32's 24 bits,
+// or of two fp16 numbers, which leaves 2^-20 of them (scaled by a power of two a row so
+// that none is too large or too small for it): 2^-9 of the output's own rounding.  (Two
+// bf16 numbers, 2^-16, left one output of some hundreds a rounding away from fp32's.)
+// fp32 rows use the fp32 matrix instructions.
 #include <float.h>
 
 #include <algorithm>
@@ -88,6 +89,8 @@ struct Kind {
   static constexpr int kVVec = DP / 16 < kVec ? DP / 16 : kVec;
   static constexpr int kVChunks = DP / (16 * kVVec);
   static constexpr int kVRows = kUnit / 4;  // rows of V that a lane loads
+  // numbers of the type that queries and weights are cut into
+  static constexpr int kTerms = !kHalf ? 1 : __is_same(T, _Float16) ? 2 : 3;
 };
 
 template <int BYTES>
@@ -141,34 +144,40 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, Bf16) {
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Two values as hi + lo: hi the largest number of the type that is below (in magnitude),
-// lo the rest, rounded.  lo has the value's sign and is not 0 for one that is not (in fp16
-// from 2^-12 on; queries and weights come scaled, their largest to 2^14 or more): a product
-// with an infinity stays that infinity.
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, _Float16) {
+// Two values as sums of numbers of the type: the first the largest one that is below (in
+// magnitude), the next the same of the rest or, as the last, the rest rounded.  Each has the
+// value's sign and is not 0 for a value that is not (in fp16 from 2^-12 on, of what comes scaled
+// to 2^14 and more; in bf16 from 2^-100 on): a product with an infinity stays that infinity.
+__device__ __forceinline__ uint32_t below(float x) { return __float_as_uint(x) - (x != 0.0f); }
+
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&t)[2], _Float16) {
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-  const float a = __uint_as_float(__float_as_uint(x) - (x != 0.0f));
-  const float b = __uint_as_float(__float_as_uint(y) - (y != 0.0f));
-  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-  const v2 h = __builtin_bit_cast(v2, hi);
-  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
+  t[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(below(x)),
+                                                                 __uint_as_float(below(y))));
+  const v2 h = __builtin_bit_cast(v2, t[0]);
+  t[1] = __builtin_bit_cast(uint32_t,
+                            __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
 }
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, Bf16) {
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&t)[3], Bf16) {
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-  const uint32_t a = __float_as_uint(x) - (x != 0.0f), b = __float_as_uint(y) - (y != 0.0f);
-  hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
-  lo = __builtin_bit_cast(uint32_t, v2{(__bf16)(x - __uint_as_float(a & 0xFFFF0000u)),
-                                       (__bf16)(y - __uint_as_float(b & 0xFFFF0000u))});
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t a = below(x), b = below(y);
+    t[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    x -= __uint_as_float(a & 0xFFFF0000u);
+    y -= __uint_as_float(b & 0xFFFF0000u);
+  }
+  t[2] = __builtin_bit_cast(uint32_t, v2{(__bf16)x, (__bf16)y});
 }
 
-template <typename T>
-__device__ __forceinline__ void split8(const float *x, u32x4 &hi, u32x4 &lo) {
+template <typename T, int TERMS>
+__device__ __forceinline__ void split8(const float *x, u32x4 (&to)[TERMS]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t h, l;
-    split2(x[2 * i], x[2 * i + 1], h, l, T());
-    hi[i] = h;
-    lo[i] = l;
+    uint32_t t[TERMS];
+    split2(x[2 * i], x[2 * i + 1], t, T());
+#pragma unroll
+    for (int j = 0; j < TERMS; ++j) to[j][i] = t[j];
   }
 }
 
@@ -304,12 +313,13 @@ struct Attend {
   TokenSpan span;
   const int *table;
   int head, u_end;
-  u32x4 qh[K::kHalf ? kQ : 1], ql[K::kHalf ? kQ : 1];
+  u32x4 qh[K::kHalf ? kQ : 1];  // the first numbers of the queries; the others are in LDS:
+  const u32x4 *q_low;           // [kTerms - 1][kChunks][64 lanes]
   float qf[K::kHalf ? 1 : kQ];
   int q_shift = 0;  // fp16: the operands are the query times 2^-q_shift
 
-  __device__ Attend(const Args &args, int lane_)
-      : g(args), lane(lane_), row16(lane_ & 15), group4(lane_ >> 4) {
+  __device__ Attend(const Args &args, int lane_, const u32x4 *low)
+      : g(args), lane(lane_), row16(lane_ & 15), group4(lane_ >> 4), q_low(low + lane_) {
     const int row = g.row_bytes, size = (int)sizeof(T);
     if (EXACT) {  // the rest of the offsets are constants
       k_off[0] = row16 * DP * size + K::kVec * group4 * size;
@@ -440,9 +450,11 @@ struct Attend {
 #pragma unroll
         for (int i = 0; i < K::kSubs; ++i) s[i] = mfma(r.k[i][c], qh[c], s[i], T());
 #pragma unroll
-      for (int c = 0; c < K::kChunks; ++c)
+      for (int t = 0; t < (K::kTerms - 1) * K::kChunks; ++t) {
+        const u32x4 q = q_low[64 * t];
 #pragma unroll
-        for (int i = 0; i < K::kSubs; ++i) s[i] = mfma(r.k[i][c], ql[c], s[i], T());
+        for (int i = 0; i < K::kSubs; ++i) s[i] = mfma(r.k[i][t % K::kChunks], q, s[i], T());
+      }
     } else {
       f32x4 s2 = s[0];
 #pragma unroll
@@ -503,8 +515,8 @@ struct Attend {
         st.l += p[4 * i + j];
       }
     if constexpr (K::kHalf) {
-      u32x4 ph, pl;
-      split8<T>(p, ph, pl);
+      u32x4 pt[K::kTerms];
+      split8<T>(p, pt);
 #pragma unroll
       for (int c = 0; c < K::kVChunks; ++c)
 #pragma unroll
@@ -516,10 +528,11 @@ struct Attend {
             b[x] = __builtin_amdgcn_perm(r.v[2 * x + 1][c][w2], r.v[2 * x][c][w2], 0x07060302u);
           }
           f32x4 &y = st.acc[c * K::kVVec + 2 * w2], &z = st.acc[c * K::kVVec + 2 * w2 + 1];
-          y = mfma(a, ph, y, T());
-          z = mfma(b, ph, z, T());
-          y = mfma(a, pl, y, T());
-          z = mfma(b, pl, z, T());
+#pragma unroll
+          for (int t = 0; t < K::kTerms; ++t) {
+            y = mfma(a, pt[t], y, T());
+            z = mfma(b, pt[t], z, T());
+          }
         }
     } else {
 #pragma unroll
@@ -572,6 +585,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
   typedef Attend<T, DP, EXACT, ONCE> A;
   constexpr int S = DP + 4;
   __shared__ __align__(16) float s_acc[kWaves][kTile][S];  // first: the queries, in [0]
+  __shared__ __align__(16) u32x4 s_q[K::kHalf ? (K::kTerms - 1) * K::kChunks * 64 : 1];
   __shared__ float s_m[kWaves][kTile], s_l[kWaves][kTile];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -611,7 +625,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
   const int c1 = !turns || rt.interleaved ? 2 * pair + 1 : pair + rt.pairs;
   const uint64_t step = turns ? rt.steps[pair] : 0;
 
-  A w(g, lane);
+  A w(g, lane, s_q);
   int seg = -1, u0 = 0;
   const auto next = [&](const Piece &pc) {
     at += pc.u1 - u0;
@@ -694,7 +708,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
           x[i] = s_acc[0][w.row16][w.k_channel(c) + i];
           if constexpr (__is_same(T, _Float16)) x[i] = __builtin_amdgcn_ldexpf(x[i], -w.q_shift);
         }
-        split8<T>(x, w.qh[c], w.ql[c]);
+        u32x4 q[K::kTerms];
+        split8<T>(x, q);
+        w.qh[c] = q[0];
+        if (c % kWaves == wave)
+#pragma unroll
+          for (int t = 1; t < K::kTerms; ++t) s_q[((t - 1) * K::kChunks + c) * 64 + lane] = q[t];
       }
     } else {
 #pragma unroll
@@ -702,7 +721,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) w.qf[4 * c + i] = s_acc[0][w.row16][w.k_channel(c) + i];
     }
-    __syncthreads();  // before s_acc is written again
+    __syncthreads();  // s_q is whole; before s_acc is written again
 
     State<DP> st;
     st.m = -INFINITY;

@@ -449,10 +449,10 @@ int adaptq_paged_append_device(adaptq_paged_t cache, const void *d_k, const void
  * [dim]; query heads h * g to h * g + g - 1 (g = n_q_heads / n_heads) attend over key
  * head h's tokens [max(0, n - window), n), n = d_lengths[b]; window 0: all.  The query
  * is the token n - 1 (its rotation).  scale: of the scores, 0 = 1 / sqrt(dim), finite.
- * Sums and statistics in fp32, rounded once; rotated queries and weights enter the
- * products to 2^-16 of a value with bf16 pages, with fp16 pages to 2^-20 (a query's
- * smallest values: 2^-38 of its largest).  Tokens without a page are left out, as above;
- * a sequence with no tokens gets zeros.  The order of the sums depends
+ * Products, statistics and sums in fp32, rounded once; with fp16 pages, rotated queries
+ * and weights enter the products to 2^-20 of a value (a query's smallest values: 2^-38 of
+ * its largest).  Tokens without a page are left out, as above; a sequence with no tokens
+ * gets zeros.  The order of the sums depends
  * on the call's shape and the lengths alone, so equal calls give equal bits.  d_out may
  * not overlap d_q.  Returns 0/-1. */
 int adaptq_paged_attend_device(adaptq_paged_t cache, const void *d_q, void *d_out, int n_q_heads,

@@ -1,5 +1,5 @@
-"""What the paged attention holds rotated fp16 queries to, whatever their size, against the
-formula in 64 bits."""
+"""What the paged attention holds its queries and weights to: rotated fp16 queries of any size,
+and bf16 queries and weights in fp32, against the formula in 64 bits with bounds derived here."""
 import math
 
 import pytest
@@ -8,6 +8,7 @@ import torch
 import paged_ref as R
 
 pytestmark = pytest.mark.gpu
+U = R.U32
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -81,3 +82,74 @@ def test_one_large_channel():
     q[0, 3::4, 5] *= 30
     k[:, :, 5] = (k[:, :, 5].float() / 30).half()
     _check(q.half(), k, v, rot=32, amplitude=1.5, scale=0.01)
+
+
+def _cancelled(w, v):
+    """v [n, dim] with its last four rows such that sum w v is 0 but for a rounding of a rounding
+    of a rounding of bf16: what the output's own rounding hides is in plain sight."""
+    v = v.clone()
+    v[-4:] = 0
+    for t in range(-1, -5, -1):
+        v[t] = (-(w @ v.double()) / w[t]).to(v.dtype)
+    return v
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("seed", range(4))
+def test_bf16_weights(dim, seed):
+    """Weights of bf16 pages hold fp32's 24 bits.  A score here is one product, q_0 k_0 (bf16 x
+    bf16: exact) times scale (a power of two) and log2(e): with |s| <= 1 off by 2^-23 |s| for the
+    constant and its product; less the largest, 2^-24 of up to 2; all of it into the weight as
+    ln 2 at most, (2 + 2) 2^-24 and as much for the largest's own, and the exponential by 2^-23:
+    10 * 2^-24.  The sums over 20 tokens (two units' halves) and the quotient round some 20 times
+    by at most 2^-24 of sum |w v|, the weights' three parts leave 2^-24: 31 in all, so 2^-19
+    covers them; the sum of the weights, off as much, scales an output near 0.  A weight held to
+    2^-16 would be off by up to 8 times that."""
+    g = torch.Generator().manual_seed(seed)
+    n, heads = 20, 4
+    k = torch.zeros(n, heads, dim, dtype=torch.bfloat16)
+    k[:, :, 0] = (torch.rand(n, heads, generator=g) * 8 - 4).bfloat16()
+    q = torch.zeros(1, heads, dim, dtype=torch.bfloat16)
+    q[0, :, 0] = 1.0
+    w = torch.softmax(k[:, :, 0].double() / 4, 0)
+    v = torch.stack([_cancelled(w[:, h], torch.randn(n, dim, generator=g).bfloat16())
+                     for h in range(heads)], 1)
+    cache, table, lengths = _cache(k, v)
+    got = cache.attend(q.cuda(), table, lengths, scale=0.25)[0].cpu().double()
+    want = (w[:, :, None] * v.double()).sum(0)
+    size = (w[:, :, None] * v.double().abs()).sum(0)
+    assert (want.abs() < 2.0 ** -22 * size).all()
+    R.check(got, want, 2.0 ** -19 * size + R.u(torch.bfloat16) * 2.0 ** -19 * size)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_bf16_rotated_queries(dim):
+    """Rotated queries of bf16 pages hold fp32's 24 bits.  Two tokens whose keys pick one member
+    each of a pair, 2^11 of it: the scores' difference, 2^11 (y1 - y2), comes out of the weights'
+    ratio.  A member is off by the rotation's 2^-20 (|x1| + |x2|) (paged_ref.rotate), a score by
+    2^-23 of itself more in fp32 (up to 2^11.5); a member held to 2^-16 would put it off by up to
+    2^-5."""
+    g = torch.Generator().manual_seed(dim)
+    heads = 64
+    q = torch.zeros(1, heads, dim, dtype=torch.bfloat16)
+    x1 = 1 + torch.rand(heads, generator=g) / 4
+    rotary_kw = dict(base=10.0)
+    n = 2
+    # x2 such that the two members come out close: at angle 1, x1 c - x2 s = x2 c + x1 s
+    q[0, :, 0] = x1.bfloat16()
+    c, s = math.cos(1), math.sin(1)
+    q[0, :, 1] = (q[0, :, 0].float() * (c - s) / (c + s)).bfloat16()
+    k = torch.zeros(n, 1, dim, dtype=torch.bfloat16)
+    k[0, 0, 0] = k[1, 0, 1] = 2.0 ** 11
+    v = torch.zeros(n, 1, dim, dtype=torch.bfloat16)
+    v[0], v[1] = 1.0, -1.0
+    cache, table, lengths = _cache(k, v, Rotary(2, **rotary_kw))
+    got = cache.attend(q.cuda(), table, lengths, scale=0.25)[0].cpu().double()
+    y, err = R.rotate(q.float(), torch.tensor([1]), 2, **rotary_kw)
+    d = 512 * (y[0, :, 0] - y[0, :, 1])
+    off = 512 * (err[0, :, 0] + err[0, :, 1]) + 2.0 ** -21 * 512 * y[0].abs().amax(-1)
+    want = torch.tanh(d / 2)[:, None].expand(-1, dim)  # (e^a - e^b) / (e^a + e^b)
+    tol = (off / 2)[:, None] * (1 - want ** 2) * 1.01 + (R.u(torch.bfloat16) + 2.0 ** -19) * want.abs() \
+        + 2.0 ** -20
+    assert (want.abs() < 0.9).any()
+    R.check(got, want, tol)
