@@ -15,6 +15,7 @@ Calls on one cache from different streams must be ordered by the caller.
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import adaptq_py
 from .rotary import IO_TYPES, Rotary, stream_of
@@ -40,7 +41,7 @@ class PagedCache:
             raise ValueError("pages must be on one GPU")
         if rotary is not None and rotary.device != self.device:
             raise ValueError(f"the rotary is on {rotary.device}, the pages on {self.device}")
-        self.k_pages, self.v_pages = k_pages, v_pages
+        self.k_pages, self.v_pages = self._pools = k_pages, v_pages
         self.pages, self.heads, self.page_size, self.dim = k_pages.shape
         self.dtype = k_pages.dtype
         self._size = k_pages.element_size()
@@ -83,6 +84,8 @@ class PagedCache:
             return
         self._handle.append(k.data_ptr(), v.data_ptr(), k.shape[0], ks[1] * size, ks[0] * size,
                             vs[1] * size, vs[0] * size, *seqs, at, stream_of(self.device))
+        # a graph that saved the pools sees that they changed, as torch's own writes do
+        increment_version(self._pools)
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
                scale: float | None = None, window: int | None = None,
@@ -91,10 +94,12 @@ class PagedCache:
         (the last ``window`` of them); q_heads a multiple of heads.  q is the token at
         lengths - 1.  scale: 1/sqrt(dim).  Sequences without tokens give zeros."""
         seqs = self._sequences(table, lengths)
-        q, out, args = self._queries(q, lengths, scale, window, out)
+        q, y, args = self._queries(q, lengths, scale, window, out)
         if q.shape[0]:
             self._handle.attend(*args[0], *seqs, *args[1], stream_of(self.device))
-        return out
+            if out is not None:
+                increment_version(out)
+        return y
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
              lengths: torch.Tensor, *, scale: float | None = None, window: int | None = None,
@@ -104,13 +109,14 @@ class PagedCache:
         k, v = self._rows(k, "k", self.heads), self._rows(v, "v", self.heads)
         if k.shape[0] != lengths.shape[0] or v.shape[0] != k.shape[0]:
             raise ValueError("k and v hold one token a sequence")
-        q, out, args = self._queries(q, lengths, scale, window, out)
+        q, y, args = self._queries(q, lengths, scale, window, out)
         if q.shape[0]:
             size, ks, vs = self._size, k.stride(), v.stride()
             self._handle.step(k.data_ptr(), v.data_ptr(), ks[1] * size, ks[0] * size,
                               vs[1] * size, vs[0] * size, *args[0], *seqs, *args[1],
                               stream_of(self.device))
-        return out
+            increment_version(self._pools if out is None else (*self._pools, out))
+        return y
 
     def _rows(self, x, name, heads):
         if x.dim() != 3 or x.shape[2] != self.dim or heads and x.shape[1] != heads:

@@ -11,6 +11,7 @@ outside the capture holds (as torch wants it of any operator).
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import adaptq_py
 
@@ -131,6 +132,8 @@ class Rotary:
             return tuple(outs)
         self._handle.rotate(positions.data_ptr(), stride, batch, tokens, dim, io, backward,
                             stream_of(self.device), *args)
+        if inplace:  # a graph that saved them sees that they changed, as torch's own writes do
+            increment_version([x for x in (q, k) if x is not None])
         return tuple(outs)
 
 

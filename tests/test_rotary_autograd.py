@@ -1,0 +1,128 @@
+"""What torch sees of the calls that go to the library by address, on the CPU: the handles'
+calls are replaced by the same arithmetic in torch."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def _tensor(address, offset_shape_strides):
+    """A float32 tensor over memory that another tensor holds."""
+    shape, strides = offset_shape_strides
+    n = 1 + sum((s - 1) * t for s, t in zip(shape, strides))
+    flat = torch.frombuffer((C.c_float * n).from_address(address), dtype=torch.float32)
+    return flat.as_strided(shape, strides)
+
+
+class RotaryHandle:
+    """Pairs (i, i + dim/2) by position * 3^-i radians; rows of float32."""
+    calls = 0
+
+    def rotate(self, positions, pos_stride, batch, tokens, dim, io, backward, stream, *rows):
+        self.calls += 1
+        assert io == 0
+        at = torch.frombuffer((C.c_int * tokens).from_address(positions), dtype=torch.int32)
+        angle = at[:, None].double() * 3.0 ** -torch.arange(dim // 2)
+        c, s = angle.cos()[:, None], angle.sin()[:, None] * (-1 if backward else 1)
+        for x, y, heads, x1, x2, x3, y1, y2, y3 in (rows[:9], rows[9:]) if rows[9:] else (rows,):
+            shape = batch, tokens, heads, dim
+            x = _tensor(x, (shape, (x3 // 4, x2 // 4, x1 // 4, 1))).double()
+            a, b = x[..., :dim // 2], x[..., dim // 2:]
+            _tensor(y, (shape, (y3 // 4, y2 // 4, y1 // 4, 1))).copy_(
+                torch.cat((a * c - b * s, b * c + a * s), -1))
+
+
+@pytest.fixture
+def rotary(monkeypatch):
+    from adaptq_amd import rotary as module
+    monkeypatch.setattr(module, "stream_of", lambda device: 0)
+    r = module.Rotary.__new__(module.Rotary)
+    r.dim, r.device, r._handle = 8, torch.device("cpu"), RotaryHandle()
+    return r
+
+
+POS = torch.arange(5, 8, dtype=torch.int32)
+
+
+def _rows(heads=2, seed=0):
+    return torch.randn(3, heads, 8, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("which", [0, 1])
+def test_inplace_is_seen_by_graphs_that_saved_the_rows(rotary, mode, which):
+    """As torch's own in-place operators: the gradient of w would be of the rotated rows."""
+    q, k = _rows(), _rows(1, 1)
+    w = torch.randn(8, requires_grad=True)
+    z = (w * (q, k)[which]).sum()
+    other = (w * 2).sum()
+    with mode():
+        rotary(POS, q, k, inplace=True)
+    other.backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+def test_inplace_of_an_activation(rotary):
+    """A view of a projection rotated under no_grad, whose graph a product had saved."""
+    x = torch.randn(3, 24, requires_grad=True)
+    fused = (x * 1).view(3, 3, 8)
+    y = (fused * fused).sum()
+    with torch.no_grad():
+        rotary(POS, fused[:, :2], inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_rows_of_inference_mode_rotate_in_place(rotary):
+    with torch.inference_mode():
+        q = _rows()
+        want = rotary(POS, q)
+        assert torch.equal(rotary(POS, q, inplace=True), want) and torch.equal(q, want)
+
+
+def test_calls_that_write_nothing_of_the_callers_raise_no_version(rotary):
+    q, k = _rows(), _rows(1, 1)
+    rotary(POS, q, k)
+    assert q._version == 0 and k._version == 0 and POS._version == 0
+
+
+class PagedHandle:
+    def append(self, *a):
+        pass
+
+    attend = step = append
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    from adaptq_amd import paged as module
+    monkeypatch.setattr(module, "stream_of", lambda device: 0)
+
+    # the class checks that its pools are on a GPU: built around that
+    c = module.PagedCache.__new__(module.PagedCache)
+    c.k_pages, c.v_pages = c._pools = torch.zeros(4, 2, 16, 8), torch.zeros(4, 2, 16, 8)
+    c.device, c.dtype, c._size, c._io = torch.device("cpu"), torch.float32, 4, 0
+    c.pages, c.heads, c.page_size, c.dim = c.k_pages.shape
+    c._handle = PagedHandle()
+    return c
+
+
+def test_pools_and_outputs_are_seen_as_written(cache):
+    table, lengths = torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    q, k, out = _rows(4), _rows(), _rows(4)
+    versions = lambda: (cache.k_pages._version, cache.v_pages._version, out._version)  # noqa: E731
+    assert versions() == (0, 0, 0)
+    cache.append(k, k, table, lengths)
+    assert versions() == (1, 1, 0)
+    assert cache.attend(q, table, lengths) is not out and versions() == (1, 1, 0)
+    assert cache.attend(q, table, lengths, out=out) is out and versions() == (1, 1, 1)
+    cache.step(q, k, k, table, lengths)
+    assert versions() == (2, 2, 1)
+    assert cache.step(q, k, k, table, lengths, out=out) is out and versions() == (3, 3, 2)
+    assert q._version == k._version == table._version == lengths._version == 0
+    w = torch.ones(8, requires_grad=True)
+    z = (w * out).sum()
+    cache.attend(q, table, lengths, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
