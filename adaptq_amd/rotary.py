@@ -4,13 +4,15 @@
     q, k = rotary(positions, q, k)         # [tokens, heads, dim] or [batch, tokens, heads, dim]
 
 Device tensors of fp32, fp16 or bf16, rotated in one launch on torch's current
-stream, in fp32 and rounded once.  Differentiable in q and k.  Calls may be captured
+stream, in fp32 and rounded once.  Differentiable in q and k, backward and forward (dual
+tensors of torch.autograd.forward_ad; the transforms of torch.func are refused).  Calls may be captured
 into a graph, a backward pass only together with its forward, on leaves that no graph
 outside the capture holds (as torch wants it of any operator).
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import adaptq_py
@@ -71,13 +73,18 @@ class Rotary:
         """Rotated q, or (q, k).  positions: int32 [tokens] or [batch, tokens]; q, k: [tokens,
         heads, dim] or [batch, tokens, heads, dim] of one type, any strides with rows side by
         side.  inplace: writes into q and k (not where they need gradients)."""
-        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
-            if inplace:
+        if inplace:
+            if _differentiated(q) or _differentiated(k):
                 raise ValueError("inplace rotation of tensors that need gradients")
-            out = _Rotate.apply(self, positions, False, q, k)
-            return out if k is not None else out[0]
-        out = self._rotate(positions, q, k, inplace, False)
+            out = self._rotate(positions, q, k, True, False)
+        else:
+            out = self._turn(positions, q, k, False)
         return out if k is not None else out[0]
+
+    def _turn(self, positions, q, k, backward):
+        if _differentiated(q) or _differentiated(k):
+            return _Rotate.apply(self, positions, backward, q, k)
+        return self._rotate(positions, q, k, False, backward)
 
     def _rotate(self, positions, q, k, inplace, backward):
         if positions.dtype != torch.int32:
@@ -137,33 +144,51 @@ class Rotary:
         return tuple(outs)
 
 
+def _differentiated(x) -> bool:
+    """Whether a call on x is to be differentiated, backward or forward."""
+    return x is not None and (
+        x.requires_grad and torch.is_grad_enabled() or
+        forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None)
+
+
 class _Rotate(torch.autograd.Function):
-    """The rotation, whose gradient is the transposed rotation of the outputs' gradients
-    (itself differentiable)."""
+    """The rotation.  It is linear: the gradient is the transposed rotation of the outputs'
+    gradients, the tangents of the outputs are the rotated tangents (both themselves
+    differentiable)."""
 
     @staticmethod
     def forward(ctx, rotary, positions, backward, q, k):
         ctx.rotary, ctx.backward_ = rotary, backward
+        ctx.shapes = q.shape, None if k is None else k.shape
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.set_materialize_grads(False)
         out = rotary._rotate(positions, q, k, False, backward)
         needs = ctx.needs_input_grad
-        if not (needs[3] and needs[4]):
+        if not (needs[3] and needs[4]) and forward_ad._current_level < 0:
             ctx.mark_non_differentiable(*(y for y, need in zip(out, needs[3:])
                                           if y is not None and not need))
         return out
 
     @staticmethod
     def backward(ctx, dq, dk):
-        (positions,) = ctx.saved_tensors
-        rotate = ctx.rotary._rotate
-        if torch.is_grad_enabled():  # a graph of the gradient is asked for
-            def rotate(positions, a, b, inplace, backward):
-                return _Rotate.apply(ctx.rotary, positions, backward, a, b)
         _, _, _, needs_q, needs_k = ctx.needs_input_grad
-        dq, dk = dq if needs_q else None, dk if needs_k else None
-        if dq is not None:
-            dq, dk = rotate(positions, dq, dk, False, not ctx.backward_)
-        elif dk is not None:
-            dk, _ = rotate(positions, dk, None, False, not ctx.backward_)
-        return None, None, None, dq, dk
+        return None, None, None, *_Rotate._each(ctx, dq if needs_q else None,
+                                                dk if needs_k else None, not ctx.backward_)
+
+    @staticmethod
+    def jvp(ctx, _rotary, _positions, _backward, tq, tk):
+        dtype = (tk if tq is None else tq).dtype
+        zeros = (t if t is not None or shape is None else
+                 torch.zeros(shape, dtype=dtype, device=ctx.rotary.device)
+                 for t, shape in zip((tq, tk), ctx.shapes))  # an output's tangent may not be None
+        return _Rotate._each(ctx, *zeros, ctx.backward_)
+
+    @staticmethod
+    def _each(ctx, a, b, backward):
+        (positions,) = ctx.saved_tensors
+        if a is not None:
+            return ctx.rotary._turn(positions, a, b, backward)
+        if b is not None:
+            return None, ctx.rotary._turn(positions, b, None, backward)[0]
+        return None, None

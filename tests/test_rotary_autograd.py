@@ -4,6 +4,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 
 def _tensor(address, offset_shape_strides):
@@ -126,3 +127,85 @@ def test_pools_and_outputs_are_seen_as_written(cache):
     cache.attend(q, table, lengths, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         z.backward()
+
+
+def _turned(x, backward=False):
+    """The stub's rotation in 64 bits."""
+    angle = POS[:, None].double() * 3.0 ** -torch.arange(4)
+    c, s = angle.cos()[:, None], angle.sin()[:, None] * (-1 if backward else 1)
+    a, b = x.double()[..., :4], x.double()[..., 4:]
+    return torch.cat((a * c - b * s, b * c + a * s), -1)
+
+
+def _near(got, want):
+    # fp64 arithmetic on fp32 rows, rounded once
+    assert ((got.double() - want).abs() <= 2.0 ** -23 * want.abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad])
+def test_forward_mode(rotary, mode):
+    """The tangent of a rotated dual tensor is the rotated tangent, of either or both."""
+    q, k, tq, tk = _rows(), _rows(1, 1), _rows(2, 2), _rows(1, 3)
+    with forward_ad.dual_level(), mode():
+        for dq, dk in ((1, 1), (1, 0), (0, 1)):
+            x = forward_ad.make_dual(q, tq) if dq else q
+            y = forward_ad.make_dual(k, tk) if dk else k
+            for out, base, t, dual in zip(rotary(POS, x, y), (q, k), (tq, tk), (dq, dk)):
+                p, d = forward_ad.unpack_dual(out)
+                _near(p, _turned(base))
+                if dual:
+                    _near(d, _turned(t))
+                else:
+                    assert d is None or not d.any()
+        p, d = forward_ad.unpack_dual(rotary(POS, forward_ad.make_dual(k, tk)))
+        _near(p, _turned(k)), _near(d, _turned(tk))
+        assert forward_ad.unpack_dual(rotary(POS, q)).tangent is None
+        with pytest.raises(ValueError, match="inplace"):
+            rotary(POS, forward_ad.make_dual(q, tq), inplace=True)
+        with pytest.raises(ValueError, match="inplace"):
+            rotary(POS, q, forward_ad.make_dual(k, tk), inplace=True)
+
+
+def test_forward_over_backward(rotary):
+    """The tangent of a gradient: of the dual gradient of the outputs."""
+    q = _rows().requires_grad_()
+    g, tg = _rows(2, 4), _rows(2, 5)
+    with forward_ad.dual_level():
+        (dq,) = torch.autograd.grad(rotary(POS, q), (q,), forward_ad.make_dual(g, tg))
+        p, d = forward_ad.unpack_dual(dq)
+        _near(p.detach(), _turned(g, True))
+        _near(d, _turned(tg, True))
+
+
+def test_backward_over_forward(rotary):
+    """The gradient of a tangent."""
+    q, tq, g = _rows(), _rows(2, 2).requires_grad_(), _rows(2, 3)
+    with forward_ad.dual_level():
+        d = forward_ad.unpack_dual(rotary(POS, forward_ad.make_dual(q, tq))).tangent
+        _near(d.detach(), _turned(tq.detach()))
+        (dt,) = torch.autograd.grad(d, (tq,), g)
+    _near(dt, _turned(g, True))
+
+
+def test_gradients_as_before(rotary):
+    """Backward of both, of one, of a second order; outputs of inputs that need none need none."""
+    q, k = _rows().requires_grad_(), _rows(1, 1).requires_grad_()
+    gq, gk = _rows(2, 2).requires_grad_(), _rows(1, 3)
+    dq, dk = torch.autograd.grad(rotary(POS, q, k), (q, k), (gq, gk), create_graph=True)
+    _near(dq.detach(), _turned(gq.detach(), True)), _near(dk, _turned(gk, True))
+    h = _rows(2, 6)
+    (dg,) = torch.autograd.grad(dq, (gq,), h)
+    _near(dg, _turned(h))
+    yq, yk = rotary(POS, q.detach(), k)
+    assert not yq.requires_grad and yk.requires_grad
+    (dk,) = torch.autograd.grad(yk, (k,), gk)
+    _near(dk, _turned(gk, True))
+
+
+def test_function_transforms_are_refused(rotary):
+    q = _rows()
+    for call in (lambda: torch.func.jvp(lambda x: rotary(POS, x), (q,), (q,)),
+                 lambda: torch.func.grad(lambda x: rotary(POS, x).sum())(q),
+                 lambda: torch.func.vmap(lambda x: rotary(POS, x))(q[None])):
+        with pytest.raises(RuntimeError):
+            call()
