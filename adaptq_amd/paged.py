@@ -9,7 +9,8 @@
 Sequence b's token p lies in page ``table[b, p // page_size]``, slot ``p % page_size``;
 ``lengths[b]`` is what it holds before the call.  All tensors are on the GPU, the table,
 lengths and offsets int32; calls run on torch's current stream, allocate only their
-output, never wait, and may be captured into a graph.  Inference only: no gradients.
+output, never wait, and may be captured into a graph.  Inference only: no gradients, and
+tracing (torch.jit.trace, make_fx, torch.export) is refused.
 Calls on one cache from different streams must be ordered by the caller.
 """
 from __future__ import annotations
@@ -18,7 +19,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import adaptq_py
-from .rotary import IO_TYPES, Rotary, stream_of
+from .rotary import IO_TYPES, Rotary, refuse_tracing, stream_of
 
 
 class PagedCache:
@@ -129,6 +130,7 @@ class PagedCache:
         return x if x.stride(2) == 1 else x.contiguous()
 
     def _sequences(self, table, lengths):
+        refuse_tracing("PagedCache")
         if table.dtype != torch.int32 or lengths.dtype != torch.int32:
             raise TypeError("table and lengths must be int32")
         n = lengths.shape[0] if lengths.dim() == 1 else -1

@@ -7,7 +7,8 @@ Device tensors of fp32, fp16 or bf16, rotated in one launch on torch's current
 stream, in fp32 and rounded once.  Differentiable in q and k, backward and forward (dual
 tensors of torch.autograd.forward_ad; the transforms of torch.func are refused).  Calls may be captured
 into a graph, a backward pass only together with its forward, on leaves that no graph
-outside the capture holds (as torch wants it of any operator).
+outside the capture holds (as torch wants it of any operator).  Tracing (torch.jit.trace,
+make_fx, torch.export) is refused; torch.compile runs them between its graphs.
 """
 from __future__ import annotations
 
@@ -31,6 +32,22 @@ def stream_of(device: torch.device) -> int:
     if _raw_stream is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_tracing_state = torch._C._get_tracing_state
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def refuse_tracing(what: str) -> None:
+    """A call goes to the library by address, past torch's dispatcher: a program traced through
+    it would hold the output's allocation alone and return memory that nobody wrote."""
+    if _tracing_state() is None:
+        if not _dispatch_modes():
+            return
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is None:
+            return
+    raise RuntimeError(f"{what} cannot be traced; leave its calls out of the traced program")
 
 
 class Rotary:
@@ -73,20 +90,21 @@ class Rotary:
         """Rotated q, or (q, k).  positions: int32 [tokens] or [batch, tokens]; q, k: [tokens,
         heads, dim] or [batch, tokens, heads, dim] of one type, any strides with rows side by
         side.  inplace: writes into q and k (not where they need gradients)."""
-        if inplace:
-            if _differentiated(q) or _differentiated(k):
+        if _differentiated(q, k):
+            if inplace:
                 raise ValueError("inplace rotation of tensors that need gradients")
-            out = self._rotate(positions, q, k, True, False)
+            out = _Rotate.apply(self, positions, False, q, k)
         else:
-            out = self._turn(positions, q, k, False)
+            out = self._rotate(positions, q, k, inplace, False)
         return out if k is not None else out[0]
 
     def _turn(self, positions, q, k, backward):
-        if _differentiated(q) or _differentiated(k):
+        if _differentiated(q, k):
             return _Rotate.apply(self, positions, backward, q, k)
         return self._rotate(positions, q, k, False, backward)
 
     def _rotate(self, positions, q, k, inplace, backward):
+        refuse_tracing("Rotary")
         if positions.dtype != torch.int32:
             raise TypeError(f"positions must be int32, got {positions.dtype}")
         io = IO_TYPES.get(q.dtype)
@@ -144,11 +162,12 @@ class Rotary:
         return tuple(outs)
 
 
-def _differentiated(x) -> bool:
-    """Whether a call on x is to be differentiated, backward or forward."""
-    return x is not None and (
-        x.requires_grad and torch.is_grad_enabled() or
-        forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None)
+def _differentiated(q, k) -> bool:
+    """Whether a call on q and k (or None) is to be differentiated, backward or forward."""
+    if (q.requires_grad or k is not None and k.requires_grad) and torch.is_grad_enabled():
+        return True
+    return forward_ad._current_level >= 0 and any(
+        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (q, k))
 
 
 class _Rotate(torch.autograd.Function):

@@ -209,3 +209,50 @@ def test_function_transforms_are_refused(rotary):
                  lambda: torch.func.vmap(lambda x: rotary(POS, x))(q[None])):
         with pytest.raises(RuntimeError):
             call()
+
+
+def _traces():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    return [lambda f, *a: make_fx(f)(*a), lambda f, *a: make_fx(f, tracing_mode="fake")(*a),
+            lambda f, *a: torch.jit.trace(f, a, check_trace=False),
+            lambda f, *a: torch.export.export(_Module(f), a, strict=False)]
+
+
+class _Module(torch.nn.Module):
+    def __init__(self, f):
+        super().__init__()
+        self.f = f
+
+    def forward(self, *a):
+        return self.f(*a)
+
+
+@pytest.mark.parametrize("trace", range(4))
+def test_traced_calls_are_refused(rotary, cache, trace):
+    """A traced program would hold the output's allocation alone."""
+    trace = _traces()[trace]
+    table, lengths = torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    q, k = _rows(4), _rows()
+    for f in (lambda q, k: rotary(POS, q, k)[0] + 1,
+              lambda q, k: rotary(POS, q.clone(), inplace=True) + 1,
+              lambda q, k: cache.attend(q, table, lengths) + 1,
+              lambda q, k: cache.step(q, k, k, table, lengths) + 1,
+              lambda q, k: (cache.append(k, k, table, lengths), q + 1)[1]):
+        with pytest.raises(RuntimeError, match="cannot be traced|data pointer"):
+            trace(f, q, k)
+    assert rotary._handle.calls == 0
+
+
+def test_compiled_calls_run(rotary):
+    """torch.compile leaves the call between its graphs."""
+    q = _rows()
+    f = torch.compile(lambda q: rotary(POS, q * 2) + 1, backend="eager")
+    _near(f(q) - 1, _turned(q * 2))
+    _near(f(q + 1) - 1, _turned((q + 1) * 2))
+
+
+def test_other_modes_run(rotary):
+    """A dispatch mode that records nothing is no trace."""
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False):
+        _near(rotary(POS, _rows()), _turned(_rows()))
