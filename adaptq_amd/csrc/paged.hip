@@ -39,7 +39,7 @@ struct Shape {
   PagedShape p;
   PagedSeqs q;
   PagedAppend a;
-  int tokens_per_block;
+  int first_token, tokens_per_block;
   int chunks, pass, items;  // items of a row: pairs, the rest of the key; with the value
   uint64_t head_mul;        // row / n_heads = row * head_mul >> 32, for row * n_heads < 2^32
 };
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Shape s) {
   const PagedSeqs &q = s.q;
   const PagedAppend &a = s.a;
   const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * s.tokens_per_block;
+  const int t0 = s.first_token + blockIdx.x * s.tokens_per_block;
   const int nt = min(s.tokens_per_block, a.n_tokens - t0), n_rows = nt * p.n_heads;
   const int pairs = p.rotary.pairs;
   const int wide = min(s.items, kThreads), rows_per = kThreads / wide;  // threads of a row
@@ -153,9 +153,10 @@ hipError_t append_n(const PagedShape &p, const PagedSeqs &q, const PagedAppend &
   int tb = kRows * kThreads / (g.items * p.n_heads);
   tb = std::min({tb, kCosSin / std::max(pairs, 1), kMaxTokens, a.n_tokens / 1024});
   g.tokens_per_block = std::max(tb, 1);
-  const int blocks = (a.n_tokens + g.tokens_per_block - 1) / g.tokens_per_block;
-  append_kernel<T, N><<<blocks, kThreads, 0, s>>>(g);
-  return hipGetLastError();
+  return launch_over_tokens(a.n_tokens, g.tokens_per_block, [&](int first, int blocks) {
+    g.first_token = first;
+    append_kernel<T, N><<<blocks, kThreads, 0, s>>>(g);
+  });
 }
 
 template <typename T>

@@ -3,9 +3,26 @@
 // the HIP launch status.
 #pragma once
 
+#include <algorithm>
+
 #include "launch.hpp"
 
 namespace aq {
+
+// A kernel over `tokens` tokens, tokens_per_block of them a block of 256 threads:
+// launch(first token, blocks), in one launch but for the most tokens, as a launch has at most
+// 2^32 - 1 threads.
+template <typename Launch>
+hipError_t launch_over_tokens(int tokens, int tokens_per_block, Launch launch) {
+  constexpr int64_t kMost = (((int64_t)1 << 32) - 1) / 256;
+  const int64_t blocks = ((int64_t)tokens + tokens_per_block - 1) / tokens_per_block;
+  for (int64_t b = 0; b < blocks; b += kMost) {
+    launch((int)(b * tokens_per_block), (int)std::min(kMost, blocks - b));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
 
 // A rotation, its per-pair steps (see rotary.hpp) in device memory.
 struct RotaryTable {

@@ -37,7 +37,7 @@ struct Shape {
   RowsArg a, b;
   const int *positions;
   int64_t pos_stride;
-  int n_batch, n_tokens, total, tokens_per_block;
+  int n_batch, n_tokens, total, first_token, tokens_per_block;
   int items, pass_vecs;  // items of a row; vectors of it that pass through
   uint64_t head_mul;     // row / heads = row * head_mul >> 32, for row * heads < 2^32
   bool backward;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Shape s) {
   typedef RowVec<T, N> Vec;
   __shared__ __align__(16) float2 s_cs[kCosSin];
   const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * s.tokens_per_block;
+  const int t0 = s.first_token + blockIdx.x * s.tokens_per_block;
   const int nt = min(s.tokens_per_block, s.total - t0);
   const int chunks = s.r.pairs / N, heads = s.a.heads + s.b.heads, n_rows = nt * heads;
   const int wide = min(s.items, kThreads), rows_per = kThreads / wide;  // threads of a row
@@ -164,9 +164,10 @@ hipError_t launch(Shape g, int dim, bool in_place, hipStream_t s) {
   int tb = kRows * kThreads / (g.items * heads);
   tb = std::min({tb, kCosSin / std::max(g.r.pairs, 1), g.total / 1024});
   g.tokens_per_block = std::max(tb, 1);
-  const int blocks = (g.total + g.tokens_per_block - 1) / g.tokens_per_block;
-  rotary_kernel<T, N><<<blocks, kThreads, 0, s>>>(g);
-  return hipGetLastError();
+  return launch_over_tokens(g.total, g.tokens_per_block, [&](int first, int blocks) {
+    g.first_token = first;
+    rotary_kernel<T, N><<<blocks, kThreads, 0, s>>>(g);
+  });
 }
 
 template <typename T>
