@@ -11,7 +11,10 @@ Sequence b's token p lies in page ``table[b, p // page_size]``, slot ``p % page_
 lengths and offsets int32; calls run on torch's current stream, allocate only their
 output, never wait, and may be captured into a graph.  Inference only: no gradients, and
 tracing (torch.jit.trace, make_fx, torch.export) is refused.
-Calls on one cache from different streams must be ordered by the caller.
+Calls on one cache from different streams wait for each other (they share its workspace as
+well as its pages; a stream that torch does not own has to outlive the cache's next call).
+Replays of a graph are ordered by the caller, among each other and with calls: those that run
+over each other give wrong outputs, and may leave the workspace such that later ones do.
 """
 from __future__ import annotations
 
@@ -46,6 +49,8 @@ class PagedCache:
         self.pages, self.heads, self.page_size, self.dim = k_pages.shape
         self.dtype = k_pages.dtype
         self._size = k_pages.element_size()
+        self._last = None  # the stream of the last call, and its address
+        self._last_address = None
         with torch.cuda.device(self.device):
             self._handle = adaptq_py.PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), self.pages,
                                                 self.page_size, self.heads, self.dim, self._io,
@@ -84,7 +89,7 @@ class PagedCache:
         if not k.shape[0]:
             return
         self._handle.append(k.data_ptr(), v.data_ptr(), k.shape[0], ks[1] * size, ks[0] * size,
-                            vs[1] * size, vs[0] * size, *seqs, at, stream_of(self.device))
+                            vs[1] * size, vs[0] * size, *seqs, at, self._stream())
         # a graph that saved the pools sees that they changed, as torch's own writes do
         increment_version(self._pools)
 
@@ -97,7 +102,7 @@ class PagedCache:
         seqs = self._sequences(table, lengths)
         q, y, args = self._queries(q, lengths, scale, window, out)
         if q.shape[0]:
-            self._handle.attend(*args[0], *seqs, *args[1], stream_of(self.device))
+            self._handle.attend(*args[0], *seqs, *args[1], self._stream())
             if out is not None:
                 increment_version(out)
         return y
@@ -115,9 +120,25 @@ class PagedCache:
             size, ks, vs = self._size, k.stride(), v.stride()
             self._handle.step(k.data_ptr(), v.data_ptr(), ks[1] * size, ks[0] * size,
                               vs[1] * size, vs[0] * size, *args[0], *seqs, *args[1],
-                              stream_of(self.device))
+                              self._stream())
             increment_version(self._pools if out is None else (*self._pools, out))
         return y
+
+    def _stream(self):
+        address = stream_of(self.device)
+        if address != self._last_address:
+            self._follow(address)
+        return address
+
+    def _follow(self, address):
+        """The current stream, which is not the last call's, waits for that one's work."""
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                return  # a capture waits for nothing outside it
+            stream = torch.cuda.current_stream()
+            if self._last is not None:
+                stream.wait_stream(self._last)
+            self._last, self._last_address = stream, address
 
     def _rows(self, x, name, heads):
         if x.dim() != 3 or x.shape[2] != self.dim or heads and x.shape[1] != heads:

@@ -418,7 +418,10 @@ int adaptq_rotary_device(adaptq_rotary_t rotary, const adaptq_rows_t *rows, int 
  * the workspace that its attention needs (8.5 MB at dim 128); it copies `rotary`
  * (NULL: rows are taken as they are), by which appended keys and the queries of
  * attention are rotated.  Several handles may share pools.  Calls on one handle from different
- * streams (graph replays too) must be ordered by the caller.  n_heads up to 32768. */
+ * streams, graph replays too, must be ordered by the caller, attentions as well: they
+ * share the workspace, and calls that run over each other, or whose lengths change while
+ * they run, give wrong outputs and may leave it such that later calls do (a new handle over
+ * the same pools does not).  n_heads up to 32768. */
 typedef void *adaptq_paged_t;
 adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
                                    int n_heads, int dim, int io_type, adaptq_rotary_t rotary);

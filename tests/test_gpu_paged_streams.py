@@ -1,0 +1,96 @@
+"""One PagedCache used on several streams that the caller has not ordered."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def api(torch_dev):
+    from adaptq_amd.paged import PagedCache
+    globals().update(PagedCache=PagedCache)
+
+
+def _cache(n, tokens, heads, dim, page=64):
+    g = torch.Generator().manual_seed(n)
+    width = -(-(tokens + 40) // page)
+    k, v = (torch.randn(n * width, heads, page, dim, generator=g).bfloat16().cuda()
+            for _ in range(2))
+    table = torch.arange(n * width, dtype=torch.int32).view(n, width).cuda()
+    return (PagedCache(k, v), table, torch.full((n,), tokens, dtype=torch.int32).cuda(),
+            lambda *s: torch.randn(*s, generator=g).bfloat16().cuda())
+
+
+def test_attends_on_two_streams():
+    """Calls that would run over each other's workspace: each gives its own result, and so does
+    every call after them."""
+    cache, table, lengths, normal = _cache(2, 20000, 2, 64)
+    qs = [normal(2, h, 64) for h in (2, 32, 6)]
+    want = [cache.attend(q, table, lengths, window=w) for q, w in zip(qs, (None, 9000, 15000))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(cache.attend(qs[i % 3], table, lengths, window=(None, 9000, 15000)[i % 3]))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 3]), i
+    for q, w, y in zip(qs, (None, 9000, 15000), want):
+        assert torch.equal(cache.attend(q, table, lengths, window=w), y)
+    # and the results are right
+    k, v = (p.view(2, -1, 2, 64, 64).transpose(1, 2).reshape(2, 2, -1, 64)[:, :, :20000].cpu()
+            for p in (cache.k_pages, cache.v_pages))
+    for i in range(2):
+        o, t = R.attend(qs[0][i].cpu().double().view(2, 1, 64), k[i], v[i], 1 / math.sqrt(64),
+                        torch.bfloat16)
+        R.check(want[0][i], o.view(2, 64), t.view(2, 64))
+
+
+def test_steps_alternate_between_streams():
+    """Rows that one stream appends are there for the next one's attention."""
+    a, table, lengths, normal = _cache(3, 5000, 2, 64)
+    b = PagedCache(a.k_pages.clone(), a.v_pages.clone())
+    streams = [torch.cuda.Stream() for _ in range(3)] + [torch.cuda.default_stream()]
+    calls = [(normal(3, 8, 64), normal(3, 2, 64), normal(3, 2, 64), lengths + i) for i in range(24)]
+    torch.cuda.synchronize()
+    got = []
+    for i, (q, k, v, n) in enumerate(calls):
+        with torch.cuda.stream(streams[i % 4]):
+            if i % 3 == 2:
+                a.append(k, v, table, n)
+            else:
+                got.append(a.step(q, k, v, table, n))
+    torch.cuda.synchronize()
+    want = []
+    for i, (q, k, v, n) in enumerate(calls):
+        if i % 3 == 2:
+            b.append(k, v, table, n)
+        else:
+            want.append(b.step(q, k, v, table, n))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert torch.equal(a.k_pages, b.k_pages) and torch.equal(a.v_pages, b.v_pages)
+
+
+def test_captured_calls_do_not_wait_for_streams_outside():
+    """A capture takes nothing from another stream; its replays are ordered by the caller."""
+    cache, table, lengths, normal = _cache(1, 3000, 2, 64)
+    q = normal(1, 4, 64)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        want = cache.attend(q, table, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, table, lengths)
+        again = cache.attend(q, table, lengths, window=100)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(cache.attend(q, table, lengths, window=100), again)
+        torch.cuda.synchronize()

@@ -105,7 +105,7 @@ def cache(monkeypatch):
     c.k_pages, c.v_pages = c._pools = torch.zeros(4, 2, 16, 8), torch.zeros(4, 2, 16, 8)
     c.device, c.dtype, c._size, c._io = torch.device("cpu"), torch.float32, 4, 0
     c.pages, c.heads, c.page_size, c.dim = c.k_pages.shape
-    c._handle = PagedHandle()
+    c._handle, c._last_address = PagedHandle(), 0
     return c
 
 
