@@ -176,6 +176,8 @@ class PagedCache:
             raise ValueError(f"scale must not be 0 in fp32, got {scale}")
         if out is None:
             out = torch.empty_like(q)  # its rows' values side by side, as q's are
+            if out.stride(2) != 1:  # (not where q's rows overlap)
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         elif self._rows(out, "out", 0) is not out or out.shape != q.shape:
             raise ValueError("out must have q's shape, its rows' values side by side")
         size, qs, os = self._size, q.stride(), out.stride()

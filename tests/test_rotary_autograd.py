@@ -256,3 +256,15 @@ def test_other_modes_run(rotary):
     from torch.utils.flop_counter import FlopCounterMode
     with FlopCounterMode(display=False):
         _near(rotary(POS, _rows()), _turned(_rows()))
+
+
+def test_queries_that_overlap_get_an_output_of_rows(cache):
+    """Windows over one row of values: like them, an output would hold its rows' values apart."""
+    table, lengths = torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    q = torch.arange(64.0).as_strided((4, 2, 8), (1, 8, 1))
+    assert torch.empty_like(q).stride(2) != 1
+    seen = []
+    cache._handle.attend = lambda *a: seen.append(a)
+    out = cache.attend(q, table, lengths)
+    assert out.shape == q.shape and out.is_contiguous()
+    assert seen[0][3:7] == (8 * 4, 1 * 4, 8 * 4, 16 * 4)  # bytes between heads and sequences
