@@ -1,10 +1,9 @@
 // paged.hip -- rows written into the pages of their sequences, keys rotated on the
 // way.
-#include <limits.h>
-
 #include <algorithm>
 
 #include "paged.hpp"
+#include "paged_split.hpp"
 #include "rotary.hpp"
 
 namespace aq {
@@ -32,7 +31,7 @@ __device__ __forceinline__ int page_of(const PagedSeqs &q, const PagedShape &p, 
 // Half or twice the tokens a block, or blocks of 512 threads, were slower.
 
 constexpr int kCosSin = 1024;   // pairs x tokens of a block
-constexpr int kMaxTokens = 16;  // of a block
+constexpr int kBlockTokens = 16;
 constexpr int kRows = 4;
 
 struct Shape {
@@ -48,8 +47,8 @@ template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void append_kernel(const Shape s) {
   typedef RowVec<T, N> Vec;
   __shared__ __align__(16) float2 s_cs[kCosSin];
-  __shared__ int64_t s_row[kMaxTokens];  // row of head 0 in the pages, or -1
-  __shared__ int s_pos[kMaxTokens];
+  __shared__ int64_t s_row[kBlockTokens];  // row of head 0 in the pages, or -1
+  __shared__ int s_pos[kBlockTokens];
   const PagedShape &p = s.p;
   const PagedSeqs &q = s.q;
   const PagedAppend &a = s.a;
@@ -103,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Shape s) {
     }
     int64_t pos = -1;
     if (j >= 0 && q.lengths[seq] >= 0) pos = (int64_t)q.lengths[seq] + j;
-    const int page = pos >= 0 && pos < INT_MAX ? page_of(q, p, seq, (int)pos) : -1;
+    const int page = pos >= 0 && pos < kMaxTokens ? page_of(q, p, seq, (int)pos) : -1;
     s_pos[tid] = (int)pos;
     s_row[tid] = page < 0 ? -1 : (int64_t)page * p.n_heads * p.page_size + pos % p.page_size;
   }
@@ -151,7 +150,7 @@ hipError_t append_n(const PagedShape &p, const PagedSeqs &q, const PagedAppend &
   // tokens of a block: enough rows to fill its threads, LDS for their cosines, and
   // no fewer than 1,024 blocks for it
   int tb = kRows * kThreads / (g.items * p.n_heads);
-  tb = std::min({tb, kCosSin / std::max(pairs, 1), kMaxTokens, a.n_tokens / 1024});
+  tb = std::min({tb, kCosSin / std::max(pairs, 1), kBlockTokens, a.n_tokens / 1024});
   g.tokens_per_block = std::max(tb, 1);
   return launch_over_tokens(a.n_tokens, g.tokens_per_block, [&](int first, int blocks) {
     g.first_token = first;

@@ -438,8 +438,8 @@ void adaptq_paged_destroy(adaptq_paged_t cache);
  * [n_seqs + 1], ascending: tokens d_offsets[b] to d_offsets[b + 1] - 1 go to sequence
  * b at positions d_lengths[b], d_lengths[b] + 1, ...; tokens outside all of them are
  * left out.  d_offsets NULL: token b goes to sequence b (n_tokens = n_seqs).  A token
- * whose position has no page (beyond table_width, a page number outside the pool, a
- * negative length) is left out; all else in the pools stays as it was.  Two tokens
+ * whose position has no page (beyond table_width or 2^31 - 33, a page number outside the
+ * pool, a negative length) is left out; all else in the pools stays as it was.  Two tokens
  * of one call must not share a slot (a page that two sequences write, a sequence
  * twice): either's values may end up there.  Returns 0/-1. */
 int adaptq_paged_append_device(adaptq_paged_t cache, const void *d_k, const void *d_v,

@@ -83,3 +83,24 @@ def test_append_at_the_end_of_an_int():
                  lengths, offsets)
     assert torch.equal(cache.k_pages[0, :, 15], row[0, 0]) and (cache.k_pages[0, :, :15] == 5).all()
     assert torch.equal(cache.v_pages[0, :, 15], row[1, 0]) and (cache.v_pages[0, :, :15] == 5).all()
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 34, 2 ** 31 - 33, 2 ** 31 - 32, 2 ** 31 - 5, 2 ** 31 - 1])
+def test_step_is_append_then_attend_at_the_last_positions(n):
+    """A token at 2^31 - 33 is a sequence's last, for an append as for a step."""
+    a, b = (PagedCache.allocate(2, 1, 65536, 8, dtype=torch.float32, rotary=Rotary(8))
+            for _ in range(2))
+    g = torch.Generator().manual_seed(0)
+    for p, r in ((a.k_pages, b.k_pages), (a.v_pages, b.v_pages)):
+        p.copy_(torch.randn(p.shape, generator=g))
+        r.copy_(p)
+    before = a.v_pages.clone()
+    table = torch.tensor([[0] * 32768, [1] * 32768], dtype=torch.int32).cuda()
+    lengths = torch.tensor([n, 70000], dtype=torch.int32).cuda()
+    q, k, v = (torch.randn(2, h, 8, generator=g).cuda() for h in (2, 1, 1))
+    got = a.step(q, k, v, table, lengths, window=100)
+    b.append(k, v, table, lengths)
+    assert torch.equal(a.k_pages, b.k_pages) and torch.equal(a.v_pages, b.v_pages)
+    assert torch.equal(a.v_pages[0], before[0]) == (n > 2 ** 31 - 33)
+    if n < 2 ** 31 - 1:
+        assert torch.equal(got, b.attend(q, table, lengths + 1, window=100))
