@@ -74,8 +74,6 @@ class AdaptQAttention(nn.Module):
                 # the position is the host's: a replay would rotate by the captured one
                 raise RuntimeError("AdaptQAttention with rotary cannot be captured; capture "
                                    "Rotary with positions that the graph advances.")
-            with torch.no_grad():
-                q, k = self.rotary(self._position(), q, k)
 
         if q.is_cuda:
             # a token's call is bound by the host: nothing here makes a tensor
@@ -85,6 +83,9 @@ class AdaptQAttention(nn.Module):
             if io is None or k.dtype != dtype or v.dtype != dtype:
                 q, k, v = (x.detach().to(torch.float32) for x in (q, k, v))
                 io = 0
+            if self.rotary is not None:
+                with torch.no_grad():
+                    q, k = self.rotary(self._position(), q, k)
             q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
             out = torch.empty_like(q)
             engine = self.engine
