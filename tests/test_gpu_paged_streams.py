@@ -94,3 +94,29 @@ def test_captured_calls_do_not_wait_for_streams_outside():
         assert torch.equal(out, want)
         assert torch.equal(cache.attend(q, table, lengths, window=100), again)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+def test_replays_and_calls_share_the_workspace(heads):
+    """A captured step replayed, its lengths advancing, with eager attention over other lengths
+    between the replays: both sides' values are those of a cache of their own."""
+    a, table, lengths, normal = _cache(3, 6000, 2, 64)
+    b = PagedCache(a.k_pages.clone(), a.v_pages.clone())
+    own, other = lengths.clone(), torch.tensor([6000, 17, 3100], dtype=torch.int32).cuda()
+    q, k, v = normal(3, heads, 64), normal(3, 2, 64), normal(3, 2, 64)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = a.step(q, k, v, table, own)
+        own.add_(1)
+    for i in range(5):
+        for x in (q, k, v):
+            x.copy_(normal(*x.shape))
+        graph.replay()
+        eager = a.attend(q, table, other)
+        want = b.step(q, k, v, table, lengths)
+        lengths += 1
+        assert torch.equal(out, want) and torch.equal(own, lengths), i
+        assert torch.equal(eager, b.attend(q, table, other)), i
+        assert torch.equal(a.k_pages, b.k_pages) and torch.equal(a.v_pages, b.v_pages)
+        torch.cuda.synchronize()
