@@ -644,7 +644,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
       u0 = __builtin_amdgcn_readfirstlane(s.u0);
     }
     const Piece pc =
-        piece_at(blockIdx.x, start, end, at, u0, w.span.units, w.span.short_, share);
+        piece_at(blockIdx.x, start, end, at, u0, w.span.units, w.span.short_, share, gridDim.x);
     if (pc.empty) {
       next(pc);
       continue;

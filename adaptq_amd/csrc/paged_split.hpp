@@ -90,8 +90,10 @@ struct Piece {
   int first, pieces;  // the first block with a piece of the segment, and how many have one
 };
 
+// blocks: of the launch; pieces are counted up to there, should the lengths have changed since
+// the total was added up.
 AQ_SPLIT_HD Piece piece_at(int block, int64_t start, int64_t end, int64_t at, int u0, int units,
-                           bool short_, int64_t share) {
+                           bool short_, int64_t share, int blocks = 1 << 30) {
   Piece p;
   if (short_) {
     p.u1 = units;
@@ -111,7 +113,8 @@ AQ_SPLIT_HD Piece piece_at(int block, int64_t start, int64_t end, int64_t at, in
   const uint32_t s = share < 0x80000000 ? (uint32_t)share : 0x80000000u;
   const int64_t before = start - (at - u0);
   p.first = before > 0 ? block - (int)(((uint32_t)before + s - 1) / s) : block;
-  p.pieces = block + (int)((uint32_t)(units - 1 - before) / s) - p.first + 1;
+  const int last = block + (int)((uint32_t)(units - 1 - before) / s);
+  p.pieces = (last < blocks ? last : blocks - 1) - p.first + 1;
   return p;
 }
 
