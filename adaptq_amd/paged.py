@@ -19,10 +19,10 @@ over each other give wrong outputs, and may leave the workspace such that later 
 from __future__ import annotations
 
 import torch
-from torch.autograd.graph import increment_version
 
 from . import adaptq_py
-from .rotary import IO_TYPES, Rotary, refuse_tracing, stream_of
+from .rotary import (IO_TYPES, Rotary, dispatch_modes, increment_version, refuse_tracing,
+                     stream_of, tracing_state)
 
 
 class PagedCache:
@@ -104,7 +104,7 @@ class PagedCache:
         if q.shape[0]:
             self._handle.attend(*args[0], *seqs, *args[1], self._stream())
             if out is not None:
-                increment_version(out)
+                increment_version((out,))
         return y
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
@@ -151,7 +151,8 @@ class PagedCache:
         return x if x.stride(2) == 1 else x.contiguous()
 
     def _sequences(self, table, lengths):
-        refuse_tracing("PagedCache")
+        if tracing_state() is not None or dispatch_modes():
+            refuse_tracing("PagedCache")
         if table.dtype != torch.int32 or lengths.dtype != torch.int32:
             raise TypeError("table and lengths must be int32")
         n = lengths.shape[0] if lengths.dim() == 1 else -1

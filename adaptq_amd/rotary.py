@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.graph import increment_version
 
 from . import adaptq_py
 
@@ -34,16 +33,17 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_tracing_state = torch._C._get_tracing_state
-_dispatch_modes = torch._C._len_torch_dispatch_stack
+# Bound here, as _raw_stream is, for a small call's host time: a check of both costs 0.1 us.
+tracing_state = torch._C._get_tracing_state
+dispatch_modes = torch._C._len_torch_dispatch_stack
+increment_version = torch._C._increment_version  # of a sequence of tensors
 
 
 def refuse_tracing(what: str) -> None:
-    """A call goes to the library by address, past torch's dispatcher: a program traced through
-    it would hold the output's allocation alone and return memory that nobody wrote."""
-    if _tracing_state() is None:
-        if not _dispatch_modes():
-            return
+    """Called where tracing_state() or dispatch_modes() is set.  A call goes to the library by
+    address, past torch's dispatcher: a program traced through it would hold the output's
+    allocation alone and return memory that nobody wrote."""
+    if tracing_state() is None:
         from torch.fx.experimental.proxy_tensor import get_proxy_mode
         if get_proxy_mode() is None:
             return
@@ -104,7 +104,8 @@ class Rotary:
         return self._rotate(positions, q, k, False, backward)
 
     def _rotate(self, positions, q, k, inplace, backward):
-        refuse_tracing("Rotary")
+        if tracing_state() is not None or dispatch_modes():
+            refuse_tracing("Rotary")
         if positions.dtype != torch.int32:
             raise TypeError(f"positions must be int32, got {positions.dtype}")
         io = IO_TYPES.get(q.dtype)
