@@ -25,7 +25,7 @@ __device__ __forceinline__ int page_of(const PagedSeqs &q, const PagedShape &p, 
 // the value, kRows of them in flight.  The rows' loads go out first; while they are
 // under way the tokens' sequences, positions and pages are looked up, and the cosines
 // and sines of their pairs computed, into LDS once for every head.  Bound: the rows'
-// bytes, read and written once; 40,000 tokens of 8 heads of 128 in bf16 72 us, 4.5 TB/s
+// bytes, read and written once; 40,000 tokens of 8 heads of 128 in bf16 71 us, 4.6 TB/s
 // (a copy of 2 GiB moves 5.0); 16 ragged prompts of fp32 rows of 80 25 us, 4.6 TB/s, 29
 // without the mark on the loads that they are not used again, 44 with it on the stores.
 // Half or twice the tokens a block, or blocks of 512 threads, were slower.

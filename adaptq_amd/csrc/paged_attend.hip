@@ -810,7 +810,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(
       // Joined by the block that finishes last: all pieces at once, or, where they are more
       // than 64 KB, by groups whose last blocks leave the group's part each, and those then
       // (a CU reads some 20 GB/s past the caches.  65,536 tokens, one key head of 128, 16
-      // query heads: 256 pieces at once 93 us, in groups 27; 84 pieces of one row 20 and 22).
+      // query heads: 256 pieces at once 83 us, in groups 28; 84 pieces of one row 20 and 22).
       const int k = blockIdx.x - pc.first;
       const bool grouped = pc.pieces > kGroup && pc.pieces * rows * DP > kJoinAtOnce;
       int piece0 = grouped ? k / kGroup * kGroup : 0, step = 1;
@@ -876,20 +876,23 @@ hipError_t launch(const Args &g, hipStream_t s) {
   const int64_t segments = g.q.n_seqs * (int64_t)g.segs;
   const int64_t most = segments * std::max(longest, (int64_t)kMinUnits);
   // Two blocks a CU overlap one's ends of segments with the other's rows (64 sequences x 8
-  // heads of 8,192 tokens 315 us, with one 320; 88 segments of up to 20 units 17.6 and 18.9;
-  // 1,666 of a few tokens 40 and 53), and with little work a wave of theirs has one unit
-  // where it would have two (28 segments of 63 units 16.0 and 17.5).  Few long segments are
+  // heads of 8,192 tokens 315 us, with one 320; 88 segments of up to 20 units 18.6 and 18.9;
+  // 1,666 of a few tokens 40 and 51), and with little work a wave of theirs has one unit
+  // where it would have two (28 segments of 63 units 15.8 and 17.1).  Few long segments are
   // cut into twice as many pieces by them, and joining those costs more (one sequence of
-  // 32,768 tokens, 8 heads: 35 us, with one block a CU 30; 36 segments of 128 units 25 and
-  // 23.3; one segment of 2,048 units, 8 query heads 24.5 and 19.8).
+  // 32,768 tokens, 8 heads: 32.6 us, with one block a CU 29.7; 36 segments of 128 units 27.9
+  // and 25.8; one segment of 2,048 units, 8 query heads 23.4 and 19.7).  How long they may be is
+  // the table's width, for the lengths are on the device: 32, 48 and 56 segments of up to
+  // 1,280, 640 and 4,000 tokens take as long with a table of 8,192 or 131,072 tokens as with
+  // one of their own (13.3, 13.2 and 23.9 us, within 0.1).
   const bool few_long = segments < g.cus / 16 ||
                         (segments < g.cus / 4 && most > 2 * kWaves * (int64_t)g.cus);
   const int resident = std::min(most_blocks(g.cus, DP), few_long ? g.cus : 2 * g.cus);
   const int blocks = (int)std::min((most + kWaves - 1) / kWaves, (int64_t)resident);
   // Rows that one tile of query heads reads are marked to leave the caches first (64
   // sequences x 8 heads of 8,192 tokens: 315 us, unmarked 358).  Rows that further tiles
-  // read stay (one sequence of 131,072 tokens, 32 query heads on one: 30.2 us, marked 35.2;
-  // 32 sequences of 8,192, 256 on 8: 300 and 324).
+  // read stay (one sequence of 131,072 tokens, 32 query heads on one: 32.0 us, marked 34.7;
+  // 32 sequences of 8,192, 256 on 8: 311 and 308).
   if (g.q_tiles == 1)
     kernel_of<T, DP, true>(g)<<<blocks, kThreads, 0, s>>>(g);
   else

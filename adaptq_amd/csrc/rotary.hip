@@ -9,9 +9,10 @@
 // bytes (the two members of N pairs, or 2 N channels that pass through), and has
 // kRows of them in flight.  The loads go out first; while they are under way the
 // tokens' cosines and sines are computed into LDS, once for every head.  8,192 tokens
-// of 32 + 8 heads of 128 in bf16: 29.6 us, 5.7 TB/s read and written (a copy of 2 GiB
-// moves 5.0); 33 with two rows in flight, 31 to 33 with streaming loads or stores, 41
-// with the loads behind the cosines.
+// of 32 + 8 heads of 128 in bf16: 35.2 us, 4.8 TB/s read and written (a copy of 2 GiB
+// moves 5.0), 29.6 where the last cache still holds some of the 168 MB; compared there: 33
+// with two rows in flight, 31 to 33 with streaming loads or stores, 41 with the loads
+// behind the cosines.
 #include <algorithm>
 
 #include "paged.hpp"
@@ -45,8 +46,9 @@ struct Shape {
 
 // Cosines and sines of a token's pairs in LDS: two pairs (16 bytes) of each chunk of N side
 // by side for all its chunks, then the next two, so that threads of neighbouring chunks read
-// neighbouring words: 29.6 us instead of 30.5 with a chunk's pairs in a row.  (The append
-// keeps them in a row: it gains nothing, and prompts over 4 heads lose 5 %.)
+// neighbouring words: 29.6 us instead of 30.5 with a chunk's pairs in a row (rows in the last
+// cache).  (The append keeps them in a row: it gains nothing, and prompts over 4 heads lose
+// 5 %.)
 template <int N>
 __device__ __forceinline__ int cos_sin_at(int pair, int chunks) {
   if (N == 1) return pair;

@@ -9,8 +9,9 @@
 Sequence b's token p lies in page ``table[b, p // page_size]``, slot ``p % page_size``;
 ``lengths[b]`` is what it holds before the call.  All tensors are on the GPU, the table,
 lengths and offsets int32; calls run on torch's current stream, allocate only their
-output, never wait, and may be captured into a graph.  Inference only: no gradients, and
-tracing (torch.jit.trace, make_fx, torch.export) is refused.
+output, never wait, and may be captured into a graph, which the cache has to outlive.
+Inference only: no gradients, and tracing (torch.jit.trace, make_fx, torch.export) is
+refused.
 Calls on one cache from different streams wait for each other (they share its workspace as
 well as its pages; a stream that torch does not own has to outlive the cache's next call).
 Replays of a graph are ordered by the caller, among each other and with calls: those that run

@@ -5,10 +5,11 @@
 
 Device tensors of fp32, fp16 or bf16, rotated in one launch on torch's current
 stream, in fp32 and rounded once.  Differentiable in q and k, backward and forward (dual
-tensors of torch.autograd.forward_ad; the transforms of torch.func are refused).  Calls may be captured
-into a graph, a backward pass only together with its forward, on leaves that no graph
-outside the capture holds (as torch wants it of any operator).  Tracing (torch.jit.trace,
-make_fx, torch.export) is refused; torch.compile runs them between its graphs.
+tensors of torch.autograd.forward_ad; the transforms of torch.func are refused).  Calls
+may be captured into a graph, which the Rotary has to outlive, a backward pass only
+together with its forward, on leaves that no graph outside the capture holds (as torch
+wants it of any operator).  Tracing (torch.jit.trace, make_fx, torch.export) is refused;
+torch.compile runs the calls between its graphs.
 """
 from __future__ import annotations
 

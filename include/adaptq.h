@@ -357,7 +357,8 @@ long long adaptq_plan_workspace_bytes(adaptq_plan_t plan);
  * nothing and waits for nothing; all may be captured into a HIP graph (creations
  * and destructions may not).  What a call reads on the device (positions, tables,
  * lengths, offsets) is read when it runs, so a captured call follows what these
- * hold at each replay.  Handles live on the HIP device current at their creation.
+ * hold at each replay; its handles have to outlive the graph.  Handles live on the HIP
+ * device current at their creation.
  * Byte strides: nb1 between heads, nb2 between tokens (or sequences), nb3 between
  * batches, multiples of the element size; a row's `dim` values lie side by side.
  * Rows aligned to 16 bytes are read fastest. */
@@ -376,8 +377,10 @@ long long adaptq_plan_workspace_bytes(adaptq_plan_t plan);
  *           (kept within 0 and rotary_dim - 1)
  * slow, fast: 0 = 1 and 4 (YARN: 1 and 32).  factor at least 1, base above 1,
  * rotary_dim even, from 2 to 1024.  amplitude a: 0 = 1 (YARN: 0.1 ln(factor) + 1).
- * Angles are exact to 2^-33 of a turn at every position.  Returns NULL and sets the last
- * error on invalid arguments. */
+ * The phase, position * f_i with its whole turns dropped, is exact to 2^-33 of a turn at
+ * every position; what it is off the next quarter turn is rounded to fp32 (by up to 2^-28
+ * of a turn) before its sine and cosine.  Returns NULL and sets the last error on invalid
+ * arguments. */
 typedef void *adaptq_rotary_t;
 enum {
   ADAPTQ_ROTARY_PLAIN = 0,
@@ -465,8 +468,9 @@ int adaptq_paged_attend_device(adaptq_paged_t cache, const void *d_q, void *d_ou
                                void *stream);
 
 /* step: append with one token a sequence, then attend over d_lengths[b] + 1 tokens;
- * same pages and outputs as those two calls.  A sequence of negative length is empty
- * and stays so. */
+ * same pages and outputs as those two calls, where no sequence attends to the slot that
+ * another's new token goes to (it may read that slot before or after).  A sequence of
+ * negative length is empty and stays so. */
 int adaptq_paged_step_device(adaptq_paged_t cache, const void *d_k, const void *d_v, size_t k_nb1,
                              size_t k_nb2, size_t v_nb1, size_t v_nb2, const void *d_q,
                              void *d_out, int n_q_heads, size_t q_nb1, size_t q_nb2,
