@@ -13,6 +13,8 @@ def api(torch_dev):
     from adaptq_amd.paged import PagedCache
     from adaptq_amd.rotary import Rotary
     globals().update(PagedCache=PagedCache, Rotary=Rotary)
+    yield
+    torch.cuda.empty_cache()  # the large tensors go back to the device
 
 
 def test_rotary_of_more_blocks_than_a_launch():
