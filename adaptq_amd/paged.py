@@ -138,7 +138,10 @@ class PagedCache:
                 return  # a capture waits for nothing outside it
             stream = torch.cuda.current_stream()
             if self._last is not None:
-                stream.wait_stream(self._last)
+                with torch.cuda.stream(self._last):
+                    captured = torch.cuda.is_current_stream_capturing()
+                if not captured:  # (what waits for a captured stream is captured with it)
+                    stream.wait_stream(self._last)
             self._last, self._last_address = stream, address
 
     def _rows(self, x, name, heads):

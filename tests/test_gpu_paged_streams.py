@@ -120,3 +120,30 @@ def test_replays_and_calls_share_the_workspace(heads):
         assert torch.equal(eager, b.attend(q, table, other)), i
         assert torch.equal(a.k_pages, b.k_pages) and torch.equal(a.v_pages, b.v_pages)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("captured_last", [True, False])
+def test_calls_beside_a_capture_stay_outside_it(captured_last):
+    """An eager call while the stream of the last call (or another) is being captured runs at
+    once: waiting for a captured stream would make the call a part of the graph."""
+    cache, table, lengths, normal = _cache(1, 3000, 2, 64)
+    q, out = normal(1, 4, 64), torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda")
+    want = cache.attend(q, table, lengths)
+    x = torch.zeros(1, device="cuda")
+    stream, other, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    if captured_last:
+        with torch.cuda.stream(stream):
+            cache.attend(q, table, lengths)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        x.add_(1)
+        with torch.cuda.stream(other):
+            cache.attend(q, table, lengths, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    out.zero_()
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert x.item() == i + 1 and not out.any()
