@@ -314,14 +314,14 @@ def prepare(case, seed):
     s["case"] = c
     four = c["kind"] in ("append4", "attend4", "step4")
     if own:
-        from adaptq_amd.paged import PagedCache, PagedCache4
+        from adaptq_amd import paged
         from adaptq_amd.rotary import Rotary
         rotary = Rotary(c["dim"], base=c["base"]) if c["rotary"] else None
         if four:
-            s["cache"] = PagedCache4.allocate(s["pages"], c["heads"], c["page_size"], c["dim"],
-                                              dtype=DTYPES[c["dtype"]], rotary=rotary)
+            s["cache"] = paged.PagedCache4.allocate(s["pages"], c["heads"], c["page_size"], c["dim"],
+                                                    dtype=DTYPES[c["dtype"]], rotary=rotary)
         else:
-            s["cache"] = PagedCache(s["k_pages"], s["v_pages"], rotary=rotary)
+            s["cache"] = paged.PagedCache(s["k_pages"], s["v_pages"], rotary=rotary)
     else:
         if c["rotary"]:
             i = torch.arange(c["dim"] // 2, dtype=torch.float64, device="cuda")
@@ -338,8 +338,8 @@ def prepare(case, seed):
         if own:
             zero = torch.zeros_like(s["lengths"])
             if c["rotary"]:  # the rows come as they are to lie in the pages
-                plain = PagedCache4(s["cache"].k_pages, s["cache"].v_pages,
-                                    dtype=DTYPES[c["dtype"]])
+                plain = paged.PagedCache4(s["cache"].k_pages, s["cache"].v_pages,
+                                          dtype=DTYPES[c["dtype"]])
                 plain.append(k, v, s["table"], zero, offsets=at)
             else:
                 s["cache"].append(k, v, s["table"], zero, offsets=at)
