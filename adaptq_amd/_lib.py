@@ -19,6 +19,12 @@ _u8 = C.POINTER(C.c_uint8)
 _ip = C.POINTER(C.c_int)
 
 
+class Scores(C.Structure):
+    """adaptq_scores_t"""
+    _fields_ = [("softcap", C.c_float), ("window", C.c_int), ("d_slopes", C.c_void_p),
+                ("d_prefix", C.c_void_p), ("d_first", C.c_void_p)]
+
+
 class Rows(C.Structure):
     """adaptq_rows_t"""
     _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("n_heads", C.c_int),
@@ -100,6 +106,9 @@ SIGNATURES = {
                                         C.c_float, _i, _v]),
     "adaptq_paged_step_device": (_i, [_v, _v, _v, _z, _z, _z, _z, _v, _v, _i, _z, _z, _z, _z, _v,
                                       _i, _i, _v, _i, C.c_float, _i, _v]),
+    "adaptq_paged_prompt_workspace": (_z, [_v, _i, _i, _i, _i]),
+    "adaptq_paged_prompt_device": (_i, [_v, _v, _v, _i, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i, _v,
+                                        C.c_float, C.POINTER(Scores), _v, _z, _v]),
 }
 
 FEAT_AVX2, FEAT_HYBRID, FEAT_SPARSE_V, FEAT_HIP = 1, 2, 4, 8

@@ -117,6 +117,7 @@ class PyMHAContext {
 using addr = uintptr_t;
 
 void *ptr(addr a) { return reinterpret_cast<void *>(a); }
+const float *floats(addr a) { return reinterpret_cast<const float *>(a); }
 const int *ints(addr a) { return reinterpret_cast<const int *>(a); }
 void check(int rc) {
   if (rc != 0) throw std::runtime_error(adaptq_last_error());
@@ -174,6 +175,18 @@ class PyPagedCache {
                                      width, stride, ints(lengths), n_seqs, scale, window,
                                      ptr(stream)));
   }
+  size_t prompt_workspace(int q_heads, int n_tokens, int n_seqs, int width) {
+    return adaptq_paged_prompt_workspace(h_, q_heads, n_tokens, n_seqs, width);
+  }
+  void prompt(addr q, addr out, int q_heads, size_t q1, size_t q2, size_t o1, size_t o2,
+              int n_tokens, addr table, int width, int stride, addr lengths, int n_seqs,
+              addr offsets, float scale, int window, float softcap, addr slopes, addr prefix,
+              addr first, addr workspace, size_t bytes, addr stream) {
+    const adaptq_scores_t s = {softcap, window, floats(slopes), ints(prefix), ints(first)};
+    check(adaptq_paged_prompt_device(h_, ptr(q), ptr(out), q_heads, n_tokens, q1, q2, o1, o2,
+                                     ints(table), width, stride, ints(lengths), n_seqs,
+                                     ints(offsets), scale, &s, ptr(workspace), bytes, ptr(stream)));
+  }
   void step(addr k, addr v, size_t k1, size_t k2, size_t v1, size_t v2, addr q, addr out,
             int q_heads, size_t q1, size_t q2, size_t o1, size_t o2, addr table, int width,
             int stride, addr lengths, int n_seqs, float scale, int window, addr stream) {
@@ -228,5 +241,7 @@ PYBIND11_MODULE(adaptq_py, m) {
       .def(py::init<addr, addr, int, int, int, int, int, const PyRotary *>())
       .def("append", &PyPagedCache::append)
       .def("attend", &PyPagedCache::attend)
+      .def("prompt_workspace", &PyPagedCache::prompt_workspace)
+      .def("prompt", &PyPagedCache::prompt)
       .def("step", &PyPagedCache::step);
 }

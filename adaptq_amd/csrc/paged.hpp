@@ -88,6 +88,33 @@ struct PagedAttend {
   int extra;   // tokens beyond `lengths` that a sequence holds by now
 };
 
+// What happens to scores on their way into the softmax, and which tokens a query at position p
+// of n tokens sees: first <= t < n and (t < prefix or p - window < t <= p).
+struct PagedScores {
+  float softcap;        // 0: none
+  int window;           // 0: all tokens
+  const float *slopes;  // [q_heads], of the distance; null: none
+  const int *prefix;    // of each query; null: 0
+  const int *first;     // of each query; null: 0
+};
+
+// Several queries a sequence: its last offsets[b + 1] - offsets[b] tokens.
+struct PagedPrompt {
+  const void *q;
+  void *out;
+  size_t q_nb[2], out_nb[2];
+  int q_heads, n_tokens;
+  const int *offsets;
+  float scale;
+  PagedScores scores;
+};
+
+// Bytes of workspace that a prompt's attention of this shape takes, from its caller.
+size_t paged_prompt_workspace(const PagedShape &p, int q_heads, int n_tokens, int n_seqs,
+                              int table_width);
+hipError_t launch_paged_prompt(const PagedShape &p, const PagedSeqs &q, const PagedPrompt &a,
+                               void *workspace, hipStream_t s);
+
 // Bytes of workspace an attention of this shape may need, zeroed once when it is made.
 size_t paged_workspace_bytes(const PagedShape &p);
 // step: one token a sequence, written into its page by the same launch (a.extra 1), or null.

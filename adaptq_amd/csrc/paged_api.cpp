@@ -199,6 +199,41 @@ bool attend_ok(const Paged *p, const void *q, const void *out, int q_heads, int 
          rows_ok(p, out, "d_out", q_heads, n_seqs, nb[2], nb[3], true, fn);
 }
 
+bool scores_ok(const adaptq_scores_t *s, aq::PagedScores *to, const char *fn) {
+  *to = aq::PagedScores{};
+  if (!s) return true;
+  if (!(s->softcap >= 0.0f && std::isfinite(s->softcap * 1.5f))) {  // (times log2(e) in the kernel)
+    set_errorf(fn, "softcap must not be negative, up to 2.2e38");
+    return false;
+  }
+  if (s->softcap > 0.0f && s->softcap < 0x1p-100f) {
+    set_errorf(fn, "softcap must be 0 or at least 2^-100");
+    return false;
+  }
+  if (s->window < 0) {
+    set_errorf(fn, "negative window");
+    return false;
+  }
+  if (!aligned_to(s->d_slopes, 4, fn) || !aligned_to(s->d_prefix, 4, fn) ||
+      !aligned_to(s->d_first, 4, fn))
+    return false;
+  *to = {s->softcap, s->window, s->d_slopes, s->d_prefix, s->d_first};
+  return true;
+}
+
+bool workspace_ok(const void *ws, size_t bytes, size_t needed, const char *fn) {
+  if (needed == 0) return true;
+  if (bytes < needed) {
+    set_errorf(fn, "the workspace is too small");
+    return false;
+  }
+  return require_pointer(ws, fn, "d_workspace") && aligned_to(ws, 16, fn);
+}
+
+float scale_of(const Paged *p, float scale) {
+  return scale != 0.0f ? scale : (float)(1.0 / std::sqrt((double)p->shape.dim));
+}
+
 bool out_apart(const Paged *p, const void *out, int out_heads, size_t o1, size_t o2,
                const void *in, int in_heads, size_t i1, size_t i2, int n, const char *fn) {
   const size_t row = size_of((int)p->shape.io) * p->shape.dim;
@@ -219,7 +254,7 @@ aq::PagedAttend attend_args(const Paged *p, const void *q, void *out, int q_head
   a.out_nb[0] = o1;
   a.out_nb[1] = o2;
   a.q_heads = q_heads;
-  a.scale = scale != 0.0f ? scale : (float)(1.0 / std::sqrt((double)p->shape.dim));
+  a.scale = scale_of(p, scale);
   a.window = window;
   a.extra = extra;
   return a;
@@ -550,6 +585,64 @@ int adaptq_paged_step_device(adaptq_paged_t h, const void *d_k, const void *d_v,
   DeviceGuard g(p->device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (hip_fail(aq::launch_paged_attend(p->shape, q, a, &ap, p->ws, s), fn)) return -1;
+  aq::clear_error();
+  return 0;
+}
+
+size_t adaptq_paged_prompt_workspace(adaptq_paged_t h, int n_q_heads, int n_tokens, int n_seqs,
+                                     int table_width) {
+  if (!h || n_q_heads <= 0 || n_tokens <= 0 || n_seqs <= 0 || table_width < 0) return 0;
+  const Paged *p = static_cast<Paged *>(h);
+  if (n_q_heads % p->shape.n_heads) return 0;
+  return aq::paged_prompt_workspace(p->shape, n_q_heads, n_tokens, n_seqs, table_width);
+}
+
+int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, int n_q_heads,
+                               int n_tokens, size_t q_nb1, size_t q_nb2, size_t out_nb1,
+                               size_t out_nb2, const int *d_table, int table_width,
+                               int table_stride, const int *d_lengths, int n_seqs,
+                               const int *d_offsets, float scale, const adaptq_scores_t *scores,
+                               void *d_workspace, size_t workspace_bytes, void *stream) {
+  const char *fn = "adaptq_paged_prompt_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (n_tokens < 0) {
+    set_errorf(fn, "negative n_tokens");
+    return -1;
+  }
+  const size_t nb[4] = {q_nb1, q_nb2, out_nb1, out_nb2};
+  aq::PagedPrompt a{};
+  if (!seqs_ok(d_table, table_width, table_stride, d_lengths, n_seqs, fn) ||
+      !attend_ok(p, d_q, d_out, n_q_heads, n_tokens, nb, scale, 0, fn) ||
+      !scores_ok(scores, &a.scores, fn))
+    return -1;
+  if (n_tokens == 0 || n_seqs == 0) {
+    aq::clear_error();
+    return 0;
+  }
+  if (!require_pointer(d_offsets, fn, "d_offsets") || !aligned_to(d_offsets, 4, fn) ||
+      !out_apart(p, d_out, n_q_heads, out_nb1, out_nb2, d_q, n_q_heads, q_nb1, q_nb2, n_tokens,
+                 fn) ||
+      !workspace_ok(d_workspace, workspace_bytes,
+                    aq::paged_prompt_workspace(p->shape, n_q_heads, n_tokens, n_seqs, table_width),
+                    fn))
+    return -1;
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  a.q = d_q;
+  a.out = d_out;
+  a.q_nb[0] = q_nb1;
+  a.q_nb[1] = q_nb2;
+  a.out_nb[0] = out_nb1;
+  a.out_nb[1] = out_nb2;
+  a.q_heads = n_q_heads;
+  a.n_tokens = n_tokens;
+  a.offsets = d_offsets;
+  a.scale = scale_of(p, scale);
+  DeviceGuard g(p->device);
+  if (hip_fail(aq::launch_paged_prompt(p->shape, q, a, d_workspace,
+                                       static_cast<hipStream_t>(stream)),
+               fn))
+    return -1;
   aq::clear_error();
   return 0;
 }

@@ -78,11 +78,7 @@ class PagedCache:
             raise ValueError("k and v differ in tokens")
         at = 0
         if offsets is not None:
-            if offsets.dtype != torch.int32 or offsets.shape != (lengths.shape[0] + 1,):
-                raise ValueError("offsets must be int32 [sequences + 1]")
-            if offsets.device != self.device:
-                raise ValueError(f"offsets must be on {self.device}")
-            offsets = offsets.contiguous()
+            offsets = self._offsets(offsets, lengths)
             at = offsets.data_ptr()
         elif k.shape[0] != lengths.shape[0]:
             raise ValueError("without offsets, k and v hold one token a sequence")
@@ -94,13 +90,38 @@ class PagedCache:
         # a graph that saved the pools sees that they changed, as torch's own writes do
         increment_version(self._pools)
 
-    def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
-               scale: float | None = None, window: int | None = None,
+    def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+               offsets: torch.Tensor | None = None, *, scale: float | None = None,
+               window: int | None = None, softcap: float | None = None,
+               slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
+               first: torch.Tensor | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one query a sequence, q [sequences, q_heads, dim], over its tokens
         (the last ``window`` of them); q_heads a multiple of heads.  q is the token at
-        lengths - 1.  scale: 1/sqrt(dim).  Sequences without tokens give zeros."""
+        lengths - 1.  scale: 1/sqrt(dim).  Sequences without tokens give zeros.
+
+        With offsets, of several: q [tokens, q_heads, dim], tokens offsets[b] to
+        offsets[b + 1] - 1 the last ones of sequence b, whose lengths[b] counts them (a prompt
+        after its append); rows outside the offsets are left as ``out`` has them.
+
+        For the query at position p and token t: scores become softcap * tanh(score / softcap),
+        then lose slopes[q_head] * |p - t| (float32); t is seen where first <= t and
+        (t < prefix or p - window < t <= p).  prefix and first are int32, one a query."""
         seqs = self._sequences(table, lengths)
+        if offsets is not None:
+            offsets = self._offsets(offsets, lengths)
+            q, y, args = self._queries(q, None, scale, window, out)
+            n = q.shape[0]
+            if n and seqs[4]:
+                shape = self._scores(n, q.shape[1], softcap, slopes, prefix, first)
+                need = self._handle.prompt_workspace(q.shape[1], n, seqs[4], seqs[1])
+                space = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+                self._handle.prompt(*args[0], n, *seqs, offsets.data_ptr(), *args[1], *shape,
+                                    0 if space is None else space.data_ptr(), need,
+                                    self._stream())
+                if out is not None:
+                    increment_version((out,))
+            return y
         q, y, args = self._queries(q, lengths, scale, window, out)
         if q.shape[0]:
             self._handle.attend(*args[0], *seqs, *args[1], self._stream())
@@ -171,9 +192,37 @@ class PagedCache:
             raise ValueError("table rows and lengths must lie side by side")
         return table.data_ptr(), width, max(stride, width), lengths.data_ptr(), n
 
+    def _offsets(self, offsets, lengths):
+        if offsets.dtype != torch.int32 or offsets.shape != (lengths.shape[0] + 1,):
+            raise ValueError("offsets must be int32 [sequences + 1]")
+        if offsets.device != self.device:
+            raise ValueError(f"offsets must be on {self.device}")
+        return offsets.contiguous()
+
+    def _scores(self, n, q_heads, softcap, slopes, prefix, first):
+        """What attention with scores of its own takes: (softcap, slopes, prefix, first)."""
+        if softcap is not None and not softcap > 0:
+            raise ValueError(f"softcap must be positive, got {softcap}")
+        at = []
+        for name, x, dtype, size in (("slopes", slopes, torch.float32, q_heads),
+                                     ("prefix", prefix, torch.int32, n),
+                                     ("first", first, torch.int32, n)):
+            if x is None:
+                at.append(0)
+                continue
+            if x.dtype != dtype or x.shape != (size,):
+                raise ValueError(f"{name} must be {dtype} [{size}], got {x.dtype} "
+                                 f"{tuple(x.shape)}")
+            if x.device != self.device:
+                raise ValueError(f"{name} must be on {self.device}")
+            if size > 1 and x.stride(0) != 1:
+                raise ValueError(f"{name} must lie side by side")
+            at.append(x.data_ptr())
+        return (softcap or 0.0, *at)
+
     def _queries(self, q, lengths, scale, window, out):
         q = self._rows(q, "q", 0)
-        if q.shape[0] != lengths.shape[0]:
+        if lengths is not None and q.shape[0] != lengths.shape[0]:
             raise ValueError("q holds one query a sequence")
         if window is not None and window <= 0:
             raise ValueError(f"window must be positive, got {window}")

@@ -478,6 +478,39 @@ int adaptq_paged_step_device(adaptq_paged_t cache, const void *d_k, const void *
                              int table_stride, const int *d_lengths, int n_seqs, float scale,
                              int window, void *stream);
 
+/* What happens to scores between the products and the softmax, and which tokens a query
+ * sees.  For the query at position p of a sequence of n tokens, and token t:
+ *   x = scale <q, k_t>;  x = softcap * tanh(x / softcap), softcap 0: as it is;
+ *   x = x - d_slopes[query head] * |p - t|, d_slopes NULL: as it is;
+ *   t is seen if first <= t < n and (t < prefix or p - window < t <= p),
+ * window 0: all tokens up to p.  first and prefix are of the query's own, d_first and
+ * d_prefix one int a query (a token of the call), NULL: 0.  So a document of a packed row
+ * is seen from its first token on, a prefix is seen from both sides, and a window keeps its
+ * first tokens.  A query that sees nothing gets zeros.  softcap not negative. */
+typedef struct {
+  float softcap;
+  int window;
+  const float *d_slopes;
+  const int *d_prefix, *d_first;
+} adaptq_scores_t;
+
+/* prompt: the queries of several tokens a sequence, d_q and d_out [n_tokens][n_q_heads][dim];
+ * tokens d_offsets[b] to d_offsets[b + 1] - 1 are the last ones of sequence b, whose
+ * d_lengths[b] counts them (append them first).  Tokens outside the offsets are left as they
+ * were.  Query heads, pages and d_out as in attend; scores NULL: every token up to its own.
+ * Half types: rotated queries and the softmax's weights are rounded to the type before
+ * the products, the rest is fp32.  n_tokens * n_q_heads up to 2^31 - 1.  d_workspace:
+ * device memory of adaptq_paged_prompt_workspace bytes (0 for many tokens), 16-byte
+ * aligned, this call's alone until it is done.  Returns 0/-1. */
+size_t adaptq_paged_prompt_workspace(adaptq_paged_t cache, int n_q_heads, int n_tokens,
+                                     int n_seqs, int table_width);
+int adaptq_paged_prompt_device(adaptq_paged_t cache, const void *d_q, void *d_out, int n_q_heads,
+                               int n_tokens, size_t q_nb1, size_t q_nb2, size_t out_nb1,
+                               size_t out_nb2, const int *d_table, int table_width,
+                               int table_stride, const int *d_lengths, int n_seqs,
+                               const int *d_offsets, float scale, const adaptq_scores_t *scores,
+                               void *d_workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
