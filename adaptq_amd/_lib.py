@@ -109,6 +109,24 @@ SIGNATURES = {
     "adaptq_paged_prompt_workspace": (_z, [_v, _i, _i, _i, _i]),
     "adaptq_paged_prompt_device": (_i, [_v, _v, _v, _i, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i, _v,
                                         C.c_float, C.POINTER(Scores), _v, _z, _v]),
+    "adaptq_paged_weights_workspace": (_z, [_v, _i, _i, _i]),
+    "adaptq_paged_attend_scores_device": (_i, [_v, _v, _v, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i,
+                                               C.c_float, C.POINTER(Scores), _v, _z, _z, _v, _z,
+                                               _v]),
+    "adaptq_paged_step_scores_device": (_i, [_v, _v, _v, _z, _z, _z, _z, _v, _v, _i, _z, _z, _z,
+                                             _z, _v, _i, _i, _v, _i, C.c_float, C.POINTER(Scores),
+                                             _v, _z, _z, _v, _z, _v]),
+    "adaptq_paged_evict_device": (_i, [_v, _v, _z, _z, _v, _i, _i, _v, _i, _i, _i, _v, _i, _i, _v,
+                                       _v]),
+    "adaptq_paged4_create": (_v, [_v, _v, _i, _i, _i, _i, _i, _v]),
+    "adaptq_paged4_destroy": (None, [_v]),
+    "adaptq_paged4_append_device": (_i, [_v, _v, _v, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i, _v,
+                                         _v]),
+    "adaptq_paged4_read_device": (_i, [_v, _v, _v, _i, _v, _i, _i, _v, _i, _v, _v]),
+    "adaptq_paged4_attend_device": (_i, [_v, _v, _v, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i,
+                                         C.c_float, C.POINTER(Scores), _v]),
+    "adaptq_paged4_step_device": (_i, [_v, _v, _v, _z, _z, _z, _z, _v, _v, _i, _z, _z, _z, _z, _v,
+                                       _i, _i, _v, _i, C.c_float, C.POINTER(Scores), _v]),
 }
 
 FEAT_AVX2, FEAT_HYBRID, FEAT_SPARSE_V, FEAT_HIP = 1, 2, 4, 8

@@ -195,8 +195,83 @@ class PyPagedCache {
                                    n_seqs, scale, window, ptr(stream)));
   }
 
+  size_t weights_workspace(int q_heads, int n_seqs, int width) {
+    return adaptq_paged_weights_workspace(h_, q_heads, n_seqs, width);
+  }
+  // attend and step (k not 0) with scores of their own
+  void scored(addr k, addr v, size_t k1, size_t k2, size_t v1, size_t v2, addr q, addr out,
+              int q_heads, size_t q1, size_t q2, size_t o1, size_t o2, addr table, int width,
+              int stride, addr lengths, int n_seqs, float scale, int window, float softcap,
+              addr slopes, addr prefix, addr first, addr weights, size_t w1, size_t w2,
+              addr workspace, size_t bytes, addr stream) {
+    const adaptq_scores_t s = {softcap, window, floats(slopes), ints(prefix), ints(first)};
+    float *w = reinterpret_cast<float *>(weights);
+    if (k)
+      check(adaptq_paged_step_scores_device(h_, ptr(k), ptr(v), k1, k2, v1, v2, ptr(q), ptr(out),
+                                            q_heads, q1, q2, o1, o2, ints(table), width, stride,
+                                            ints(lengths), n_seqs, scale, &s, w, w1, w2,
+                                            ptr(workspace), bytes, ptr(stream)));
+    else
+      check(adaptq_paged_attend_scores_device(h_, ptr(q), ptr(out), q_heads, q1, q2, o1, o2,
+                                              ints(table), width, stride, ints(lengths), n_seqs,
+                                              scale, &s, w, w1, w2, ptr(workspace), bytes,
+                                              ptr(stream)));
+  }
+  void evict(addr weights, size_t w1, size_t w2, addr table, int width, int stride, addr lengths,
+             int n_seqs, int keep, int recent, addr into, int into_width, int into_stride,
+             addr kept, addr stream) {
+    check(adaptq_paged_evict_device(h_, reinterpret_cast<float *>(weights), w1, w2, ints(table),
+                                    width, stride, ints(lengths), n_seqs, keep, recent, ints(into),
+                                    into_width, into_stride, reinterpret_cast<int *>(kept),
+                                    ptr(stream)));
+  }
+
  private:
   adaptq_paged_t h_;
+};
+
+class PyPagedCache4 {
+ public:
+  PyPagedCache4(addr k_pages, addr v_pages, int n_pages, int page_size, int n_heads, int dim,
+                int io, const PyRotary *rotary)
+      : h_(adaptq_paged4_create(ptr(k_pages), ptr(v_pages), n_pages, page_size, n_heads, dim, io,
+                                rotary ? rotary->handle() : nullptr)) {
+    if (!h_) throw std::runtime_error(adaptq_last_error());
+  }
+  ~PyPagedCache4() { adaptq_paged4_destroy(h_); }
+  PyPagedCache4(const PyPagedCache4 &) = delete;
+  PyPagedCache4 &operator=(const PyPagedCache4 &) = delete;
+
+  void append(addr k, addr v, int n_tokens, size_t k1, size_t k2, size_t v1, size_t v2, addr table,
+              int width, int stride, addr lengths, int n_seqs, addr offsets, addr stream) {
+    check(adaptq_paged4_append_device(h_, ptr(k), ptr(v), n_tokens, k1, k2, v1, v2, ints(table),
+                                      width, stride, ints(lengths), n_seqs, ints(offsets),
+                                      ptr(stream)));
+  }
+  void read(addr k, addr v, int n_tokens, addr table, int width, int stride, addr lengths,
+            int n_seqs, addr offsets, addr stream) {
+    check(adaptq_paged4_read_device(h_, reinterpret_cast<float *>(k), reinterpret_cast<float *>(v),
+                                    n_tokens, ints(table), width, stride, ints(lengths), n_seqs,
+                                    ints(offsets), ptr(stream)));
+  }
+  // attend and step (k not 0)
+  void scored(addr k, addr v, size_t k1, size_t k2, size_t v1, size_t v2, addr q, addr out,
+              int q_heads, size_t q1, size_t q2, size_t o1, size_t o2, addr table, int width,
+              int stride, addr lengths, int n_seqs, float scale, int window, float softcap,
+              addr slopes, addr prefix, addr first, addr stream) {
+    const adaptq_scores_t s = {softcap, window, floats(slopes), ints(prefix), ints(first)};
+    if (k)
+      check(adaptq_paged4_step_device(h_, ptr(k), ptr(v), k1, k2, v1, v2, ptr(q), ptr(out),
+                                      q_heads, q1, q2, o1, o2, ints(table), width, stride,
+                                      ints(lengths), n_seqs, scale, &s, ptr(stream)));
+    else
+      check(adaptq_paged4_attend_device(h_, ptr(q), ptr(out), q_heads, q1, q2, o1, o2, ints(table),
+                                        width, stride, ints(lengths), n_seqs, scale, &s,
+                                        ptr(stream)));
+  }
+
+ private:
+  adaptq_paged4_t h_;
 };
 
 }  // namespace
@@ -243,5 +318,13 @@ PYBIND11_MODULE(adaptq_py, m) {
       .def("attend", &PyPagedCache::attend)
       .def("prompt_workspace", &PyPagedCache::prompt_workspace)
       .def("prompt", &PyPagedCache::prompt)
-      .def("step", &PyPagedCache::step);
+      .def("step", &PyPagedCache::step)
+      .def("weights_workspace", &PyPagedCache::weights_workspace)
+      .def("scored", &PyPagedCache::scored)
+      .def("evict", &PyPagedCache::evict);
+  py::class_<PyPagedCache4>(m, "PagedCache4")
+      .def(py::init<addr, addr, int, int, int, int, int, const PyRotary *>())
+      .def("append", &PyPagedCache4::append)
+      .def("read", &PyPagedCache4::read)
+      .def("scored", &PyPagedCache4::scored);
 }

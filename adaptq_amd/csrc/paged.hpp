@@ -121,4 +121,43 @@ size_t paged_workspace_bytes(const PagedShape &p);
 hipError_t launch_paged_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
                                const PagedAppend *step, void *workspace, hipStream_t s);
 
+
+// Where the weights of tokens are added up, fp32 [n_seqs][n_heads][tokens], strides in values;
+// null: not asked for.  workspace: paged_weights_workspace bytes.
+struct PagedWeights {
+  float *weights;
+  int64_t nb[2];  // between heads, sequences
+  void *workspace;
+};
+
+size_t paged_weights_workspace(const PagedShape &p, int q_heads, int n_seqs, int width);
+// As launch_paged_attend, with scores of its own; workspace is the handle's.
+hipError_t launch_paged_shaped(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
+                               const PagedAppend *step, const PagedScores &sc,
+                               const PagedWeights &w, void *workspace, hipStream_t s);
+
+// Eviction: per sequence and key head the `keep` tokens that stay, of those the `recent` last
+// ones, to the front of its pages or into others.
+struct PagedEvict {
+  float *weights;  // [n_seqs][n_heads][tokens], strides in values
+  int64_t nb[2];
+  int keep, recent;
+  const int *into;  // [n_seqs] rows of into_width pages, into_stride apart; null: in place
+  int into_width, into_stride;
+  int *kept;  // [n_seqs][n_heads][keep]
+};
+
+hipError_t launch_paged_evict(const PagedShape &p, const PagedSeqs &q, const PagedEvict &e,
+                              hipStream_t s);
+
+// Pages of 4-bit values (paged4.hpp): PagedShape's pools hold them, its io is the rows' type.
+hipError_t launch_paged4_append(const PagedShape &p, const PagedSeqs &q, const PagedAppend &a,
+                                hipStream_t s);
+// k, v: [n_tokens][n_heads][dim] fp32, of the tokens that an append of these arguments writes.
+hipError_t launch_paged4_read(const PagedShape &p, const PagedSeqs &q, int n_tokens,
+                              const int *offsets, float *k, float *v, hipStream_t s);
+hipError_t launch_paged4_attend(const PagedShape &p, const PagedSeqs &q, const PagedAttend &a,
+                                const PagedAppend *step, const PagedScores &sc, void *workspace,
+                                hipStream_t s);
+
 }  // namespace aq

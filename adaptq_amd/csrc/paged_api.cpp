@@ -48,7 +48,20 @@ struct Paged {
   aq::PagedShape shape{};
   uint64_t *d_steps = nullptr;
   void *ws = nullptr;
+  bool four = false;  // pages of 4-bit values
+  size_t pool = 0;    // bytes of each
 };
+
+bool exact_pages(const Paged *p, const char *fn) {
+  if (!p->four) return true;
+  set_errorf(fn, "the cache holds 4-bit values");
+  return false;
+}
+bool four_bits(const Paged *p, const char *fn) {
+  if (p->four) return true;
+  set_errorf(fn, "the cache holds exact rows");
+  return false;
+}
 
 size_t size_of(int io_type) { return io_type == ADAPTQ_IO_F32 ? 4 : 2; }
 
@@ -159,7 +172,7 @@ bool rows_ok(const Paged *p, const void *rows, const char *name, int heads, int 
     return false;
   }
   const Span x = span_of(rows, row, counts, nb, 2);
-  const size_t pool = row * s.page_size * s.n_heads * (size_t)s.n_pages;
+  const size_t pool = p->pool;
   for (const void *q : {s.k_pages, s.v_pages}) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
     if (x.lo < lo + pool && lo < x.hi) {
@@ -258,6 +271,201 @@ aq::PagedAttend attend_args(const Paged *p, const void *q, void *out, int q_head
   a.window = window;
   a.extra = extra;
   return a;
+}
+
+void destroy_paged(Paged *p) {
+  DeviceGuard g(p->device);
+  if (p->d_steps) (void)hipFree(p->d_steps);  // waits for the device
+  if (p->ws) (void)hipFree(p->ws);
+  delete p;
+}
+
+Paged *create_paged(void *d_k_pages, void *d_v_pages, int n_pages, int page_size, int n_heads,
+                    int dim, int io_type, adaptq_rotary_t rotary, bool four, const char *fn) {
+  if (!require_pointer(d_k_pages, fn, "d_k_pages") || !require_pointer(d_v_pages, fn, "d_v_pages") ||
+      !io_ok(io_type, fn))
+    return nullptr;
+  if (n_pages <= 0 || n_heads <= 0 || n_heads > kMaxHeads) {
+    set_errorf(fn, "n_pages must be positive, n_heads from 1 to 32768");
+    return nullptr;
+  }
+  if (page_size <= 0 || page_size % kPageUnit || page_size > kMaxPageSize) {
+    set_errorf(fn, "page_size must be a multiple of 16 up to 65536");
+    return nullptr;
+  }
+  if (dim <= 0 || dim % (four ? 32 : 8) || dim > kMaxPagedDim) {
+    set_errorf(fn, four ? "dim must be a multiple of 32 up to 256"
+                        : "dim must be a multiple of 8 up to 256");
+    return nullptr;
+  }
+  if (!aligned_to(d_k_pages, 16, fn) || !aligned_to(d_v_pages, 16, fn)) {
+    set_errorf(fn, "pages must be aligned to 16 bytes");
+    return nullptr;
+  }
+  const size_t token = four ? (size_t)17 * dim / 32 : size_of(io_type) * dim;
+  const size_t page = token * page_size * (size_t)n_heads;
+  if ((size_t)n_pages > ((size_t)1 << 60) / page) {
+    set_errorf(fn, "the pages are too large");
+    return nullptr;
+  }
+  const uintptr_t k = reinterpret_cast<uintptr_t>(d_k_pages),
+                  v = reinterpret_cast<uintptr_t>(d_v_pages);
+  if (k < v + page * n_pages && v < k + page * n_pages) {
+    set_errorf(fn, "d_k_pages and d_v_pages overlap");
+    return nullptr;
+  }
+  const Rotary *r = static_cast<Rotary *>(rotary);
+  if (r && 2 * (int)r->steps.size() > dim) {
+    set_errorf(fn, "the rotary's rotary_dim is larger than dim");
+    return nullptr;
+  }
+  int device = 0, cus = 0;
+  if (hip_fail(hipGetDevice(&device), fn) ||
+      hip_fail(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device), fn))
+    return nullptr;
+  Paged *p = new (std::nothrow) Paged();
+  if (!p) {
+    set_errorf(fn, "host allocation failed");
+    return nullptr;
+  }
+  p->device = device;
+  p->four = four;
+  p->pool = page * n_pages;
+  p->shape = {d_k_pages, d_v_pages, n_pages, page_size, n_heads, dim,
+              static_cast<aq::IoType>(io_type), {}, cus};
+  hipError_t e = hipSuccess;
+  if (r) {
+    p->shape.rotary = r->table();
+    e = upload_steps(r->steps, &p->d_steps);  // its own: the rotary may be destroyed
+    p->shape.rotary.steps = p->d_steps;
+  }
+  const size_t ws = aq::paged_workspace_bytes(p->shape);
+  if (e == hipSuccess && ws) {
+    e = hipMalloc(&p->ws, ws);
+    if (e != hipSuccess) p->ws = nullptr;
+    if (e == hipSuccess) e = hipMemset(p->ws, 0, ws);
+    if (e == hipSuccess) e = hipDeviceSynchronize();  // before any stream may use it
+  }
+  if (hip_fail(e, fn)) {
+    destroy_paged(p);
+    return nullptr;
+  }
+  aq::clear_error();
+  return p;
+}
+
+int paged_append(Paged *p, const void *d_k, const void *d_v, int n_tokens, const size_t *nb,
+                 const aq::PagedSeqs &q, const int *d_offsets, void *stream, const char *fn) {
+  if (n_tokens < 0) {
+    set_errorf(fn, "negative n_tokens");
+    return -1;
+  }
+  if (!seqs_ok(q.table, q.width, q.stride, q.lengths, q.n_seqs, fn)) return -1;
+  if (!d_offsets && n_tokens != q.n_seqs) {
+    set_errorf(fn, "without d_offsets, n_tokens must be n_seqs (one token a sequence)");
+    return -1;
+  }
+  if (n_tokens == 0 || q.n_seqs == 0) {
+    aq::clear_error();
+    return 0;
+  }
+  if (!append_ok(p, d_k, d_v, n_tokens, nb, fn)) return -1;
+  if (d_offsets && !aligned_to(d_offsets, 4, fn)) return -1;
+  const aq::PagedAppend a{d_k, d_v, {nb[0], nb[1]}, {nb[2], nb[3]}, n_tokens, d_offsets};
+  DeviceGuard g(p->device);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (hip_fail(p->four ? aq::launch_paged4_append(p->shape, q, a, s)
+                       : aq::launch_paged_append(p->shape, q, a, s),
+               fn))
+    return -1;
+  aq::clear_error();
+  return 0;
+}
+
+// Queries of a call of one token a sequence, and for a step (k) its rows.
+struct Token {
+  const void *k, *v;
+  size_t kv_nb[4];
+  const void *q;
+  void *out;
+  int q_heads;
+  size_t q_nb[4];  // of q, of out
+  float scale;
+  int window;
+};
+
+int paged_token(Paged *p, const Token &t, const aq::PagedSeqs &q, const aq::PagedScores *scores,
+                const aq::PagedWeights *weights, void *stream, const char *fn) {
+  if (!seqs_ok(q.table, q.width, q.stride, q.lengths, q.n_seqs, fn) ||
+      !attend_ok(p, t.q, t.out, t.q_heads, q.n_seqs, t.q_nb, t.scale, t.window, fn))
+    return -1;
+  if (q.n_seqs == 0) {
+    aq::clear_error();
+    return 0;
+  }
+  const int H = p->shape.n_heads;
+  const size_t *nb = t.q_nb, *knb = t.kv_nb;
+  if (t.k && !append_ok(p, t.k, t.v, q.n_seqs, knb, fn)) return -1;
+  if (!out_apart(p, t.out, t.q_heads, nb[2], nb[3], t.q, t.q_heads, nb[0], nb[1], q.n_seqs, fn))
+    return -1;
+  if (t.k && (!out_apart(p, t.out, t.q_heads, nb[2], nb[3], t.k, H, knb[0], knb[1], q.n_seqs, fn) ||
+              !out_apart(p, t.out, t.q_heads, nb[2], nb[3], t.v, H, knb[2], knb[3], q.n_seqs, fn)))
+    return -1;
+  const aq::PagedAppend ap{t.k, t.v, {knb[0], knb[1]}, {knb[2], knb[3]}, q.n_seqs, nullptr};
+  const aq::PagedAppend *step = t.k ? &ap : nullptr;
+  const aq::PagedAttend a = attend_args(p, t.q, t.out, t.q_heads, nb[0], nb[1], nb[2], nb[3],
+                                        t.scale, t.window, t.k ? 1 : 0);
+  DeviceGuard g(p->device);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  if (p->four)
+    e = aq::launch_paged4_attend(p->shape, q, a, step, scores ? *scores : aq::PagedScores{}, p->ws, s);
+  else if (scores)
+    e = aq::launch_paged_shaped(p->shape, q, a, step, *scores,
+                                weights ? *weights : aq::PagedWeights{}, p->ws, s);
+  else
+    e = aq::launch_paged_attend(p->shape, q, a, step, p->ws, s);
+  if (hip_fail(e, fn)) return -1;
+  aq::clear_error();
+  return 0;
+}
+
+// Weights [n_seqs][n_heads][tokens] of a call, and the memory their scores take meanwhile.
+bool weights_ok(const Paged *p, float *w, size_t nb1, size_t nb2, const aq::PagedSeqs &q,
+                aq::PagedWeights *to, const char *fn) {
+  *to = aq::PagedWeights{};
+  if (!w) return true;
+  const size_t nb[2] = {nb1, nb2};
+  const int n[2] = {p->shape.n_heads, q.n_seqs};
+  if (!aligned_to(w, 4, fn) || !strides_ok(4, n, nb, 2, fn)) return false;
+  if (!rows_apart((size_t)q.width * p->shape.page_size * 4, n, nb, 2)) {
+    set_errorf(fn, "d_weights has rows of fewer than table_width * page_size values");
+    return false;
+  }
+  to->weights = w;
+  to->nb[0] = (int64_t)(nb1 / 4);
+  to->nb[1] = (int64_t)(nb2 / 4);
+  return true;
+}
+
+int paged_scored(Paged *p, const Token &t, const aq::PagedSeqs &q, const adaptq_scores_t *scores,
+                 float *d_weights, size_t w_nb1, size_t w_nb2, void *ws, size_t ws_bytes,
+                 void *stream, const char *fn) {
+  aq::PagedScores sc;
+  aq::PagedWeights w;
+  if (q.n_seqs < 0 || q.width < 0) return paged_token(p, t, q, nullptr, nullptr, stream, fn);
+  if (!scores_ok(scores, &sc, fn) || !weights_ok(p, d_weights, w_nb1, w_nb2, q, &w, fn)) return -1;
+  if (w.weights) {
+    if (t.q_heads <= 0 || t.q_heads % p->shape.n_heads || (long long)q.n_seqs * t.q_heads > INT_MAX)
+      return paged_token(p, t, q, nullptr, nullptr, stream, fn);  // (refuses)
+    if (!workspace_ok(ws, ws_bytes,
+                      aq::paged_weights_workspace(p->shape, t.q_heads, q.n_seqs, q.width), fn))
+      return -1;
+    w.workspace = ws;
+  }
+  Token to = t;
+  to.window = sc.window;
+  return paged_token(p, to, q, &sc, &w, stream, fn);
 }
 
 }  // namespace
@@ -415,82 +623,13 @@ int adaptq_rotary_device(adaptq_rotary_t h, const adaptq_rows_t *rows, int n_row
 
 adaptq_paged_t adaptq_paged_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
                                    int n_heads, int dim, int io_type, adaptq_rotary_t rotary) {
-  const char *fn = "adaptq_paged_create";
-  if (!require_pointer(d_k_pages, fn, "d_k_pages") || !require_pointer(d_v_pages, fn, "d_v_pages") ||
-      !io_ok(io_type, fn))
-    return nullptr;
-  if (n_pages <= 0 || n_heads <= 0 || n_heads > kMaxHeads) {
-    set_errorf(fn, "n_pages must be positive, n_heads from 1 to 32768");
-    return nullptr;
-  }
-  if (page_size <= 0 || page_size % kPageUnit || page_size > kMaxPageSize) {
-    set_errorf(fn, "page_size must be a multiple of 16 up to 65536");
-    return nullptr;
-  }
-  if (dim <= 0 || dim % 8 || dim > kMaxPagedDim) {
-    set_errorf(fn, "dim must be a multiple of 8 up to 256");
-    return nullptr;
-  }
-  if (!aligned_to(d_k_pages, 16, fn) || !aligned_to(d_v_pages, 16, fn)) {
-    set_errorf(fn, "pages must be aligned to 16 bytes");
-    return nullptr;
-  }
-  const size_t page = size_of(io_type) * dim * page_size * (size_t)n_heads;
-  if ((size_t)n_pages > ((size_t)1 << 60) / page) {
-    set_errorf(fn, "the pages are too large");
-    return nullptr;
-  }
-  const uintptr_t k = reinterpret_cast<uintptr_t>(d_k_pages),
-                  v = reinterpret_cast<uintptr_t>(d_v_pages);
-  if (k < v + page * n_pages && v < k + page * n_pages) {
-    set_errorf(fn, "d_k_pages and d_v_pages overlap");
-    return nullptr;
-  }
-  const Rotary *r = static_cast<Rotary *>(rotary);
-  if (r && 2 * (int)r->steps.size() > dim) {
-    set_errorf(fn, "the rotary's rotary_dim is larger than dim");
-    return nullptr;
-  }
-  int device = 0, cus = 0;
-  if (hip_fail(hipGetDevice(&device), fn) ||
-      hip_fail(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device), fn))
-    return nullptr;
-  Paged *p = new (std::nothrow) Paged();
-  if (!p) {
-    set_errorf(fn, "host allocation failed");
-    return nullptr;
-  }
-  p->device = device;
-  p->shape = {d_k_pages, d_v_pages, n_pages, page_size, n_heads, dim,
-              static_cast<aq::IoType>(io_type), {}, cus};
-  hipError_t e = hipSuccess;
-  if (r) {
-    p->shape.rotary = r->table();
-    e = upload_steps(r->steps, &p->d_steps);  // its own: the rotary may be destroyed
-    p->shape.rotary.steps = p->d_steps;
-  }
-  const size_t ws = aq::paged_workspace_bytes(p->shape);
-  if (e == hipSuccess && ws) {
-    e = hipMalloc(&p->ws, ws);
-    if (e != hipSuccess) p->ws = nullptr;
-    if (e == hipSuccess) e = hipMemset(p->ws, 0, ws);
-    if (e == hipSuccess) e = hipDeviceSynchronize();  // before any stream may use it
-  }
-  if (hip_fail(e, fn)) {
-    adaptq_paged_destroy(p);
-    return nullptr;
-  }
-  aq::clear_error();
-  return p;
+  return create_paged(d_k_pages, d_v_pages, n_pages, page_size, n_heads, dim, io_type, rotary,
+                      false, "adaptq_paged_create");
 }
 
 void adaptq_paged_destroy(adaptq_paged_t h) {
   if (!h) return;
-  Paged *p = static_cast<Paged *>(h);
-  DeviceGuard g(p->device);
-  if (p->d_steps) (void)hipFree(p->d_steps);  // waits for the device
-  if (p->ws) (void)hipFree(p->ws);
-  delete p;
+  destroy_paged(static_cast<Paged *>(h));
 }
 
 int adaptq_paged_append_device(adaptq_paged_t h, const void *d_k, const void *d_v, int n_tokens,
@@ -500,7 +639,166 @@ int adaptq_paged_append_device(adaptq_paged_t h, const void *d_k, const void *d_
                                void *stream) {
   const char *fn = "adaptq_paged_append_device";
   if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn)) return -1;
+  const size_t nb[4] = {k_nb1, k_nb2, v_nb1, v_nb2};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_append(p, d_k, d_v, n_tokens, nb, q, d_offsets, stream, fn);
+}
+
+int adaptq_paged_attend_device(adaptq_paged_t h, const void *d_q, void *d_out, int n_q_heads,
+                               size_t q_nb1, size_t q_nb2, size_t out_nb1, size_t out_nb2,
+                               const int *d_table, int table_width, int table_stride,
+                               const int *d_lengths, int n_seqs, float scale, int window,
+                               void *stream) {
+  const char *fn = "adaptq_paged_attend_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn)) return -1;
+  const Token t{nullptr, nullptr, {}, d_q, d_out, n_q_heads, {q_nb1, q_nb2, out_nb1, out_nb2},
+                scale, window};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_token(p, t, q, nullptr, nullptr, stream, fn);
+}
+
+int adaptq_paged_step_device(adaptq_paged_t h, const void *d_k, const void *d_v, size_t k_nb1,
+                             size_t k_nb2, size_t v_nb1, size_t v_nb2, const void *d_q,
+                             void *d_out, int n_q_heads, size_t q_nb1, size_t q_nb2,
+                             size_t out_nb1, size_t out_nb2, const int *d_table, int table_width,
+                             int table_stride, const int *d_lengths, int n_seqs, float scale,
+                             int window, void *stream) {
+  const char *fn = "adaptq_paged_step_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn) || (n_seqs > 0 && !require_pointer(d_k, fn, "d_k"))) return -1;
+  const Token t{d_k, d_v, {k_nb1, k_nb2, v_nb1, v_nb2}, d_q, d_out, n_q_heads,
+                {q_nb1, q_nb2, out_nb1, out_nb2}, scale, window};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_token(p, t, q, nullptr, nullptr, stream, fn);
+}
+
+size_t adaptq_paged_weights_workspace(adaptq_paged_t h, int n_q_heads, int n_seqs,
+                                      int table_width) {
+  if (!h || n_q_heads <= 0 || n_seqs <= 0 || table_width < 0) return 0;
   const Paged *p = static_cast<Paged *>(h);
+  return aq::paged_weights_workspace(p->shape, n_q_heads, n_seqs, table_width);
+}
+
+int adaptq_paged_attend_scores_device(adaptq_paged_t h, const void *d_q, void *d_out,
+                                      int n_q_heads, size_t q_nb1, size_t q_nb2, size_t out_nb1,
+                                      size_t out_nb2, const int *d_table, int table_width,
+                                      int table_stride, const int *d_lengths, int n_seqs,
+                                      float scale, const adaptq_scores_t *scores,
+                                      float *d_weights, size_t w_nb1, size_t w_nb2,
+                                      void *d_workspace, size_t workspace_bytes, void *stream) {
+  const char *fn = "adaptq_paged_attend_scores_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn)) return -1;
+  const Token t{nullptr, nullptr, {}, d_q, d_out, n_q_heads, {q_nb1, q_nb2, out_nb1, out_nb2},
+                scale, 0};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_scored(p, t, q, scores, d_weights, w_nb1, w_nb2, d_workspace, workspace_bytes,
+                      stream, fn);
+}
+
+int adaptq_paged_step_scores_device(adaptq_paged_t h, const void *d_k, const void *d_v,
+                                    size_t k_nb1, size_t k_nb2, size_t v_nb1, size_t v_nb2,
+                                    const void *d_q, void *d_out, int n_q_heads, size_t q_nb1,
+                                    size_t q_nb2, size_t out_nb1, size_t out_nb2,
+                                    const int *d_table, int table_width, int table_stride,
+                                    const int *d_lengths, int n_seqs, float scale,
+                                    const adaptq_scores_t *scores, float *d_weights, size_t w_nb1,
+                                    size_t w_nb2, void *d_workspace, size_t workspace_bytes,
+                                    void *stream) {
+  const char *fn = "adaptq_paged_step_scores_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn) || (n_seqs > 0 && !require_pointer(d_k, fn, "d_k"))) return -1;
+  const Token t{d_k, d_v, {k_nb1, k_nb2, v_nb1, v_nb2}, d_q, d_out, n_q_heads,
+                {q_nb1, q_nb2, out_nb1, out_nb2}, scale, 0};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_scored(p, t, q, scores, d_weights, w_nb1, w_nb2, d_workspace, workspace_bytes,
+                      stream, fn);
+}
+
+int adaptq_paged_evict_device(adaptq_paged_t h, float *d_weights, size_t w_nb1, size_t w_nb2,
+                              const int *d_table, int table_width, int table_stride,
+                              const int *d_lengths, int n_seqs, int keep, int recent,
+                              const int *d_into, int into_width, int into_stride, int *d_kept,
+                              void *stream) {
+  const char *fn = "adaptq_paged_evict_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn)) return -1;
+  if (p->shape.rotary.pairs) {
+    set_errorf(fn, "a cache with a rotary takes positions from its lengths, which eviction changes");
+    return -1;
+  }
+  if (keep <= 0 || recent < 0 || recent > keep) {
+    set_errorf(fn, "keep must be positive, recent from 0 to keep");
+    return -1;
+  }
+  if (!seqs_ok(d_table, table_width, table_stride, d_lengths, n_seqs, fn)) return -1;
+  if (d_into && (into_width < 0 || into_stride < into_width)) {
+    set_errorf(fn, "into_stride is smaller than into_width, or one is negative");
+    return -1;
+  }
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  aq::PagedWeights w;
+  if (n_seqs == 0) {
+    aq::clear_error();
+    return 0;
+  }
+  if (!require_pointer(d_weights, fn, "d_weights") || !require_pointer(d_kept, fn, "d_kept") ||
+      !aligned_to(d_kept, 4, fn) || !aligned_to(d_into, 4, fn) ||
+      !weights_ok(p, d_weights, w_nb1, w_nb2, q, &w, fn))
+    return -1;
+  if ((size_t)n_seqs * p->shape.n_heads > ((size_t)1 << 58) / (size_t)keep) {
+    set_errorf(fn, "d_kept is too large");
+    return -1;
+  }
+  const aq::PagedEvict e{w.weights, {w.nb[0], w.nb[1]}, keep, recent,
+                         d_into, into_width, into_stride, d_kept};
+  DeviceGuard g(p->device);
+  if (hip_fail(aq::launch_paged_evict(p->shape, q, e, static_cast<hipStream_t>(stream)), fn))
+    return -1;
+  aq::clear_error();
+  return 0;
+}
+
+adaptq_paged4_t adaptq_paged4_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
+                                     int n_heads, int dim, int io_type, adaptq_rotary_t rotary) {
+  return create_paged(d_k_pages, d_v_pages, n_pages, page_size, n_heads, dim, io_type, rotary,
+                      true, "adaptq_paged4_create");
+}
+
+void adaptq_paged4_destroy(adaptq_paged4_t h) {
+  if (h) destroy_paged(static_cast<Paged *>(h));
+}
+
+int adaptq_paged4_append_device(adaptq_paged4_t h, const void *d_k, const void *d_v, int n_tokens,
+                                size_t k_nb1, size_t k_nb2, size_t v_nb1, size_t v_nb2,
+                                const int *d_table, int table_width, int table_stride,
+                                const int *d_lengths, int n_seqs, const int *d_offsets,
+                                void *stream) {
+  const char *fn = "adaptq_paged4_append_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!four_bits(p, fn)) return -1;
+  const size_t nb[4] = {k_nb1, k_nb2, v_nb1, v_nb2};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_append(p, d_k, d_v, n_tokens, nb, q, d_offsets, stream, fn);
+}
+
+int adaptq_paged4_read_device(adaptq_paged4_t h, float *d_k, float *d_v, int n_tokens,
+                              const int *d_table, int table_width, int table_stride,
+                              const int *d_lengths, int n_seqs, const int *d_offsets,
+                              void *stream) {
+  const char *fn = "adaptq_paged4_read_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!four_bits(p, fn)) return -1;
   if (n_tokens < 0) {
     set_errorf(fn, "negative n_tokens");
     return -1;
@@ -514,79 +812,62 @@ int adaptq_paged_append_device(adaptq_paged_t h, const void *d_k, const void *d_
     aq::clear_error();
     return 0;
   }
-  const size_t nb[4] = {k_nb1, k_nb2, v_nb1, v_nb2};
-  if (!append_ok(p, d_k, d_v, n_tokens, nb, fn)) return -1;
-  if (d_offsets && !aligned_to(d_offsets, 4, fn)) return -1;
-  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
-  const aq::PagedAppend a{d_k, d_v, {k_nb1, k_nb2}, {v_nb1, v_nb2}, n_tokens, d_offsets};
-  DeviceGuard g(p->device);
-  if (hip_fail(aq::launch_paged_append(p->shape, q, a, static_cast<hipStream_t>(stream)), fn))
+  if (!require_pointer(d_k, fn, "d_k") || !require_pointer(d_v, fn, "d_v") ||
+      !aligned_to(d_k, 16, fn) || !aligned_to(d_v, 16, fn) || !aligned_to(d_offsets, 4, fn))
     return -1;
-  aq::clear_error();
-  return 0;
-}
-
-int adaptq_paged_attend_device(adaptq_paged_t h, const void *d_q, void *d_out, int n_q_heads,
-                               size_t q_nb1, size_t q_nb2, size_t out_nb1, size_t out_nb2,
-                               const int *d_table, int table_width, int table_stride,
-                               const int *d_lengths, int n_seqs, float scale, int window,
-                               void *stream) {
-  const char *fn = "adaptq_paged_attend_device";
-  if (!require_handle(h, fn)) return -1;
-  Paged *p = static_cast<Paged *>(h);
-  const size_t nb[4] = {q_nb1, q_nb2, out_nb1, out_nb2};
-  if (!seqs_ok(d_table, table_width, table_stride, d_lengths, n_seqs, fn) ||
-      !attend_ok(p, d_q, d_out, n_q_heads, n_seqs, nb, scale, window, fn))
+  const size_t bytes = (size_t)n_tokens * p->shape.n_heads * p->shape.dim * 4;
+  const uintptr_t k = reinterpret_cast<uintptr_t>(d_k), v = reinterpret_cast<uintptr_t>(d_v);
+  if (k < v + bytes && v < k + bytes) {
+    set_errorf(fn, "d_k and d_v overlap");
     return -1;
-  if (n_seqs == 0) {
-    aq::clear_error();
-    return 0;
   }
-  if (!out_apart(p, d_out, n_q_heads, out_nb1, out_nb2, d_q, n_q_heads, q_nb1, q_nb2, n_seqs, fn))
-    return -1;
+  for (const uintptr_t x : {k, v})
+    for (const void *pool : {p->shape.k_pages, p->shape.v_pages}) {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(pool);
+      if (x < lo + p->pool && lo < x + bytes) {
+        set_errorf(fn, "rows overlap the pages");
+        return -1;
+      }
+    }
   const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
-  const aq::PagedAttend a =
-      attend_args(p, d_q, d_out, n_q_heads, q_nb1, q_nb2, out_nb1, out_nb2, scale, window, 0);
   DeviceGuard g(p->device);
-  if (hip_fail(aq::launch_paged_attend(p->shape, q, a, nullptr, p->ws, static_cast<hipStream_t>(stream)),
+  if (hip_fail(aq::launch_paged4_read(p->shape, q, n_tokens, d_offsets, d_k, d_v,
+                                      static_cast<hipStream_t>(stream)),
                fn))
     return -1;
   aq::clear_error();
   return 0;
 }
 
-int adaptq_paged_step_device(adaptq_paged_t h, const void *d_k, const void *d_v, size_t k_nb1,
-                             size_t k_nb2, size_t v_nb1, size_t v_nb2, const void *d_q,
-                             void *d_out, int n_q_heads, size_t q_nb1, size_t q_nb2,
-                             size_t out_nb1, size_t out_nb2, const int *d_table, int table_width,
-                             int table_stride, const int *d_lengths, int n_seqs, float scale,
-                             int window, void *stream) {
-  const char *fn = "adaptq_paged_step_device";
+int adaptq_paged4_attend_device(adaptq_paged4_t h, const void *d_q, void *d_out, int n_q_heads,
+                                size_t q_nb1, size_t q_nb2, size_t out_nb1, size_t out_nb2,
+                                const int *d_table, int table_width, int table_stride,
+                                const int *d_lengths, int n_seqs, float scale,
+                                const adaptq_scores_t *scores, void *stream) {
+  const char *fn = "adaptq_paged4_attend_device";
   if (!require_handle(h, fn)) return -1;
   Paged *p = static_cast<Paged *>(h);
-  const size_t knb[4] = {k_nb1, k_nb2, v_nb1, v_nb2}, qnb[4] = {q_nb1, q_nb2, out_nb1, out_nb2};
-  if (!seqs_ok(d_table, table_width, table_stride, d_lengths, n_seqs, fn) ||
-      !attend_ok(p, d_q, d_out, n_q_heads, n_seqs, qnb, scale, window, fn))
-    return -1;
-  if (n_seqs == 0) {
-    aq::clear_error();
-    return 0;
-  }
-  const int H = p->shape.n_heads;
-  if (!append_ok(p, d_k, d_v, n_seqs, knb, fn) ||
-      !out_apart(p, d_out, n_q_heads, out_nb1, out_nb2, d_q, n_q_heads, q_nb1, q_nb2, n_seqs, fn) ||
-      !out_apart(p, d_out, n_q_heads, out_nb1, out_nb2, d_k, H, k_nb1, k_nb2, n_seqs, fn) ||
-      !out_apart(p, d_out, n_q_heads, out_nb1, out_nb2, d_v, H, v_nb1, v_nb2, n_seqs, fn))
-    return -1;
+  if (!four_bits(p, fn)) return -1;
+  const Token t{nullptr, nullptr, {}, d_q, d_out, n_q_heads, {q_nb1, q_nb2, out_nb1, out_nb2},
+                scale, 0};
   const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
-  const aq::PagedAppend ap{d_k, d_v, {k_nb1, k_nb2}, {v_nb1, v_nb2}, n_seqs, nullptr};
-  const aq::PagedAttend a =
-      attend_args(p, d_q, d_out, n_q_heads, q_nb1, q_nb2, out_nb1, out_nb2, scale, window, 1);
-  DeviceGuard g(p->device);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (hip_fail(aq::launch_paged_attend(p->shape, q, a, &ap, p->ws, s), fn)) return -1;
-  aq::clear_error();
-  return 0;
+  return paged_scored(p, t, q, scores, nullptr, 0, 0, nullptr, 0, stream, fn);
+}
+
+int adaptq_paged4_step_device(adaptq_paged4_t h, const void *d_k, const void *d_v, size_t k_nb1,
+                              size_t k_nb2, size_t v_nb1, size_t v_nb2, const void *d_q,
+                              void *d_out, int n_q_heads, size_t q_nb1, size_t q_nb2,
+                              size_t out_nb1, size_t out_nb2, const int *d_table, int table_width,
+                              int table_stride, const int *d_lengths, int n_seqs, float scale,
+                              const adaptq_scores_t *scores, void *stream) {
+  const char *fn = "adaptq_paged4_step_device";
+  if (!require_handle(h, fn)) return -1;
+  Paged *p = static_cast<Paged *>(h);
+  if (!four_bits(p, fn) || (n_seqs > 0 && !require_pointer(d_k, fn, "d_k"))) return -1;
+  const Token t{d_k, d_v, {k_nb1, k_nb2, v_nb1, v_nb2}, d_q, d_out, n_q_heads,
+                {q_nb1, q_nb2, out_nb1, out_nb2}, scale, 0};
+  const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
+  return paged_scored(p, t, q, scores, nullptr, 0, 0, nullptr, 0, stream, fn);
 }
 
 size_t adaptq_paged_prompt_workspace(adaptq_paged_t h, int n_q_heads, int n_tokens, int n_seqs,
@@ -606,6 +887,7 @@ int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, i
   const char *fn = "adaptq_paged_prompt_device";
   if (!require_handle(h, fn)) return -1;
   Paged *p = static_cast<Paged *>(h);
+  if (!exact_pages(p, fn)) return -1;
   if (n_tokens < 0) {
     set_errorf(fn, "negative n_tokens");
     return -1;

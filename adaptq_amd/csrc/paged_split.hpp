@@ -74,6 +74,57 @@ AQ_SPLIT_HD TokenSpan token_span(int length, int extra, int window, int64_t cap,
   return s;
 }
 
+// The same where tokens before `first` are hidden and those before `prefix` stay seen behind a
+// window: [lo, n) without [hole0, hole1).  Units inside the hole are not counted: from gap_at on,
+// unit u of the launch is unit u + gap of the sequence.
+struct SeenSpan : TokenSpan {
+  int hole0, hole1;
+  int gap_at, gap;
+};
+
+AQ_SPLIT_HD SeenSpan seen_span(int length, int extra, int window, int64_t cap, int unit, int least,
+                               int first, int prefix) {
+  SeenSpan s;
+  const TokenSpan all = token_span(length, extra, 0, cap, unit, 1);
+  const int n = all.n;
+  const int64_t held = length < 0 ? 0 : (int64_t)length + extra;
+  const int64_t back = window > 0 && held > window ? held - window : 0;
+  const int w = (int)(back < n ? back : n);
+  const int f = first < 0 ? 0 : first < n ? first : n, p = prefix < 0 ? 0 : prefix < n ? prefix : n;
+  s.n = n;
+  s.hole0 = s.hole1 = n;
+  if (w <= p) {
+    s.lo = f;
+  } else if (f >= p) {
+    s.lo = f > w ? f : w;
+  } else {
+    s.lo = f;
+    s.hole0 = p;
+    s.hole1 = w;
+  }
+  s.first_unit = s.lo / unit;
+  s.units = s.lo < n ? (n - 1) / unit + 1 - s.first_unit : 1;
+  s.gap_at = 0x7FFFFFFF;
+  s.gap = 0;
+  if (s.hole0 < s.hole1) {
+    // the units that hold tokens before the hole end here; those behind it may begin in the same
+    const int end = (s.hole0 - 1) / unit + 1, next = s.hole1 / unit;
+    if (next > end) {
+      s.gap_at = end;
+      s.gap = next - end;
+      // (a window that ends behind the table leaves nothing behind the hole)
+      s.units -= s.hole1 < n ? s.gap : (n - 1) / unit + 1 - end;
+    }
+  }
+  s.short_ = s.units <= least;
+  if (s.short_) s.units = least;
+  return s;
+}
+
+AQ_SPLIT_HD int real_unit(const SeenSpan &s, int unit) {
+  return unit >= s.gap_at ? unit + s.gap : unit;
+}
+
 // Units of a block: an equal share of the total, in whole passes of the block's waves.
 AQ_SPLIT_HD int64_t share_of(int64_t total, int blocks, int waves) {
   const int64_t s = ((total + blocks - 1) / blocks + waves - 1) / waves * waves;

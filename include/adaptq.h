@@ -511,6 +511,84 @@ int adaptq_paged_prompt_device(adaptq_paged_t cache, const void *d_q, void *d_ou
                                const int *d_offsets, float scale, const adaptq_scores_t *scores,
                                void *d_workspace, size_t workspace_bytes, void *stream);
 
+/* attend and step with scores of their own (NULL: none), one query a sequence at position
+ * n - 1 (of the n tokens it then holds).  d_weights, NULL or fp32 [n_seqs][n_heads] rows of at
+ * least table_width * page_size values, w_nb1 and w_nb2 bytes apart: to each token that is
+ * seen, the sum of its weights in the softmaxes of its key head's query heads is added (in
+ * their order; one more launch).  d_workspace: then device memory of
+ * adaptq_paged_weights_workspace bytes (4 a column of the table, slot and query head),
+ * 16-byte aligned, this call's alone until it is done.  Returns 0/-1. */
+size_t adaptq_paged_weights_workspace(adaptq_paged_t cache, int n_q_heads, int n_seqs,
+                                      int table_width);
+int adaptq_paged_attend_scores_device(adaptq_paged_t cache, const void *d_q, void *d_out,
+                                      int n_q_heads, size_t q_nb1, size_t q_nb2, size_t out_nb1,
+                                      size_t out_nb2, const int *d_table, int table_width,
+                                      int table_stride, const int *d_lengths, int n_seqs,
+                                      float scale, const adaptq_scores_t *scores,
+                                      float *d_weights, size_t w_nb1, size_t w_nb2,
+                                      void *d_workspace, size_t workspace_bytes, void *stream);
+int adaptq_paged_step_scores_device(adaptq_paged_t cache, const void *d_k, const void *d_v,
+                                    size_t k_nb1, size_t k_nb2, size_t v_nb1, size_t v_nb2,
+                                    const void *d_q, void *d_out, int n_q_heads, size_t q_nb1,
+                                    size_t q_nb2, size_t out_nb1, size_t out_nb2,
+                                    const int *d_table, int table_width, int table_stride,
+                                    const int *d_lengths, int n_seqs, float scale,
+                                    const adaptq_scores_t *scores, float *d_weights, size_t w_nb1,
+                                    size_t w_nb2, void *d_workspace, size_t workspace_bytes,
+                                    void *stream);
+
+/* evict: of each sequence and key head that holds n > keep tokens, `keep` stay: the `recent`
+ * last ones, and of the others those of the largest d_weights (of equal ones the earlier; NaN
+ * counts as larger than infinity, or if negative as smaller than all).  They move, in their
+ * order, to the first `keep` places of the sequence: in place, or with d_into to the pages
+ * that it names (rows of into_width page numbers, into_stride ints apart; none of them pages
+ * that the sequences hold), where sequences of up to `keep` tokens are copied whole.  Their
+ * weights move likewise within d_weights, with zeros behind (of sequences over `keep`).
+ * d_kept [n_seqs][n_heads][keep]: where each place's token lay, -1 where there is none.
+ * d_lengths is read alone: the caller lowers it to at most keep after the call.  Rows without
+ * a page, or without one to go to, are not moved.  A page that several of the call's
+ * sequences hold may not be evicted in place.  Caches with a rotary are refused.  Returns 0/-1. */
+int adaptq_paged_evict_device(adaptq_paged_t cache, float *d_weights, size_t w_nb1, size_t w_nb2,
+                              const int *d_table, int table_width, int table_stride,
+                              const int *d_lengths, int n_seqs, int keep, int recent,
+                              const int *d_into, int into_width, int into_stride, int *d_kept,
+                              void *stream);
+
+/* A cache of 4-bit values in pages.  32 consecutive channels of a row (after its rotation, which
+ * rounds to io_type) share the scale 2^e, the smallest that takes the largest of them to 6 or
+ * below (-125 <= e <= 125); each value is held as its sign and the nearest of 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 times the scale, of two equally near ones 0, 1, 2 or 4, at most 6; if one of the 32 is
+ * infinite or NaN, all read as NaN.  dim a multiple of 32 up to 256; io_type is the type of the
+ * calls' rows.  The pools are the caller's, [n_pages][n_heads][page_size] * 17 * dim / 32 bytes
+ * each, 16-byte aligned, their inside the library's.  append, attend and step are the exact
+ * cache's, attention reading the values as they are held (a step's own token too), scores as
+ * above.  read: the values of the tokens that an append of the same arguments writes, d_k and
+ * d_v fp32 [n_tokens][n_heads][dim], 16-byte aligned; zeros where there is no page. */
+typedef void *adaptq_paged4_t;
+adaptq_paged4_t adaptq_paged4_create(void *d_k_pages, void *d_v_pages, int n_pages, int page_size,
+                                     int n_heads, int dim, int io_type, adaptq_rotary_t rotary);
+void adaptq_paged4_destroy(adaptq_paged4_t cache);
+int adaptq_paged4_append_device(adaptq_paged4_t cache, const void *d_k, const void *d_v,
+                                int n_tokens, size_t k_nb1, size_t k_nb2, size_t v_nb1,
+                                size_t v_nb2, const int *d_table, int table_width,
+                                int table_stride, const int *d_lengths, int n_seqs,
+                                const int *d_offsets, void *stream);
+int adaptq_paged4_read_device(adaptq_paged4_t cache, float *d_k, float *d_v, int n_tokens,
+                              const int *d_table, int table_width, int table_stride,
+                              const int *d_lengths, int n_seqs, const int *d_offsets,
+                              void *stream);
+int adaptq_paged4_attend_device(adaptq_paged4_t cache, const void *d_q, void *d_out,
+                                int n_q_heads, size_t q_nb1, size_t q_nb2, size_t out_nb1,
+                                size_t out_nb2, const int *d_table, int table_width,
+                                int table_stride, const int *d_lengths, int n_seqs, float scale,
+                                const adaptq_scores_t *scores, void *stream);
+int adaptq_paged4_step_device(adaptq_paged4_t cache, const void *d_k, const void *d_v,
+                              size_t k_nb1, size_t k_nb2, size_t v_nb1, size_t v_nb2,
+                              const void *d_q, void *d_out, int n_q_heads, size_t q_nb1,
+                              size_t q_nb2, size_t out_nb1, size_t out_nb2, const int *d_table,
+                              int table_width, int table_stride, const int *d_lengths, int n_seqs,
+                              float scale, const adaptq_scores_t *scores, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
