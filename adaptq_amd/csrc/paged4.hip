@@ -18,6 +18,7 @@ struct Args {
   PagedAppend a;
   float *k_out, *v_out;  // read: [n_tokens][n_heads][dim]
   int first_token, tokens_per_block;
+  uint64_t token_mul;    // row / tokens_per_block = row * token_mul >> 32, for a block's rows
   bool vec;              // rows of 16 bytes' alignment
 };
 
@@ -46,18 +47,54 @@ __device__ __forceinline__ void find_token(const Args &g, int t, int *page, int 
   if (x >= 0 && x < g.p.n_pages) *page = x;
 }
 
-// A block takes a few tokens of all heads; a lane 8 channels of a (token, head)'s key and value,
-// four neighbours a scale.  Bound: the input rows' bytes.
+// A block takes a few tokens of all heads; a lane 8 channels of the keys or values of a (token,
+// head), four neighbours a scale, kRows rows of them in flight.  Rows go token by token within a
+// head, so that neighbouring rows' codes, which lie side by side in a block of 16 tokens, are
+// written together.  Bound: the bytes.
+constexpr int kRows = 4;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
   __shared__ float2 s_cs[kCosSin];
   __shared__ int s_page[kBlockTokens], s_pos[kBlockTokens];
-  const int tid = threadIdx.x, dim = g.p.dim, heads = g.p.n_heads;
-  const int t0 = g.first_token + blockIdx.x * g.tokens_per_block;
-  const int nt = min(g.tokens_per_block, g.a.n_tokens - t0);
+  const int tid = threadIdx.x, dim = g.p.dim, tb = g.tokens_per_block;
+  const int t0 = g.first_token + blockIdx.x * tb;
+  const int nt = min(tb, g.a.n_tokens - t0);
+  const RotaryTable &rt = g.p.rotary;
+  const int lanes = dim / 8, rows = g.p.n_heads * tb;
+  const int per = kThreads / (2 * lanes);  // rows of a pass: keys, then values
+  const int item = tid % (2 * lanes), row0 = tid < per * 2 * lanes ? tid / (2 * lanes) : rows;
+  const bool value = item >= lanes;
+  const int chunk = value ? item - lanes : item;
+  const char *in = static_cast<const char *>(value ? g.a.v : g.a.k) + t0 * (int64_t)(value ? g.a.v_nb[1] : g.a.k_nb[1]);
+  const int64_t nb1 = value ? g.a.v_nb[0] : g.a.k_nb[0], nb2 = value ? g.a.v_nb[1] : g.a.k_nb[1];
+  float x[kRows][8];
+  int tok[kRows], head[kRows];
+  const auto load = [&](int r0) {
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const int r = r0 + j * per;
+      head[j] = (int)((uint64_t)r * g.token_mul >> 32);
+      tok[j] = r < rows ? r - head[j] * tb : nt;
+      if (tok[j] >= nt) continue;
+      const T *from = reinterpret_cast<const T *>(in + tok[j] * nb2 + head[j] * nb1) + 8 * chunk;
+      if (g.vec) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int k = 0; k < 8; k += N) {
+          const RowVec<T, N> y = load_rows<true, T, N>(from + k);
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[j][k + i] = row_get(y.x[i]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[j][k] = row_get(from[k]);
+      }
+    }
+  };
+  load(row0);
   for (int t = tid; t < nt; t += kThreads) find_token(g, t0 + t, &s_page[t], &s_pos[t]);
   __syncthreads();
-  const RotaryTable &rt = g.p.rotary;
   if (rt.pairs) {
     for (int i = tid; i < nt * rt.pairs; i += kThreads) {
       const int t = i / rt.pairs;
@@ -65,85 +102,83 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
     }
     __syncthreads();
   }
-  const int lanes = dim / 8, items = nt * heads * lanes;
-  // (whole groups of four lanes: items is a multiple of 4)
-  for (int i = tid; i < items; i += kThreads) {
-    const int row = i / lanes, chunk = i - row * lanes;
-    const int t = row / heads, head = row - t * heads;
-    const void *rows[2] = {
-        static_cast<const char *>(g.a.k) + (t0 + t) * (int64_t)g.a.k_nb[1] + head * (int64_t)g.a.k_nb[0],
-        static_cast<const char *>(g.a.v) + (t0 + t) * (int64_t)g.a.v_nb[1] + head * (int64_t)g.a.v_nb[0]};
-    float x[2][8];
+  char *pool = static_cast<char *>(value ? g.p.v_pages : g.p.k_pages);
+  // (the four lanes of a scale have the same rows)
+  for (int r0 = row0; r0 < rows; r0 += kRows * per) {
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      const T *from = static_cast<const T *>(rows[v]) + 8 * chunk;
-      if (g.vec) {
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int k = 0; k < 8; k += N) {
-          const RowVec<T, N> y = load_rows<true, T, N>(from + k);
-#pragma unroll
-          for (int j = 0; j < N; ++j) x[v][k + j] = row_get(y.x[j]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[v][k] = row_get(from[k]);
-      }
-    }
-    if (rt.pairs)
-      rotate8(x[0], rows[0], chunk, g.p.io, rt, [&](int pair) { return s_cs[t * rt.pairs + pair]; });
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
+    for (int j = 0; j < kRows; ++j) {
+      const int t = tok[j];
+      if (t >= nt) continue;
+      if (rt.pairs && !value)
+        rotate8(x[j], in + t * nb2 + head[j] * nb1, chunk, g.p.io, rt,
+                [&](int pair) { return s_cs[t * rt.pairs + pair]; });
       int byte;
-      const uint32_t codes = encode4(x[v], &byte);
+      const uint32_t codes = encode4(x[j], &byte);
       if (s_page[t] < 0) continue;
       const int slot = s_pos[t] % g.p.page_size;
-      store4(static_cast<char *>(v ? g.p.v_pages : g.p.k_pages) + block4_at(g.p, s_page[t], head, slot),
-             slot & 15, chunk, codes, byte, v, dim);
+      store4(pool + block4_at(g.p, s_page[t], head[j], slot), slot & 15, chunk, codes, byte, value,
+             dim);
     }
+    load(r0 + kRows * per);
   }
 }
 
+// The same way back, a lane 4 channels so that a wave writes whole lines.
 __global__ __launch_bounds__(kThreads) void read4_kernel(const Args g) {
   __shared__ int s_page[kBlockTokens], s_pos[kBlockTokens];
-  const int tid = threadIdx.x, dim = g.p.dim, heads = g.p.n_heads;
-  const int t0 = g.first_token + blockIdx.x * g.tokens_per_block;
-  const int nt = min(g.tokens_per_block, g.a.n_tokens - t0);
+  const int tid = threadIdx.x, dim = g.p.dim, tb = g.tokens_per_block;
+  const int t0 = g.first_token + blockIdx.x * tb;
+  const int nt = min(tb, g.a.n_tokens - t0);
   for (int t = tid; t < nt; t += kThreads) find_token(g, t0 + t, &s_page[t], &s_pos[t]);
   __syncthreads();
-  const int lanes = dim / 8, items = nt * heads * lanes;
-  for (int i = tid; i < items; i += kThreads) {
-    const int row = i / lanes, chunk = i - row * lanes;
-    const int t = row / heads, head = row - t * heads;
-    const int64_t to = ((int64_t)(t0 + t) * heads + head) * dim + 8 * chunk;
+  const int lanes = dim / 4, rows = g.p.n_heads * tb;
+  const int per = max(kThreads / (2 * lanes), 1);
+  for (int item = tid; item < per * 2 * lanes; item += kThreads) {
+    const int row0 = item / (2 * lanes), c = item - row0 * 2 * lanes;
+    const bool value = c >= lanes;
+    const int d = 4 * (value ? c - lanes : c);
+    const char *pool = static_cast<const char *>(value ? g.p.v_pages : g.p.k_pages);
+    float *out = (value ? g.v_out : g.k_out) + (int64_t)t0 * g.p.n_heads * dim + d;
+    for (int r0 = row0; r0 < rows; r0 += kRows * per) {
+      uint32_t codes[kRows];
+      int byte[kRows];
+      int64_t to[kRows];
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      uint32_t codes = 0;
-      int byte = 127;
-      if (s_page[t] >= 0) {
+      for (int j = 0; j < kRows; ++j) {
+        const int r = r0 + j * per;
+        const int head = (int)((uint64_t)r * g.token_mul >> 32), t = r - head * tb;
+        codes[j] = 0;
+        byte[j] = 127;
+        to[j] = -1;
+        if (r >= rows || t >= nt) continue;
+        to[j] = ((int64_t)t * g.p.n_heads + head) * dim;
+        if (s_page[t] < 0) continue;
         const int slot = s_pos[t] % g.p.page_size;
-        codes = load4(static_cast<const char *>(v ? g.p.v_pages : g.p.k_pages) +
-                          block4_at(g.p, s_page[t], head, slot),
-                      slot & 15, chunk, v, dim, &byte);
+        codes[j] = load4(pool + block4_at(g.p, s_page[t], head, slot), slot & 15, d, value, dim,
+                         &byte[j]);
       }
-      const float scale = scale4(byte);
-      float *out = (v ? g.v_out : g.k_out) + to;
 #pragma unroll
-      for (int k = 0; k < 8; k += 4) {
+      for (int j = 0; j < kRows; ++j) {
+        if (to[j] < 0) continue;
+        const float scale = scale4(byte[j]);
         RowVec<float, 4> y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y.x[j] = value4(codes >> 4 * (k + j), scale);
-        store_rows<true>(out + k, y);
+        for (int i = 0; i < 4; ++i) y.x[i] = value4(codes[j] >> 4 * i, scale);
+        store_rows<true>(out + to[j], y);
       }
     }
   }
 }
 
-// Tokens of a block: a few rounds of its threads, and no fewer than 2,048 blocks for it.
-int tokens_per_block(const PagedShape &p, int n_tokens, bool rotates) {
-  int tb = std::max(1, 8 * kThreads / (p.n_heads * p.dim / 8));
-  if (rotates && p.rotary.pairs) tb = std::min(tb, kCosSin / p.rotary.pairs);
-  return std::max(1, std::min({tb, kBlockTokens, n_tokens / 2048}));
+// Tokens of a block: a few rounds of its threads, of lanes for 8 channels, in fours that share a
+// place in the pages, and no fewer than 1,024 blocks for it.
+void cut_tokens(Args &g, int lanes, bool rotates) {
+  int tb = std::max(1, 4 * kRows * kThreads / (2 * lanes * g.p.n_heads));
+  if (rotates && g.p.rotary.pairs) tb = std::min(tb, kCosSin / g.p.rotary.pairs);
+  tb = std::max(1, std::min({tb, kBlockTokens, g.a.n_tokens / 1024}));
+  if (tb > 4) tb = tb / 4 * 4;
+  g.tokens_per_block = tb;
+  g.token_mul = (((uint64_t)1 << 32) + tb - 1) / tb;
 }
 
 }  // namespace
@@ -154,7 +189,7 @@ hipError_t launch_paged4_append(const PagedShape &p, const PagedSeqs &q, const P
   size_t x = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
   for (int k = 0; k < 2; ++k) x |= a.k_nb[k] | a.v_nb[k];
   g.vec = x % 16 == 0;
-  g.tokens_per_block = tokens_per_block(p, a.n_tokens, true);
+  cut_tokens(g, p.dim / 8, true);
   return launch_over_tokens(a.n_tokens, g.tokens_per_block, [&](int first, int blocks) {
     g.first_token = first;
     switch (p.io) {
@@ -172,7 +207,7 @@ hipError_t launch_paged4_read(const PagedShape &p, const PagedSeqs &q, int n_tok
   g.a.offsets = offsets;
   g.k_out = k;
   g.v_out = v;
-  g.tokens_per_block = tokens_per_block(p, n_tokens, false);
+  cut_tokens(g, p.dim / 4, false);
   return launch_over_tokens(n_tokens, g.tokens_per_block, [&](int first, int blocks) {
     g.first_token = first;
     read4_kernel<<<blocks, kThreads, 0, s>>>(g);

@@ -93,22 +93,20 @@ __device__ __forceinline__ void store4(char *at, int in, int chunk, uint32_t cod
   if (chunk % 4 == 0) scales[(group * blocks + chunk / 4) * 4 + token] = (char)byte;
 }
 
-// 8 channels of a token and their scale's byte.
-__device__ __forceinline__ uint32_t load4(const char *at, int in, int chunk, bool value, int dim,
+// 4 channels of a token, from channel d on, and their scale's byte.
+__device__ __forceinline__ uint32_t load4(const char *at, int in, int d, bool value, int dim,
                                           int *byte) {
   const int blocks = dim / kBlock4;
   const char *scales = at + 8 * dim;
   if (!value) {
-    *byte = (uint8_t)scales[in * blocks + chunk / 4];
-    return *reinterpret_cast<const uint32_t *>(at + in * (dim / 2) + 4 * chunk);
+    *byte = (uint8_t)scales[in * blocks + d / kBlock4];
+    return *reinterpret_cast<const uint16_t *>(at + in * (dim / 2) + d / 2);
   }
   const int group = in / 4, token = in % 4;
-  *byte = (uint8_t)scales[(group * blocks + chunk / 4) * 4 + token];
-  if (value_channels4(dim) == 8)
-    return *reinterpret_cast<const uint32_t *>(at + (group * (dim / 8) + chunk) * 16 + 4 * token);
-  const char *from = at + (group * (dim / 4) + 2 * chunk) * 8 + 2 * token;
-  return *reinterpret_cast<const uint16_t *>(from) |
-         (uint32_t)*reinterpret_cast<const uint16_t *>(from + 8) << 16;
+  *byte = (uint8_t)scales[(group * blocks + d / kBlock4) * 4 + token];
+  const int c = value_channels4(dim);
+  return *reinterpret_cast<const uint16_t *>(at + (group * (dim / c) + d / c) * 2 * c +
+                                             token * (c / 2) + d % c / 2);
 }
 
 // 8 channels of an input row, from channel 8 * chunk on: a key's rotated to its position and

@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kSelect = 1024;
 constexpr int kSelectWaves = kSelect / 64;
+constexpr int kBatch = 8;  // weights that a thread has under way
 constexpr int kMove = 256;
 constexpr int kInFlight = 8;  // rows of 16 bytes that a thread has under way
 
@@ -66,30 +67,33 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   for (int shift = 24; room > 0 && shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += kSelect) s_count[i] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < old; t0 += kSelect) {
-      const int t = t0 + tid;
-      bool counts = t < old;
-      uint32_t key = 0;
-      if (counts) {
-        key = key_of(w[t]);
-        counts = shift == 24 || key >> (shift + 8) == prefix >> (shift + 8);
-      }
-      const uint32_t digit = key >> shift & 255;
-      // equal digits of a wave are counted together, two of them at the most (tokens without
-      // any weight are many, and one counter takes one lane at a time)
+    for (int t0 = 0; t0 < old; t0 += kBatch * kSelect) {
+      float x[kBatch];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint64_t there = __ballot(counts);
-        if (!there) break;
-        const uint32_t of = __builtin_amdgcn_readlane(digit, __ffsll((unsigned long long)there) - 1);
-        const uint64_t same = __ballot(counts && digit == of);
-        if (counts && digit == of) {
-          if (lane == __ffsll((unsigned long long)same) - 1)
-            atomicAdd(&s_count[of], __popcll(same));
-          counts = false;
+      for (int j = 0; j < kBatch; ++j) x[j] = w[min(t0 + j * kSelect + tid, old - 1)];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (t0 + j * kSelect >= old) break;  // (uniform)
+        const uint32_t key = key_of(x[j]), digit = key >> shift & 255;
+        bool counts = t0 + j * kSelect + tid < old &&
+                      (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8));
+        // equal digits of a wave are counted together, two of them at the most (tokens without
+        // any weight are many, and one counter takes one lane at a time)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint64_t there = __ballot(counts);
+          if (!there) break;
+          const uint32_t of =
+              __builtin_amdgcn_readlane(digit, __ffsll((unsigned long long)there) - 1);
+          const uint64_t same = __ballot(counts && digit == of);
+          if (counts && digit == of) {
+            if (lane == __ffsll((unsigned long long)same) - 1)
+              atomicAdd(&s_count[of], __popcll(same));
+            counts = false;
+          }
         }
+        if (counts) atomicAdd(&s_count[digit], 1);
       }
-      if (counts) atomicAdd(&s_count[digit], 1);
     }
     __syncthreads();
     if (wave == 0) {  // the digit at which `room` values from the top are reached
@@ -129,10 +133,17 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   const int t0 = min(wave * per, old), t1 = min(t0 + per, old);
   const bool none = keep == g.e.recent;
   int gt = 0, eq = 0;
-  for (int t = t0 + lane; t - lane < t1; t += 64) {
-    const uint32_t key = t < t1 ? key_of(w[t]) : 0;
-    gt += __popcll(__ballot(t < t1 && !none && key > prefix));
-    eq += __popcll(__ballot(t < t1 && !none && key == prefix));
+  for (int u0 = t0; !none && u0 < t1; u0 += kBatch * 64) {
+    float x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = w[min(u0 + j * 64 + lane, t1 - 1)];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const bool in = u0 + j * 64 + lane < t1;
+      const uint32_t key = key_of(x[j]);
+      gt += __popcll(__ballot(in && key > prefix));
+      eq += __popcll(__ballot(in && key == prefix));
+    }
   }
   if (lane == 0) {
     s_gt[wave] = gt;
@@ -145,16 +156,22 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
     ties += s_eq[k];
   }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int t = t0 + lane; t - lane < t1; t += 64) {
-    const uint32_t key = t < t1 ? key_of(w[t]) : 0;
-    const bool tie = t < t1 && !none && key == prefix;
-    const uint64_t tied = __ballot(tie);
-    const bool stays = (t < t1 && !none && key > prefix) ||
-                       (tie && ties + __popcll(tied & below) < room);
-    const uint64_t all = __ballot(stays);
-    if (stays) kept[at + __popcll(all & below)] = t;
-    at += __popcll(all);
-    ties += __popcll(tied);
+  for (int u0 = t0; !none && u0 < t1; u0 += kBatch * 64) {
+    float x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = w[min(u0 + j * 64 + lane, t1 - 1)];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int t = u0 + j * 64 + lane;
+      const uint32_t key = key_of(x[j]);
+      const bool tie = t < t1 && key == prefix;
+      const uint64_t tied = __ballot(tie);
+      const bool stays = (t < t1 && key > prefix) || (tie && ties + __popcll(tied & below) < room);
+      const uint64_t all = __ballot(stays);
+      if (stays) kept[at + __popcll(all & below)] = t;
+      at += __popcll(all);
+      ties += __popcll(tied);
+    }
   }
   for (int j = tid; j < g.e.recent; j += kSelect) kept[keep - g.e.recent + j] = old + j;
 }

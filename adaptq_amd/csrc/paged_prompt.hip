@@ -14,21 +14,17 @@
 //   and P^T goes from the first product's registers into the second's as it is, if the
 //   values' tokens are taken in the order that the registers hold them: group i of four
 //   tokens in half (i & 1) of the wave.
-// * Values are transposed on their way into LDS: a lane loads 4 tokens of up to 8 channels
-//   and writes each channel's 4 tokens together.  Addresses are turned by the channel so
-//   that neither side meets in a bank.
-// * The next tokens' rows are loaded into registers while these are used, and go into the
-//   other half of LDS after: one barrier a pass.
+// * Rows of half types go from memory into LDS without passing registers, the next pass's while
+//   this one's are used (one barrier a pass), and values are transposed as they are read.  fp32
+//   rows are held in registers on the way.
 // * Tiles of few queries over many tokens are cut over the tokens, and joined by a second
 //   launch.
 //
 // Rows of half types: products of their values are exact and summed in fp32; rotated queries
-// are rounded to the type, as Rotary's are; weights are rounded to it, by up to 2^-9 (bf16)
-// and 2^-12 (fp16) of each on the average, independently, where the output itself rounds by
-// as much once: their mean over the tokens adds less than that (1.4 times the error of one
-// rounding in all; a second number for the weights' rest would cost half as much again on
-// the matrix cores).  Their sum takes them unrounded.  fp32 rows use the fp32 matrix
-// instructions.
+// are rounded to the type, as Rotary's are; weights enter as two numbers of it, 2^-16 of a
+// weight in bf16 and 2^-20 in fp16 (one number would be off by up to 2^-8 or 2^-11 each: as
+// much as the outputs' own rounding, which then came to 1.4 to 1.7 times that of fp32
+// weights).  fp32 rows use the fp32 matrix instructions.
 #include <float.h>
 
 #include <algorithm>
@@ -76,6 +72,8 @@ struct Args {
   float *partial;  // [tiles][heads][splits][kRows][DP + 2]
 };
 
+// DP: dim padded to 64, 128 or 256, as rows lie in LDS; DC: to a multiple of 32, as the products
+// take them.
 template <typename T, int DP>
 struct Kind {
   static constexpr bool kHalf = sizeof(T) == 2;
@@ -83,26 +81,20 @@ struct Kind {
   static constexpr int kSubs = kKeys / 32;
   static constexpr int kVec = 16 / (int)sizeof(T);  // values of 16 bytes
   static constexpr int kBlocks = kKeys / 16;        // blocks of 16 tokens, which lie together
-  // K: 16 bytes a lane and pass of the threads
+  // a wave loads its share of the tokens, which lies in one block of 16; 16 bytes a lane
   static constexpr int kRowLoads = DP / kVec;
-  static constexpr int kKPasses = kKeys * kRowLoads / kThreads;
-  static constexpr int kKStride = DP * sizeof(T) + 16;
-  // V, half types: 4 tokens of kVVec channels a lane
-  static constexpr int kVVec = DP / 16 < 8 ? DP / 16 : 8;
-  static constexpr int kVPasses = kHalf ? DP / (16 * kVVec) : kKPasses;
-  static constexpr int kVBytes = kHalf ? DP * kKeys * 2 : kKeys * (DP + 8) * 4;
-  static constexpr int kBuffer = kKeys * kKStride + kVBytes;
-  static constexpr int kQ = kHalf ? DP / 16 : DP / 2;  // operand registers of the queries
+  static constexpr int kPasses = kKeys * kRowLoads / kThreads;
+  static constexpr int kWaveRows = kKeys / kWaves;
+  static constexpr int kRowsAPass = 64 / kRowLoads;
+  // bytes of a row in LDS: half types whole rows, turned by the row, fp32 with room behind
+  static constexpr int kKStride = DP * sizeof(T) + (kHalf ? 0 : 16);
+  static constexpr int kVStride = DP * sizeof(T) + (kHalf ? 0 : 32);
+  static constexpr int kBuffer = kKeys * (kKStride + kVStride);
+  static constexpr int kTurns = kHalf ? (kRowsAPass < 8 ? 8 / kRowsAPass : 1) : 1;
   static constexpr int kResident = DP == 256 ? 1 : 2;
-};
-
-template <int BYTES>
-struct VecOf {
-  typedef u32x4 type;
-};
-template <>
-struct VecOf<8> {
-  typedef u32x2 type;
+  // fp16 weights are taken times 2^7 (so is their sum): small ones stay normal numbers, and with
+  // kLazy the largest stay below 2^15
+  static constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
 };
 
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c, _Float16) {
@@ -121,6 +113,60 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, _Float16) {
 __device__ __forceinline__ uint32_t pack2(float x, float y, Bf16) {
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, v2{(__bf16)x, (__bf16)y});
+}
+
+// Two weights as sums of two numbers of the type: what it holds of them, and the rest.
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, Bf16 t) {
+  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  lo = pack2(x - __uint_as_float(a & 0xFFFF0000u), y - __uint_as_float(b & 0xFFFF0000u), t);
+}
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo, _Float16 t) {
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+  const v2 h = __builtin_bit_cast(v2, hi);
+  lo = pack2(x - (float)h[0], y - (float)h[1], t);
+}
+
+// Values that are infinite or NaN: whether there are, and zeros in their place.
+template <typename T>
+__device__ __forceinline__ bool wild(uint32_t x) {
+  constexpr uint32_t top = __is_same(T, float) ? 0x7F800000u : __is_same(T, Bf16) ? 0x7F80u : 0x7C00u;
+  if (sizeof(T) == 4) return (x & top) == top;
+  return (x & top) == top || (x & top << 16) == top << 16;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t tamed(uint32_t x) {
+  if (sizeof(T) == 4) return wild<T>(x) ? 0 : x;
+  const uint32_t lo = x & 0xFFFFu, hi = x & 0xFFFF0000u;
+  return (wild<T>(lo) ? 0 : lo) | (wild<T>(hi) ? 0 : hi);
+}
+
+template <typename T>
+__device__ __forceinline__ bool wild4(u32x4 x) {
+  return wild<T>(x[0]) || wild<T>(x[1]) || wild<T>(x[2]) || wild<T>(x[3]);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 tamed4(u32x4 x) {
+  return u32x4{tamed<T>(x[0]), tamed<T>(x[1]), tamed<T>(x[2]), tamed<T>(x[3])};
+}
+
+// 16 bytes a lane of a buffer straight into LDS, in the lanes' order from `to` on; what lies
+// beyond the buffer arrives as 0.  The caller waits (vmcnt) before it reads them.
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, int off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(to), "v"(off), "s"(from)
+               : "memory", "m0");
+}
+
+// Of each 16 lanes the 4 x 16 values that they point at, a row of 16 four lanes: a column each.
+__device__ __forceinline__ u32x2 read_tr(const char *lds) {
+  typedef short v4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                 (__attribute__((address_space(3))) v4 *)(uintptr_t)(uint32_t)(uintptr_t)(
+                     __attribute__((address_space(3))) const char *)lds));
 }
 
 __device__ __forceinline__ float half_max(float x) {  // over lanes l and l ^ 32
@@ -186,11 +232,13 @@ struct Sight {
   int a, pe, w, e;
 };
 
-template <typename T, int DP, bool EXACT, bool SHAPED>
+template <typename T, int DP, int DC, bool SHAPED>
 __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_kernel(const Args g) {
   typedef Kind<T, DP> K;
   extern __shared__ __align__(16) char lds[];
   __shared__ int s_red[kWaves][8];
+  __shared__ __align__(4) uint8_t s_page[2][kWaves];  // whether a wave's tokens have a page
+  __shared__ int s_wild;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dim = g.p.dim, heads = g.p.n_heads;
@@ -238,6 +286,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     for (int i = 1; i < 6; ++i) x = lane == i ? red[i] : x;
     s_red[wave][lane] = x;
   }
+  if (tid == 0) s_wild = 0;
   __syncthreads();
   int lo = INT_MAX, pe = 0, w = INT_MAX, e = 0, w_all = 0, e_all = INT_MAX;
 #pragma unroll
@@ -274,123 +323,110 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   const int i0 = (int)((int64_t)units * split / g.splits),
             i1 = (int)((int64_t)units * (split + 1) / g.splits);
 
-  // where this thread's parts of the rows lie
+  // where this thread's parts of the rows lie.  Half types: 16 bytes c of row r lie at c ^ (r & 7)
+  // (keys) and c ^ 2 (r & 3) (values) of the row in LDS, so that the rows that are read together
+  // lie in different banks; LDS is filled in the order of the lanes, so the lane's own c is turned.
   const int *table = g.q.table + (int64_t)tile.seq * g.q.stride;
-  const int k_row = tid / K::kRowLoads, k_chunk = tid % K::kRowLoads;
-  constexpr int kKRowsAPass = kThreads / K::kRowLoads;
-  const int v_chunk = tid & 15, v_quad = tid >> 4;
-  typedef typename VecOf<K::kVVec * sizeof(T)>::type VLoad;
-  u32x4 k_in[K::kKPasses], v_in4[K::kHalf ? 1 : K::kVPasses];
-  VLoad v_in[K::kHalf ? K::kVPasses : 1][4];
+  const int wave_row = wave * K::kWaveRows;  // first of the wave's tokens of a pass
+  const int l_row = lane / K::kRowLoads, l_chunk = lane % K::kRowLoads;
+  int k_off[K::kTurns], v_off[K::kTurns];
+#pragma unroll
+  for (int i = 0; i < K::kTurns; ++i) {
+    const int row = i * K::kRowsAPass + l_row, in = (wave_row & 15) + l_row;
+    const int kc = K::kVec * (K::kHalf ? l_chunk ^ (row & 7) : l_chunk);
+    const int vc = K::kVec * (K::kHalf ? l_chunk ^ 2 * (row & 3) : l_chunk);
+    k_off[i] = kc < dim ? in * g.row_bytes + kc * (int)sizeof(T) : kBeyond;
+    v_off[i] = vc < dim ? in * g.row_bytes + vc * (int)sizeof(T) : kBeyond;
+  }
+  const uint32_t lds_at = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
+  u32x4 k_in[K::kHalf ? 1 : K::kPasses], v_in[K::kHalf ? 1 : K::kPasses];
 
-  struct Where {
-    int page[K::kBlocks], slot[K::kBlocks];
-  };
   const auto real = [&](int i) {  // unit of pass i
     const int u = u_first + i;
     return u >= gap_at ? u + gap : u;
   };
+  // the wave's tokens of pass i: their page (-1: none) and slot
+  struct Where {
+    int page, slot;
+  };
   const auto locate = [&](int i) {
-    Where x;
-    const int u = real(i);
-#pragma unroll
-    for (int k = 0; k < K::kBlocks; ++k) {
-      const int b = u * K::kBlocks + k;
-      x.page[k] = -1;
-      x.slot[k] = 0;
-      if (i < i1 && b * 16 < n) {
-        const int c = page_column(g.page_of, b);
-        const int page = ((cint *)(uint64_t)table)[c];
-        x.page[k] = page < g.p.n_pages ? page : -1;
-        x.slot[k] = (b - c * g.page_of.blocks) * 16;
-      }
+    Where x{-1, 0};
+    const int b = (real(i) * K::kKeys + wave_row) >> 4;
+    if (i < i1 && b * 16 < n) {
+      const int c = page_column(g.page_of, b);
+      const int page = ((cint *)(uint64_t)table)[c];
+      x.page = page < g.p.n_pages ? page : -1;
+      x.slot = (b - c * g.page_of.blocks) * 16;
     }
     return x;
   };
-  // 16 tokens' rows as a buffer that ends behind the last one and is empty without a page
-  const auto rows16 = [&](const void *pool, const Where &x, int k, int t0) {
-    const int64_t page = max(x.page[k], 0);
-    const char *from = static_cast<const char *>(pool) +
-                       ((page * heads + head) * g.p.page_size + x.slot[k]) * g.row_bytes;
-    const int rows = x.page[k] < 0 ? 0 : max(0, min(16, n - (t0 + 16 * k)));
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(from), 0,
-                                             __builtin_amdgcn_readfirstlane(rows * g.row_bytes),
-                                             0x00020000);
-  };
-  const auto pick = [&](const Where &x, int k) {  // block k, the same for the whole wave
-    Where y;
-    y.page[0] = x.page[0];
-    y.slot[0] = x.slot[0];
-#pragma unroll
-    for (int j = 1; j < K::kBlocks; ++j) {
-      y.page[0] = k == j ? x.page[j] : y.page[0];
-      y.slot[0] = k == j ? x.slot[j] : y.slot[0];
-    }
-    return y;
-  };
   const auto load = [&](const Where &x, int i) {
-    const int t0 = real(i) * K::kKeys;
-#pragma unroll
-    for (int p = 0; p < K::kKPasses; ++p) {
-      const int blk = __builtin_amdgcn_readfirstlane((p * kKRowsAPass + k_row) >> 4);
-      const auto from = rows16(g.p.k_pages, pick(x, blk), 0, t0 + 16 * blk);
-      const int in = (p * kKRowsAPass + k_row) & 15, c = k_chunk * K::kVec;
-      k_in[p] = __builtin_amdgcn_raw_buffer_load_b128(
-          from, EXACT || c < dim ? in * g.row_bytes + c * (int)sizeof(T) : kBeyond, 0, 0);
-      if constexpr (!K::kHalf) {
-        const auto vfrom = rows16(g.p.v_pages, pick(x, blk), 0, t0 + 16 * blk);
-        v_in4[p] = __builtin_amdgcn_raw_buffer_load_b128(
-            vfrom, EXACT || c < dim ? in * g.row_bytes + c * (int)sizeof(T) : kBeyond, 0, 0);
-      }
-    }
+    // their block's rows as a buffer that ends behind the last token, empty without a page
+    const int t0 = (real(i) * K::kKeys + wave_row) & ~15;
+    const int64_t at =
+        (((int64_t)max(x.page, 0) * heads + head) * g.p.page_size + x.slot) * g.row_bytes;
+    const int rows = x.page < 0 ? 0 : max(0, min(16, n - t0));
+    const int bytes = __builtin_amdgcn_readfirstlane(rows * g.row_bytes);
+    const auto ks = __builtin_amdgcn_make_buffer_rsrc(static_cast<char *>(g.p.k_pages) + at, 0,
+                                                      bytes, 0x00020000);
+    const auto vs = __builtin_amdgcn_make_buffer_rsrc(static_cast<char *>(g.p.v_pages) + at, 0,
+                                                      bytes, 0x00020000);
     if constexpr (K::kHalf) {
-      // the wave's 16 tokens are one block
-      const auto from = rows16(g.p.v_pages, pick(x, wave), 0, t0 + 16 * wave);
+      // straight into LDS, where the buffer of pass i is free
+      const uint32_t to = lds_at + ((i - i0) & 1) * K::kBuffer + wave_row * K::kKStride;
 #pragma unroll
-      for (int p = 0; p < K::kVPasses; ++p) {
-        const int c = (v_chunk + 16 * p) * K::kVVec;
+      for (int p = 0; p < K::kPasses; ++p) {
+        load_lds(ks, k_off[p % K::kTurns] + p * K::kRowsAPass * g.row_bytes, to + p * 1024);
+        load_lds(vs, v_off[p % K::kTurns] + p * K::kRowsAPass * g.row_bytes,
+                 to + K::kKeys * K::kKStride + p * 1024);
+      }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int off = EXACT || c < dim
-                              ? ((v_quad & 3) * 4 + j) * g.row_bytes + c * (int)sizeof(T)
-                              : kBeyond;
-          if constexpr (K::kVVec == 4)
-            v_in[p][j] = __builtin_amdgcn_raw_buffer_load_b64(from, off, 0, 0);
-          else
-            v_in[p][j] = __builtin_amdgcn_raw_buffer_load_b128(from, off, 0, 0);
-        }
+      for (int p = 0; p < K::kPasses; ++p) {
+        const int off = k_off[0] + p * K::kRowsAPass * g.row_bytes;
+        k_in[p] = __builtin_amdgcn_raw_buffer_load_b128(ks, off, 0, 0);
+        v_in[p] = __builtin_amdgcn_raw_buffer_load_b128(vs, off, 0, 0);
       }
     }
+    if (lane == 0) s_page[(i - i0) & 1][wave] = x.page >= 0;
   };
-  const auto store = [&](char *to) {
+  const auto all_seen = [&](int t0) { return t0 >= w_all && t0 + K::kKeys <= e_all; };
+  // The loads of pass i are in LDS (of this wave).  An infinity or NaN among the values of a token
+  // that some query does not see must not meet its weight of 0: zeros take its place, and at the
+  // end it is added for the queries that do see it.
+  const auto arrive = [&](int i) {
+    char *to = lds + ((i - i0) & 1) * K::kBuffer;
     char *v_to = to + K::kKeys * K::kKStride;
-#pragma unroll
-    for (int p = 0; p < K::kKPasses; ++p) {
-      *reinterpret_cast<u32x4 *>(to + (p * kKRowsAPass + k_row) * K::kKStride + k_chunk * 16) =
-          k_in[p];
-      if constexpr (!K::kHalf)
-        *reinterpret_cast<u32x4 *>(v_to + ((p * kKRowsAPass + k_row) * (DP + 8) + k_chunk * 4) * 4) =
-            v_in4[p];
-    }
+    const bool whole = all_seen(real(i) * K::kKeys);
     if constexpr (K::kHalf) {
-      const int unit = v_quad / 4 * 2 + (v_quad & 1), part = (v_quad >> 1) & 1;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (whole) return;
 #pragma unroll
-      for (int p = 0; p < K::kVPasses; ++p)
+      for (int p = 0; p < K::kPasses; ++p) {
+        u32x4 *at = reinterpret_cast<u32x4 *>(v_to + wave_row * K::kVStride + p * 1024 + lane * 16);
+        const u32x4 y = *at;
+        if (!__any(wild4<T>(y))) continue;
+        s_wild = 1;
+        *at = tamed4<T>(y);
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < K::kVVec; ++i) {
-          const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
-          u32x2 x;
-          x[0] = __builtin_amdgcn_perm(v_in[p][1][i / 2], v_in[p][0][i / 2], sel);
-          x[1] = __builtin_amdgcn_perm(v_in[p][3][i / 2], v_in[p][2][i / 2], sel);
-          const int ch = (v_chunk + 16 * p) * K::kVVec + i;
-          *reinterpret_cast<u32x2 *>(v_to + ch * 128 + ((unit ^ ((ch ^ (ch >> 3)) & 7)) << 4) +
-                                     part * 8) = x;
+      for (int p = 0; p < K::kPasses; ++p) {
+        const int row = wave_row + p * K::kRowsAPass + l_row;
+        u32x4 y = v_in[p];
+        if (!whole && __any(wild4<T>(y))) {
+          s_wild = 1;
+          y = tamed4<T>(y);
         }
+        *reinterpret_cast<u32x4 *>(to + row * K::kKStride + l_chunk * 16) = k_in[p];
+        *reinterpret_cast<u32x4 *>(v_to + row * K::kVStride + l_chunk * 16) = y;
+      }
     }
   };
 
-  Where here = locate(i0), next = locate(i0 + 1);
-  if (i0 < i1) load(here, i0);
+  const Where first_tokens = locate(i0);
+  if (!K::kHalf && i0 < i1) load(first_tokens, i0);
 
   // the queries, rotated: cosines and sines of the tile's tokens through LDS
   const RotaryTable &rt = g.p.rotary;
@@ -408,13 +444,13 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     }
     __syncthreads();
   }
-  u32x4 qh[K::kHalf ? K::kQ : 1];
-  float qf[K::kHalf ? 1 : K::kQ];
+  u32x4 qh[K::kHalf ? DC / 16 : 1];
+  float qf[K::kHalf ? 1 : DC / 2];
   {
     const float2 *cs = s_cs + (token - token0) * rt.pairs;
     constexpr int N = K::kVec, kStep = 2 * N;
 #pragma unroll
-    for (int c = 0; c < DP / kStep; ++c) {
+    for (int c = 0; c < DC / kStep; ++c) {
       const int d0 = kStep * c + N * half;
       RowVec<T, N> x;
       if (g.q_vec && d0 + N <= dim) {
@@ -451,28 +487,41 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   if (SHAPED && g.a.scores.slopes) slope2 = g.a.scores.slopes[q_head] * kLog2e;
   if (rt.pairs) __syncthreads();  // the cosines are read: LDS is the rows' now
 
-  f32x16 acc[DP / 32];
+  f32x16 acc[DC / 32];
   float m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{0};
+  for (int i = 0; i < DC / 32; ++i) acc[i] = f32x16{0};
 
-  const auto use = [&](const char *buf, const Where &x, int t0) {
+  // where this lane reads: keys 16 bytes of its row, values 4 tokens of 16 channels a group of 16
+  // lanes, 8 bytes each, which the load transposes
+  const uint32_t k_at = col * K::kKStride + ((half ^ (col & 7)) << 4);
+  const int in16 = lane & 15;
+  const uint32_t v_at0 = K::kKeys * K::kKStride + (4 * half + (in16 >> 2)) * K::kVStride +
+                         (((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ 2 * (in16 >> 2)) << 4) +
+                         8 * (lane & 1);
+
+  const auto use = [&](int buffer, int t0) {
+    const char *buf = lds + buffer * K::kBuffer;
+    const uint32_t there_are = *reinterpret_cast<const uint32_t *>(s_page[buffer]);
     const char *v_at = buf + K::kKeys * K::kKStride;
     f32x16 s[K::kSubs];
+#ifdef PRIO
+    __builtin_amdgcn_s_setprio(1);
+#endif
 #pragma unroll
     for (int i = 0; i < K::kSubs; ++i) s[i] = f32x16{0};
     if constexpr (K::kHalf) {
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c)
+      for (int c = 0; c < DC / 16; ++c)
 #pragma unroll
         for (int i = 0; i < K::kSubs; ++i) {
-          const u32x4 k = *reinterpret_cast<const u32x4 *>(buf + (32 * i + col) * K::kKStride +
-                                                           32 * c + 16 * half);
+          const u32x4 k = *reinterpret_cast<const u32x4 *>(buf + (k_at ^ (c << 5)) +
+                                                           32 * i * K::kKStride);
           s[i] = mfma(k, qh[c], s[i], T());
         }
     } else {
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
+      for (int c = 0; c < DC / 8; ++c) {
         const f32x4 k =
             *reinterpret_cast<const f32x4 *>(buf + col * K::kKStride + 32 * c + 16 * half);
 #pragma unroll
@@ -480,9 +529,11 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
           s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], qf[4 * c + i], s[0], 0, 0, 0);
       }
     }
-    bool full = t0 >= w_all && t0 + K::kKeys <= e_all;
-#pragma unroll
-    for (int k = 0; k < K::kBlocks; ++k) full = full && x.page[k] >= 0;
+#ifdef PRIO
+    __builtin_amdgcn_s_setprio(0);
+#endif
+    const uint32_t pages = __builtin_amdgcn_readfirstlane(there_are);
+    const bool full = all_seen(t0) && pages == 0x01010101u;
     const int t1 = t0 + 4 * half;
     float scale2 = g.scale2;
     if constexpr (SHAPED) {
@@ -515,7 +566,8 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int t = t1 + 32 * i + 8 * (j / 4) + j % 4;
-          const bool there = x.page[2 * i + j / 8] >= 0 &&
+          constexpr int kWavesABlock = 16 / K::kWaveRows;
+          const bool there = (pages >> 8 * ((2 * i + j / 8) * kWavesABlock) & 1) &&
                              ((t >= see.w && t < see.e) || (t >= see.a && t < see.pe));
           any = any || there;
           s[i][j] = there ? s[i][j] : -INFINITY;
@@ -536,10 +588,10 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
       const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
       l *= keep;
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) acc[i] *= keep;
+      for (int i = 0; i < DC / 32; ++i) acc[i] *= keep;
       m = to;
     }
-    const float from = fmaxf(m, -FLT_MAX);
+    const float from = fmaxf(m, -FLT_MAX) - K::kLift;
 #pragma unroll
     for (int i = 0; i < K::kSubs; ++i)
 #pragma unroll
@@ -547,52 +599,90 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
         s[i][j] = __builtin_amdgcn_exp2f(SHAPED ? s[i][j] - from : fmaf(s[i][j], scale2, -from));
         l += s[i][j];
       }
+#if PRIO == 2
+    __builtin_amdgcn_s_setprio(1);
+#endif
     if constexpr (K::kHalf) {
 #pragma unroll
       for (int k = 0; k < K::kKeys / 16; ++k) {
-        u32x4 p;
+        u32x4 p, rest;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          p[j] = pack2(s[k / 2][8 * (k % 2) + 2 * j], s[k / 2][8 * (k % 2) + 2 * j + 1], T());
+        for (int j = 0; j < 4; ++j) {
+          uint32_t hi, lo;
+          split2(s[k / 2][8 * (k % 2) + 2 * j], s[k / 2][8 * (k % 2) + 2 * j + 1], hi, lo, T());
+          p[j] = hi;
+          rest[j] = lo;
+        }
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-          const int ch = 32 * i + col;
-          const u32x4 v = *reinterpret_cast<const u32x4 *>(
-              v_at + ch * 128 + (((2 * k + half) ^ ((ch ^ (ch >> 3)) & 7)) << 4));
+        for (int i = 0; i < DC / 32; ++i) {
+          const char *from = buf + (v_at0 ^ (i << 6)) + 16 * k * K::kVStride;
+          const u32x2 v0 = read_tr(from), v1 = read_tr(from + 8 * K::kVStride);
+          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
           acc[i] = mfma(v, p, acc[i], T());
+          acc[i] = mfma(v, rest, acc[i], T());
         }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
+        for (int i = 0; i < DC / 32; ++i) {
           const float v = *reinterpret_cast<const float *>(
-              v_at + ((8 * (j / 4) + 4 * half + j % 4) * (DP + 8) + 32 * i + col) * 4);
+              v_at + (8 * (j / 4) + 4 * half + j % 4) * K::kVStride + (32 * i + col) * 4);
           acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[0][j], acc[i], 0, 0, 0);
         }
     }
+#if PRIO == 2
+    __builtin_amdgcn_s_setprio(0);
+#endif
   };
 
-  if (i0 < i1) store(lds);
-  __syncthreads();
+  Where next = locate(i0 + 1);
+  if (K::kHalf && i0 < i1) load(first_tokens, i0);
   for (int i = i0; i < i1; ++i) {
-    const Where after = locate(i + 2);
+    arrive(i);
+    __syncthreads();  // pass i is there, and the buffer of pass i - 1 free
     if (i + 1 < i1) load(next, i + 1);
+    next = locate(i + 2);
     const int t0 = real(i) * K::kKeys;
-    if (t0 < wave_e && t0 + K::kKeys > wave_lo) use(lds + ((i - i0) & 1) * K::kBuffer, here, t0);
-    if (i + 1 < i1) store(lds + ((i - i0 + 1) & 1) * K::kBuffer);
-    __syncthreads();
-    here = next;
-    next = after;
+    if (t0 < wave_e && t0 + K::kKeys > wave_lo) use((i - i0) & 1, t0);
   }
+  __syncthreads();
 
+  if (s_wild) {
+    // the tokens of the passes that not every query sees whole, one by one
+    for (int i = i0; i < i1; ++i) {
+      const int t0 = real(i) * K::kKeys;
+      if (all_seen(t0)) continue;
+      for (int t = t0; t < min(t0 + K::kKeys, n); ++t) {
+        const int c = page_column(g.page_of, t >> 4);
+        const int page = ((cint *)(uint64_t)table)[c];
+        if (page < 0 || page >= g.p.n_pages) continue;
+        const T *v = reinterpret_cast<const T *>(
+            static_cast<const char *>(g.p.v_pages) +
+            (((int64_t)page * heads + head) * g.p.page_size + (t - c * g.p.page_size)) *
+                g.row_bytes);
+        const bool there = (t >= see.w && t < see.e) || (t >= see.a && t < see.pe);
+        bool some = false;
+        for (int d = lane; d < dim; d += 64) some = some || !(fabsf(row_get(v[d])) <= FLT_MAX);
+        if (!__any(some)) continue;
+#pragma unroll
+        for (int k = 0; k < DC / 32; ++k)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int d = 32 * k + 8 * (j / 4) + 4 * half + j % 4;
+            const float x = d < dim ? row_get(v[d]) : 0.0f;
+            if (there && !(fabsf(x) <= FLT_MAX)) acc[k][j] += x;
+          }
+      }
+    }
+  }
   l = half_sum(l);
   if (!live) return;
   if (g.splits > 1) {
     float *part = g.partial + (((index * heads + head) * g.splits + split) * kRows + row) * (DP + 2);
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < DC / 32; ++i)
 #pragma unroll
       for (int j = 0; j < 16; j += 2)
         *reinterpret_cast<float2 *>(part + 32 * i + 8 * (j / 4) + 4 * half + j % 4) =
@@ -603,11 +693,11 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   T *o = reinterpret_cast<T *>(static_cast<char *>(g.a.out) + flat * (int64_t)g.a.out_nb[1] +
                                q_head * (int64_t)g.a.out_nb[0]);
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+  for (int i = 0; i < DC / 32; ++i)
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
       const int d = 32 * i + 2 * j + 4 * half;
-      if (!EXACT && d >= dim) continue;
+      if (d >= dim) continue;
       RowVec<T, 4> y;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -689,14 +779,11 @@ hipError_t over_blocks(Args &g, int64_t blocks, Launch launch) {
   return hipSuccess;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 hipError_t launch(Args &g, hipStream_t s) {
   typedef Kind<T, DP> K;
-  const bool shaped = g.a.scores.softcap > 0 || g.a.scores.slopes, exact = g.p.dim == DP;
-  const auto kernel = exact ? (shaped ? prompt_kernel<T, DP, true, true>
-                                      : prompt_kernel<T, DP, true, false>)
-                            : (shaped ? prompt_kernel<T, DP, false, true>
-                                      : prompt_kernel<T, DP, false, false>);
+  const bool shaped = g.a.scores.softcap > 0 || g.a.scores.slopes;
+  const auto kernel = shaped ? prompt_kernel<T, DP, DC, true> : prompt_kernel<T, DP, DC, false>;
   // the rows twice, or the cosines of a tile's tokens before them
   const int group = g.group, tokens = std::min(kRows, kRows / group + 2);
   const int bytes = std::max(2 * K::kBuffer, tokens * g.p.rotary.pairs * (int)sizeof(float2));
@@ -712,11 +799,12 @@ hipError_t launch(Args &g, hipStream_t s) {
 
 template <typename T>
 hipError_t launch_type(Args &g, hipStream_t s) {
-  switch (padded_dim(g.p.dim)) {
-    case 64: return launch<T, 64>(g, s);
-    case 128: return launch<T, 128>(g, s);
-    default: return launch<T, 256>(g, s);
-  }
+  const int dim = g.p.dim;
+  if (dim <= 64) return launch<T, 64, 64>(g, s);
+  if (dim <= 96) return launch<T, 128, 96>(g, s);
+  if (dim <= 128) return launch<T, 128, 128>(g, s);
+  if (dim <= 192) return launch<T, 256, 192>(g, s);
+  return launch<T, 256, 256>(g, s);
 }
 
 int64_t cap_of(const PagedShape &p, int width) {
