@@ -161,10 +161,10 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(const Args g) {
       for (int j = 0; j < kRows; ++j) {
         if (to[j] < 0) continue;
         const float scale = scale4(byte[j]);
-        RowVec<float, 4> y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y.x[i] = value4(codes[j] >> 4 * i, scale);
-        store_rows<true>(out + to[j], y);
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[j], scale, 0);
+        const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[j], scale, 1);
+        store_rows<true>(out + to[j], RowVec<float, 4>{{a[0], a[1], b[0], b[1]}});
       }
     }
   }

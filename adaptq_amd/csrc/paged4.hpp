@@ -33,28 +33,15 @@ __device__ __forceinline__ int64_t block4_at(const PagedShape &p, int page, int 
          (int64_t)(slot / 16) * block4_bytes(p.dim);
 }
 
-__device__ __forceinline__ float scale4(uint32_t byte) {
-  return __uint_as_float(byte == 255 ? 0x7FC00000u : byte << 23);
-}
+// A byte as the scale of the card's conversions: they take its exponent field alone (so what
+// lies above and below may be anything), 255 as NaN.
+__device__ __forceinline__ float scale4(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // The scale's byte for the largest magnitude's bits.
 __device__ __forceinline__ int scale4_of(uint32_t top) {
   if (top >= 0x7F800000u) return 255;
   const int e = (int)(top >> 23) - ((top & 0x7FFFFFu) > 0x400000u ? 1 : 2);  // + 127
   return min(max(e, 2), 252);
-}
-
-__device__ __forceinline__ uint32_t code4(float x, int byte) {
-  const float a = __builtin_amdgcn_ldexpf(fabsf(x), 127 - byte);
-  const int c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) +
-                (a >= 3.5f) + (a > 5.0f);
-  return c | (x < 0.0f ? 8u : 0u);
-}
-
-__device__ __forceinline__ float value4(uint32_t code, float scale) {
-  const int m = code & 7;
-  const float a = m < 2 ? 0.5f * m : __builtin_amdgcn_ldexpf(1.0f + 0.5f * (m & 1), (m >> 1) - 1);
-  return (code & 8 ? -a : a) * scale;
 }
 
 // 8 channels of a row, from channel 8 * chunk on, by a lane of four that hold its 32: their codes,
@@ -66,10 +53,12 @@ __device__ __forceinline__ uint32_t encode4(const float (&x)[8], int *byte) {
   top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
   top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
   *byte = scale4_of(top);
+  const float scale = scale4(*byte);
   uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) codes |= code4(x[i], *byte) << (4 * i);
-  return codes;
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
 }
 
 // Writes them at a token's place: `at` its block of 16, `in` its number there.

@@ -52,7 +52,11 @@ struct Rows4 {
   uint32_t ks[K::kSubs][K::kKLoads], vs[K::kSubs][K::kVChunks];  // scales: one, of 4 tokens
 };
 
-template <int DP_, bool ONCE, bool STEP, bool SHAPED_>
+// PACKED: up to 4 query heads.  Of a product's 16 columns the three numbers of a query take a
+// column each, (query head, number) in lane head + 4 * number, so that one product does what
+// three do otherwise; a score is the sum over its three columns, and so is an output at the end
+// (64 sequences x 8 heads of 8,192 tokens, 4 query heads each: XX us, unpacked XX).
+template <int DP_, bool ONCE, bool STEP, bool SHAPED_, bool PACKED>
 struct Attend4 {
   typedef Bf16 Product;
   static constexpr int DP = DP_;
@@ -62,6 +66,8 @@ struct Attend4 {
   typedef aq::Where<K::kSubs> Where;
   static constexpr int kPolicy = ONCE ? 2 : 0;
   static constexpr float kLift = 0.0f;
+  static constexpr bool kPacked = PACKED;
+  __device__ int query_row() const { return PACKED ? row16 & 3 : row16; }
 
   const Args &g;
   const int lane, row16, group4;
@@ -194,15 +200,26 @@ struct Attend4 {
 #pragma unroll
     for (int c = 0; c < K::kChunks; ++c) {
       constexpr int per = K::kKVec / 8;
-      const u32x4 q1 = q_low[64 * c], q2 = q_low[64 * (K::kChunks + c)];
+      u32x4 q1, q2;
+      if constexpr (!PACKED) {
+        q1 = q_low[64 * c];
+        q2 = q_low[64 * (K::kChunks + c)];
+      }
 #pragma unroll
       for (int i = 0; i < K::kSubs; ++i) {
         const u32x4 k = bf16_of(r.k[i][c / per][c % per], scale4(r.ks[i][c / per]));
         s[i] = mfma(k, qh[c], s[i], Bf16());
-        s[i] = mfma(k, q1, s[i], Bf16());
-        s[i] = mfma(k, q2, s[i], Bf16());
+        if constexpr (!PACKED) {
+          s[i] = mfma(k, q1, s[i], Bf16());
+          s[i] = mfma(k, q2, s[i], Bf16());
+        }
       }
     }
+    if constexpr (PACKED)
+#pragma unroll
+      for (int i = 0; i < K::kSubs; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = packed_sum(s[i][j]);
     const float scale2 = SHAPED && g.sc.softcap > 0.0f ? g.cap_in : g.scale2;
 #pragma unroll
     for (int i = 0; i < K::kSubs; ++i) s[i] *= scale2;
@@ -253,7 +270,21 @@ struct Attend4 {
           st.l += p[4 * i + j];
         }
       u32x4 pt[3];
-      split8<Bf16>(p, pt);
+      if constexpr (PACKED) {
+        const int term = row16 >> 2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float rest = p[i] - __uint_as_float(__float_as_uint(p[i]) & 0xFFFF0000u);
+          const float last = rest - __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
+          p[i] = term == 0 ? p[i] : term == 1 ? rest : term == 2 ? last : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pt[0][i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]),
+                                           0x07060302u);
+      } else {
+        split8<Bf16>(p, pt);
+      }
 #pragma unroll
       for (int c = 0; c < K::kVChunks; ++c) {
         u32x4 x[8];  // of each token, its channels
@@ -262,7 +293,9 @@ struct Attend4 {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const auto &v = r.v[2 * u + i][c];
-            const float scale = scale4(r.vs[2 * u + i][c] >> (8 * j) & 255u);
+            const uint32_t four = r.vs[2 * u + i][c];
+            // (byte j to the exponent's place)
+            const float scale = __uint_as_float(j == 3 ? four >> 1 : four << (23 - 8 * j));
             if constexpr (K::kVVec == 8) {
               x[4 * i + j] = bf16_of(v[j], scale);
             } else {  // two tokens a word
@@ -281,7 +314,7 @@ struct Attend4 {
           }
           f32x4 &y = st.acc[c * K::kVVec + 2 * w2], &z = st.acc[c * K::kVVec + 2 * w2 + 1];
 #pragma unroll
-          for (int t = 0; t < 3; ++t) {
+          for (int t = 0; t < (PACKED ? 1 : 3); ++t) {
             y = mfma(a, pt[t], y, Bf16());
             z = mfma(b, pt[t], z, Bf16());
           }
@@ -291,14 +324,20 @@ struct Attend4 {
   }
 };
 
+template <int DP, bool STEP, bool SHAPED>
+hipError_t launch4_rows(const Args &g, hipStream_t s) {
+  if (g.group <= 4) {  // (one tile of query heads: rows are read once)
+    const auto kernel = attend_kernel<Attend4<DP, true, STEP, SHAPED, true>>;
+    return launch_attend<DP, Kind4<DP>::kUnit>(g, kernel, kernel, s);
+  }
+  return launch_attend<DP, Kind4<DP>::kUnit>(
+      g, attend_kernel<Attend4<DP, true, STEP, SHAPED, false>>,
+      attend_kernel<Attend4<DP, false, STEP, SHAPED, false>>, s);
+}
+
 template <int DP, bool SHAPED>
 hipError_t launch4(const Args &g, hipStream_t s) {
-  return g.n.k ? launch_attend<DP, Kind4<DP>::kUnit>(
-                     g, attend_kernel<Attend4<DP, true, true, SHAPED>>,
-                     attend_kernel<Attend4<DP, false, true, SHAPED>>, s)
-               : launch_attend<DP, Kind4<DP>::kUnit>(
-                     g, attend_kernel<Attend4<DP, true, false, SHAPED>>,
-                     attend_kernel<Attend4<DP, false, false, SHAPED>>, s);
+  return g.n.k ? launch4_rows<DP, true, SHAPED>(g, s) : launch4_rows<DP, false, SHAPED>(g, s);
 }
 
 template <bool SHAPED>

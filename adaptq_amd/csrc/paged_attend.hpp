@@ -146,6 +146,12 @@ __device__ __forceinline__ float cross_sum(float x) {
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// Over the four lanes of 16 that are four apart, in all of them.
+__device__ __forceinline__ float packed_sum(float x) {
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 15, 15, true));
+  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 15, 15, true));
+}
+
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, _Float16) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -447,6 +453,9 @@ struct Attend {
       for (int i = 0; i < 4; ++i) o[i] = v.x[i];
     }
   }
+
+  static constexpr bool kPacked = false;
+  __device__ int query_row() const { return row16; }
 
   __device__ int k_channel(int chunk) const {  // first of the 8 (4) channels of a K load
     return K::kVec * (group4 + 4 * chunk);
@@ -771,7 +780,7 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
     // (a short segment counts for more units than it has)
     w.u_end = min(w.span.first_unit + pc.u1, w.span.units_end(K::kUnit));
     if constexpr (SHAPED) {
-      const int64_t qh = qh0 + min(w.row16, rows - 1);
+      const int64_t qh = qh0 + min(w.query_row(), rows - 1);
       if (g.sc.slopes) w.slope2 = g.sc.slopes[qh] * kLog2e;
       w.query_at = (int64_t)length + (g.a.extra - 1);
       w.score_row = g.scores && w.row16 < rows
@@ -833,11 +842,18 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[i] = s_acc[0][w.row16][w.k_channel(c) + i];
+          x[i] = s_acc[0][w.query_row()][w.k_channel(c) + i];
           if constexpr (kHalfProduct) x[i] = __builtin_amdgcn_ldexpf(x[i], -w.q_shift);
         }
         u32x4 q[K::kTerms];
         split8<typename A::Product>(x, q);
+        if constexpr (A::kPacked) {  // the lane's own number of them
+          const int term = w.row16 >> 2;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w.qh[c][i] = term == 0 ? q[0][i] : term == 1 ? q[1][i] : term == 2 ? q[2][i] : 0;
+          continue;
+        }
         w.qh[c] = q[0];
         if (c % kWaves == wave)
 #pragma unroll
@@ -872,6 +888,12 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
 
     // the waves' parts together
     st.l = cross_sum(st.l);
+    if constexpr (A::kPacked) {
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.acc[i][r] = packed_sum(st.acc[i][r]);
+    }
     if (w.row16 < rows) {
 #pragma unroll
       for (int c = 0; c < K::kVChunks; ++c)

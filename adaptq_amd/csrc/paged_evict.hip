@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kSelect = 1024;
 constexpr int kSelectWaves = kSelect / 64;
-constexpr int kBatch = 8;  // weights that a thread has under way
+constexpr int kBatch = 16;  // weights that a thread has under way
 constexpr int kMove = 256;
 constexpr int kInFlight = 8;  // rows of 16 bytes that a thread has under way
 

@@ -40,8 +40,9 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kRows = 128;  // of a tile
+constexpr int kRows = 32 * kWaves;  // of a tile
 constexpr int kBeyond = 1 << 30;
+constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
 // A maximum is followed only when it grows by more than this (in powers of two): weights
 // are then up to 2^8 of what they would be, which no sum or type minds, and most passes
 // leave the sums as they are.
@@ -90,8 +91,13 @@ struct Kind {
   static constexpr int kKStride = DP * sizeof(T) + (kHalf ? 0 : 16);
   static constexpr int kVStride = DP * sizeof(T) + (kHalf ? 0 : 32);
   static constexpr int kBuffer = kKeys * (kKStride + kVStride);
-  static constexpr int kTurns = kHalf ? (kRowsAPass < 8 ? 8 / kRowsAPass : 1) : 1;
-  static constexpr int kResident = DP == 256 ? 1 : 2;
+  // which 16 bytes of a row lie in place 0 (half types): rows that are read together, 16 of keys
+  // at one place and 4 of values at two pairs of places, lie in different banks
+  static constexpr int key_turn(int row) { return DP == 64 ? row >> 1 & 7 : row & 15; }
+  static constexpr int value_turn(int row) { return DP == 64 ? 4 * (row >> 1 & 1) : 4 * (row & 3); }
+  // waves of a SIMD: at 64 channels a third one hides more than its registers would hold (fp16,
+  // biased scores, 14 query heads on 2: 50.4 us, with two 57.5; with four, which spill, 89)
+  static constexpr int kResident = DP == 256 ? 1 : DP == 128 ? 2 : 3;
   // fp16 weights are taken times 2^7 (so is their sum): small ones stay normal numbers, and with
   // kLazy the largest stay below 2^15
   static constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
@@ -151,14 +157,22 @@ __device__ __forceinline__ u32x4 tamed4(u32x4 x) {
   return u32x4{tamed<T>(x[0]), tamed<T>(x[1]), tamed<T>(x[2]), tamed<T>(x[3])};
 }
 
-// 16 bytes a lane of a buffer straight into LDS, in the lanes' order from `to` on; what lies
-// beyond the buffer arrives as 0.  The caller waits (vmcnt) before it reads them.
-__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, int off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(to), "v"(off), "s"(from)
-               : "memory", "m0");
+// 16 bytes a lane of a buffer at each of the offsets, straight into LDS, in the lanes' order from
+// `to` on; what lies beyond the buffer arrives as 0.  The caller waits (vmcnt) before it reads
+// them.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is the compiler's, and named for that
+template <int N>
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, const int (&off)[N],
+                                         uint32_t to) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(to + 1024 * i), "v"(off[i]), "s"(from)
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Of each 16 lanes the 4 x 16 values that they point at, a row of 16 four lanes: a column each.
 __device__ __forceinline__ u32x2 read_tr(const char *lds) {
@@ -237,7 +251,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   typedef Kind<T, DP> K;
   extern __shared__ __align__(16) char lds[];
   __shared__ int s_red[kWaves][8];
-  __shared__ __align__(4) uint8_t s_page[2][kWaves];  // whether a wave's tokens have a page
+  __shared__ __align__(4) uint8_t s_page[2][4];  // whether a block of 16 tokens has a page
   __shared__ int s_wild;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -323,20 +337,19 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   const int i0 = (int)((int64_t)units * split / g.splits),
             i1 = (int)((int64_t)units * (split + 1) / g.splits);
 
-  // where this thread's parts of the rows lie.  Half types: 16 bytes c of row r lie at c ^ (r & 7)
-  // (keys) and c ^ 2 (r & 3) (values) of the row in LDS, so that the rows that are read together
-  // lie in different banks; LDS is filled in the order of the lanes, so the lane's own c is turned.
+  // where this thread's parts of the rows lie.  Half types: LDS is filled in the order of the
+  // lanes, so the lane's own part of a row is turned.
   const int *table = g.q.table + (int64_t)tile.seq * g.q.stride;
   const int wave_row = wave * K::kWaveRows;  // first of the wave's tokens of a pass
   const int l_row = lane / K::kRowLoads, l_chunk = lane % K::kRowLoads;
-  int k_off[K::kTurns], v_off[K::kTurns];
+  int k_off[K::kPasses], v_off[K::kPasses];
 #pragma unroll
-  for (int i = 0; i < K::kTurns; ++i) {
-    const int row = i * K::kRowsAPass + l_row, in = (wave_row & 15) + l_row;
-    const int kc = K::kVec * (K::kHalf ? l_chunk ^ (row & 7) : l_chunk);
-    const int vc = K::kVec * (K::kHalf ? l_chunk ^ 2 * (row & 3) : l_chunk);
-    k_off[i] = kc < dim ? in * g.row_bytes + kc * (int)sizeof(T) : kBeyond;
-    v_off[i] = vc < dim ? in * g.row_bytes + vc * (int)sizeof(T) : kBeyond;
+  for (int p = 0; p < K::kPasses; ++p) {
+    const int row = p * K::kRowsAPass + l_row, in = (wave_row & 15) + row;
+    const int kc = K::kVec * (K::kHalf ? l_chunk ^ K::key_turn(in) : l_chunk);
+    const int vc = K::kVec * (K::kHalf ? l_chunk ^ K::value_turn(in) : l_chunk);
+    k_off[p] = kc < dim ? in * g.row_bytes + kc * (int)sizeof(T) : kBeyond;
+    v_off[p] = vc < dim ? in * g.row_bytes + vc * (int)sizeof(T) : kBeyond;
   }
   const uint32_t lds_at = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
@@ -346,50 +359,49 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     const int u = u_first + i;
     return u >= gap_at ? u + gap : u;
   };
-  // the wave's tokens of pass i: their page (-1: none) and slot
-  struct Where {
-    int page, slot;
-  };
+  // Where the wave's tokens of 64 passes lie, a pass a lane: the offset of their block's rows in
+  // the pools, and how many bytes of it are there (0: no page, or no tokens).
+  uint64_t at64 = 0;
+  int bytes64 = 0;
   const auto locate = [&](int i) {
-    Where x{-1, 0};
-    const int b = (real(i) * K::kKeys + wave_row) >> 4;
-    if (i < i1 && b * 16 < n) {
+    const int b = (real(i + lane) * K::kKeys + wave_row) >> 4;
+    bytes64 = 0;
+    at64 = 0;
+    if (i + lane < i1 && b * 16 < n) {
       const int c = page_column(g.page_of, b);
-      const int page = ((cint *)(uint64_t)table)[c];
-      x.page = page < g.p.n_pages ? page : -1;
-      x.slot = (b - c * g.page_of.blocks) * 16;
+      const int page = table[c];
+      if (page >= 0 && page < g.p.n_pages) {
+        at64 = (((uint64_t)page * heads + head) * g.p.page_size + (b - c * g.page_of.blocks) * 16) *
+               (uint64_t)g.row_bytes;
+        bytes64 = min(16, n - 16 * b) * g.row_bytes;
+      }
     }
-    return x;
   };
-  const auto load = [&](const Where &x, int i) {
-    // their block's rows as a buffer that ends behind the last token, empty without a page
-    const int t0 = (real(i) * K::kKeys + wave_row) & ~15;
-    const int64_t at =
-        (((int64_t)max(x.page, 0) * heads + head) * g.p.page_size + x.slot) * g.row_bytes;
-    const int rows = x.page < 0 ? 0 : max(0, min(16, n - t0));
-    const int bytes = __builtin_amdgcn_readfirstlane(rows * g.row_bytes);
+  // A block's rows as a buffer that ends behind the last token.  Half types: straight into LDS,
+  // where the buffer of pass i is free.
+  const auto load = [&](int i) {
+    const int j = (i - i0) & 63;
+    if (j == 0 && i != i0) locate(i);
+    const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at64 >> 32), j) << 32 |
+                        (uint32_t)__builtin_amdgcn_readlane((int)at64, j);
+    const int bytes = __builtin_amdgcn_readlane(bytes64, j);
     const auto ks = __builtin_amdgcn_make_buffer_rsrc(static_cast<char *>(g.p.k_pages) + at, 0,
                                                       bytes, 0x00020000);
     const auto vs = __builtin_amdgcn_make_buffer_rsrc(static_cast<char *>(g.p.v_pages) + at, 0,
                                                       bytes, 0x00020000);
+    const int buffer = (i - i0) & 1;
     if constexpr (K::kHalf) {
-      // straight into LDS, where the buffer of pass i is free
-      const uint32_t to = lds_at + ((i - i0) & 1) * K::kBuffer + wave_row * K::kKStride;
-#pragma unroll
-      for (int p = 0; p < K::kPasses; ++p) {
-        load_lds(ks, k_off[p % K::kTurns] + p * K::kRowsAPass * g.row_bytes, to + p * 1024);
-        load_lds(vs, v_off[p % K::kTurns] + p * K::kRowsAPass * g.row_bytes,
-                 to + K::kKeys * K::kKStride + p * 1024);
-      }
+      const uint32_t to = lds_at + buffer * K::kBuffer + wave_row * K::kKStride;
+      load_lds(ks, k_off, to);
+      load_lds(vs, v_off, to + K::kKeys * K::kKStride);
     } else {
 #pragma unroll
       for (int p = 0; p < K::kPasses; ++p) {
-        const int off = k_off[0] + p * K::kRowsAPass * g.row_bytes;
-        k_in[p] = __builtin_amdgcn_raw_buffer_load_b128(ks, off, 0, 0);
-        v_in[p] = __builtin_amdgcn_raw_buffer_load_b128(vs, off, 0, 0);
+        k_in[p] = __builtin_amdgcn_raw_buffer_load_b128(ks, k_off[p], 0, 0);
+        v_in[p] = __builtin_amdgcn_raw_buffer_load_b128(vs, v_off[p], 0, 0);
       }
     }
-    if (lane == 0) s_page[(i - i0) & 1][wave] = x.page >= 0;
+    if (lane == 0 && wave_row % 16 == 0) s_page[buffer][wave_row / 16] = bytes > 0;
   };
   const auto all_seen = [&](int t0) { return t0 >= w_all && t0 + K::kKeys <= e_all; };
   // The loads of pass i are in LDS (of this wave).  An infinity or NaN among the values of a token
@@ -425,8 +437,10 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     }
   };
 
-  const Where first_tokens = locate(i0);
-  if (!K::kHalf && i0 < i1) load(first_tokens, i0);
+  // under way while the queries come; but LDS holds the cosines first
+  const bool early = !K::kHalf || g.p.rotary.pairs == 0;
+  locate(i0);
+  if (early && i0 < i1) load(i0);
 
   // the queries, rotated: cosines and sines of the tile's tokens through LDS
   const RotaryTable &rt = g.p.rotary;
@@ -449,37 +463,66 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   {
     const float2 *cs = s_cs + (token - token0) * rt.pairs;
     constexpr int N = K::kVec, kStep = 2 * N;
+    typedef RowVec<T, N> Vec;
+    const auto vec = [&](int d0) {  // channels d0 to d0 + N - 1
+      Vec x;
+      if (g.q_vec && d0 + N <= dim) return load_rows<false, T, N>(q_row + d0);
 #pragma unroll
-    for (int c = 0; c < DC / kStep; ++c) {
-      const int d0 = kStep * c + N * half;
-      RowVec<T, N> x;
-      if (g.q_vec && d0 + N <= dim) {
-        x = load_rows<false, T, N>(q_row + d0);
-      } else {
+      for (int i = 0; i < N; ++i)
+        if (d0 + i < dim) x.x[i] = q_row[d0 + i];
+        else row_put(x.x[i], 0.0f);
+      return x;
+    };
+    Vec x[DC / kStep];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (d0 + i < dim) x.x[i] = q_row[d0 + i];
-          else row_put(x.x[i], 0.0f);
+    for (int c = 0; c < DC / kStep; ++c) x[c] = vec(kStep * c + N * half);
+    if (rt.pairs && !rt.interleaved && rt.pairs % N == 0) {
+      // the pairs' other members are vectors too
+      Vec y[DC / kStep];
+#pragma unroll
+      for (int c = 0; c < DC / kStep; ++c) {
+        const int d0 = kStep * c + N * half;
+        y[c] = vec(d0 < rt.pairs ? d0 + rt.pairs : d0 < 2 * rt.pairs ? d0 - rt.pairs : d0);
       }
-      if (d0 < 2 * rt.pairs) {
+#pragma unroll
+      for (int c = 0; c < DC / kStep; ++c) {
+        const int d0 = kStep * c + N * half;
+        if (d0 >= 2 * rt.pairs) continue;
+        const bool one = d0 < rt.pairs;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int d = d0 + i;
-          if (d >= 2 * rt.pairs) break;
-          const bool one = rt.interleaved ? !(d & 1) : d < rt.pairs;
-          const int pair = rt.interleaved ? d >> 1 : one ? d : d - rt.pairs;
-          const int other = rt.interleaved ? d ^ 1 : one ? d + rt.pairs : d - rt.pairs;
-          const float u = row_get(x.x[i]), v = row_get(q_row[other]);
-          const float2 a = cs[pair];
-          row_put(x.x[i], one ? fmaf(u, a.x, -(v * a.y)) : fmaf(u, a.x, v * a.y));
+          const float u = row_get(x[c].x[i]), v = row_get(y[c].x[i]);
+          const float2 a = cs[one ? d0 + i : d0 + i - rt.pairs];
+          row_put(x[c].x[i], one ? fmaf(u, a.x, -(v * a.y)) : fmaf(u, a.x, v * a.y));
         }
       }
+    } else if (rt.pairs) {
+#pragma unroll
+      for (int c = 0; c < DC / kStep; ++c) {
+        const Vec own = x[c];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int d = kStep * c + N * half + i;
+          if (d >= 2 * rt.pairs) continue;
+          const bool one = rt.interleaved ? !(i & 1) : d < rt.pairs;
+          const int pair = rt.interleaved ? d >> 1 : one ? d : d - rt.pairs;
+          const float u = row_get(own.x[i]);
+          const float v = row_get(rt.interleaved ? own.x[i ^ 1]
+                                                 : q_row[one ? d + rt.pairs : d - rt.pairs]);
+          const float2 a = cs[pair];
+          row_put(x[c].x[i], one ? fmaf(u, a.x, -(v * a.y)) : fmaf(u, a.x, v * a.y));
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < DC / kStep; ++c) {
       if constexpr (K::kHalf) {
-        qh[c] = __builtin_bit_cast(u32x4, x);
+        qh[c] = __builtin_bit_cast(u32x4, x[c]);
         if (g.flip) qh[c] ^= 0x80008000u;
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) qf[N * c + i] = g.flip ? -row_get(x.x[i]) : row_get(x.x[i]);
+        for (int i = 0; i < N; ++i)
+          qf[N * c + i] = g.flip ? -row_get(x[c].x[i]) : row_get(x[c].x[i]);
       }
     }
   }
@@ -494,20 +537,16 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
 
   // where this lane reads: keys 16 bytes of its row, values 4 tokens of 16 channels a group of 16
   // lanes, 8 bytes each, which the load transposes
-  const uint32_t k_at = col * K::kKStride + ((half ^ (col & 7)) << 4);
+  const uint32_t k_at = col * K::kKStride + ((half ^ K::key_turn(col)) << 4);
   const int in16 = lane & 15;
   const uint32_t v_at0 = K::kKeys * K::kKStride + (4 * half + (in16 >> 2)) * K::kVStride +
-                         (((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ 2 * (in16 >> 2)) << 4) +
+                         (((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ K::value_turn(in16 >> 2))
+                          << 4) +
                          8 * (lane & 1);
 
-  const auto use = [&](int buffer, int t0) {
+  typedef f32x16 Scores[K::kSubs];
+  const auto products = [&](Scores &s, int buffer) {
     const char *buf = lds + buffer * K::kBuffer;
-    const uint32_t there_are = *reinterpret_cast<const uint32_t *>(s_page[buffer]);
-    const char *v_at = buf + K::kKeys * K::kKStride;
-    f32x16 s[K::kSubs];
-#ifdef PRIO
-    __builtin_amdgcn_s_setprio(1);
-#endif
 #pragma unroll
     for (int i = 0; i < K::kSubs; ++i) s[i] = f32x16{0};
     if constexpr (K::kHalf) {
@@ -529,11 +568,15 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
           s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], qf[4 * c + i], s[0], 0, 0, 0);
       }
     }
-#ifdef PRIO
-    __builtin_amdgcn_s_setprio(0);
-#endif
+  };
+  // What follows the products of a pass.
+  const auto weigh = [&](Scores &s, int buffer, int t0) {
+    const char *buf = lds + buffer * K::kBuffer;
+    const char *v_at = buf + K::kKeys * K::kKStride;
+    const uint32_t there_are = *reinterpret_cast<const uint32_t *>(s_page[buffer]);
     const uint32_t pages = __builtin_amdgcn_readfirstlane(there_are);
-    const bool full = all_seen(t0) && pages == 0x01010101u;
+    constexpr uint32_t kAll = K::kBlocks == 4 ? 0x01010101u : 0x0101u;
+    const bool full = all_seen(t0) && (pages & kAll) == kAll;
     const int t1 = t0 + 4 * half;
     float scale2 = g.scale2;
     if constexpr (SHAPED) {
@@ -566,8 +609,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int t = t1 + 32 * i + 8 * (j / 4) + j % 4;
-          constexpr int kWavesABlock = 16 / K::kWaveRows;
-          const bool there = (pages >> 8 * ((2 * i + j / 8) * kWavesABlock) & 1) &&
+          const bool there = (pages >> 8 * (2 * i + j / 8) & 1) &&
                              ((t >= see.w && t < see.e) || (t >= see.a && t < see.pe));
           any = any || there;
           s[i][j] = there ? s[i][j] : -INFINITY;
@@ -599,9 +641,6 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
         s[i][j] = __builtin_amdgcn_exp2f(SHAPED ? s[i][j] - from : fmaf(s[i][j], scale2, -from));
         l += s[i][j];
       }
-#if PRIO == 2
-    __builtin_amdgcn_s_setprio(1);
-#endif
     if constexpr (K::kHalf) {
 #pragma unroll
       for (int k = 0; k < K::kKeys / 16; ++k) {
@@ -632,20 +671,19 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
           acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[0][j], acc[i], 0, 0, 0);
         }
     }
-#if PRIO == 2
-    __builtin_amdgcn_s_setprio(0);
-#endif
   };
 
-  Where next = locate(i0 + 1);
-  if (K::kHalf && i0 < i1) load(first_tokens, i0);
+  if (!early && i0 < i1) load(i0);
   for (int i = i0; i < i1; ++i) {
     arrive(i);
     __syncthreads();  // pass i is there, and the buffer of pass i - 1 free
-    if (i + 1 < i1) load(next, i + 1);
-    next = locate(i + 2);
+    if (i + 1 < i1) load(i + 1);
     const int t0 = real(i) * K::kKeys;
-    if (t0 < wave_e && t0 + K::kKeys > wave_lo) use((i - i0) & 1, t0);
+    if (t0 < wave_e && t0 + K::kKeys > wave_lo) {
+      Scores s;
+      products(s, (i - i0) & 1);
+      weigh(s, (i - i0) & 1, t0);
+    }
   }
   __syncthreads();
 
@@ -728,16 +766,34 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Args g) {
     const float *part = g.partial + (at * g.splits * kRows + row) * (DP + 2);
     float m = -INFINITY, l = 0.0f;
     f32x4 y = {0, 0, 0, 0};
-    for (int k = 0; k < g.splits; ++k, part += (int64_t)kRows * (DP + 2)) {
-      const float2 ml = *reinterpret_cast<const float2 *>(part + DP);
-      if (ml.x == -INFINITY) continue;
-      const float2 a = *reinterpret_cast<const float2 *>(part + d);
-      const float2 b = *reinterpret_cast<const float2 *>(part + d + 2);
-      const float to = fmaxf(m, ml.x);
-      const float keep = __builtin_amdgcn_exp2f(m - to), e = __builtin_amdgcn_exp2f(ml.x - to);
-      l = fmaf(l, keep, e * ml.y);
-      y = y * keep + e * f32x4{a.x, a.y, b.x, b.y};
+    constexpr int64_t kPart = (int64_t)kRows * (DP + 2);
+    for (int k0 = 0; k0 < g.splits; k0 += kBatch) {
+      float2 ml[kBatch], a[kBatch], b[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {  // (the last again: no weight)
+        const float *from = part + min(k0 + k, g.splits - 1) * kPart;
+        ml[k] = *reinterpret_cast<const float2 *>(from + DP);
+        a[k] = *reinterpret_cast<const float2 *>(from + d);
+        b[k] = *reinterpret_cast<const float2 *>(from + d + 2);
+      }
+      float to = m;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (k0 + k >= g.splits) ml[k].x = -INFINITY;
+        to = fmaxf(to, ml[k].x);
+      }
+      if (to == -INFINITY) continue;
+      const float keep = __builtin_amdgcn_exp2f(m - to);
+      l *= keep;
+      y *= keep;
       m = to;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (ml[k].x == -INFINITY) continue;
+        const float e = __builtin_amdgcn_exp2f(ml[k].x - to);
+        l = fmaf(e, ml[k].y, l);
+        y += e * f32x4{a[k].x, a[k].y, b[k].x, b[k].y};
+      }
     }
     const int r = tile.r0 + row, token = r / g.group;
     T *o = reinterpret_cast<T *>(static_cast<char *>(g.a.out) +
@@ -756,14 +812,18 @@ struct Cut {
   int splits;
 };
 
-// Tiles (a bound: the offsets are on the device), and into how many pieces each is cut.
+// Tiles (a bound: the offsets are on the device), and into how many pieces each is cut: until
+// there are two blocks a CU, of fp32, where a pass takes the matrix cores sixteen times as long
+// and a piece more is cheap beside it, four (3 prompts of 1,277 tokens, 4 heads of 96, window 500:
+// 164 -> 138 us); pieces of at least four passes.
 Cut cut_of(const PagedShape &p, int q_heads, int n_tokens, int n_seqs, int64_t cap) {
-  const int group = q_heads / p.n_heads;
+  const int64_t rows = (int64_t)n_tokens * (q_heads / p.n_heads);
+  const bool half = p.io != IoType::F32;
   Cut c;
-  c.tiles = std::min((int64_t)n_tokens * group / kRows + n_seqs, (int64_t)n_tokens * group);
-  const int64_t blocks = c.tiles * p.n_heads, want = 2 * p.cus;
-  const int64_t most = std::max<int64_t>(1, cap / 256);
-  c.splits = (int)std::min(most, std::max<int64_t>(1, want / blocks));
+  c.tiles = std::min(rows / kRows + n_seqs, rows);
+  const int64_t blocks = c.tiles * p.n_heads, want = (half ? 2 : 4) * (int64_t)p.cus;
+  const int64_t most = std::max<int64_t>(1, cap / (half ? 256 : 128));
+  c.splits = (int)std::min(most, std::max<int64_t>(1, (want + (half ? 0 : blocks / 2)) / blocks));
   return c;
 }
 
@@ -785,7 +845,7 @@ hipError_t launch(Args &g, hipStream_t s) {
   const bool shaped = g.a.scores.softcap > 0 || g.a.scores.slopes;
   const auto kernel = shaped ? prompt_kernel<T, DP, DC, true> : prompt_kernel<T, DP, DC, false>;
   // the rows twice, or the cosines of a tile's tokens before them
-  const int group = g.group, tokens = std::min(kRows, kRows / group + 2);
+  const int tokens = std::min(kRows, kRows / g.group + 2);
   const int bytes = std::max(2 * K::kBuffer, tokens * g.p.rotary.pairs * (int)sizeof(float2));
   hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
