@@ -22,8 +22,10 @@ struct Args {
   bool vec;              // rows of 16 bytes' alignment
 };
 
-// A token's page, slot and position, or a page of -1: as the exact cache's append has it.
-__device__ __forceinline__ void find_token(const Args &g, int t, int *page, int *pos) {
+// Where a token lies: the byte in the pools that its block of 16 begins at for head 0, or -1, its
+// number in it, and its position; as the exact cache's append has it.
+__device__ __forceinline__ void find_token(const Args &g, int t, int64_t *at_block, int *in,
+                                           int *pos) {
   int seq = t, j = 0;
   if (g.a.offsets) {
     int lo = 0, hi = g.q.n_seqs;  // the last sequence that begins at or before t
@@ -35,7 +37,8 @@ __device__ __forceinline__ void find_token(const Args &g, int t, int *page, int 
     seq = lo;
     j = g.a.offsets[lo] <= t && t < g.a.offsets[lo + 1] ? t - g.a.offsets[lo] : -1;
   }
-  *page = -1;
+  *at_block = -1;
+  *in = 0;
   *pos = 0;
   if (j < 0 || g.q.lengths[seq] < 0) return;
   const int64_t at = (int64_t)g.q.lengths[seq] + j;
@@ -44,7 +47,10 @@ __device__ __forceinline__ void find_token(const Args &g, int t, int *page, int 
   const int col = *pos / g.p.page_size;
   if (col >= g.q.width) return;
   const int x = g.q.table[(int64_t)seq * g.q.stride + col];
-  if (x >= 0 && x < g.p.n_pages) *page = x;
+  if (x < 0 || x >= g.p.n_pages) return;
+  const int slot = *pos - col * g.p.page_size;
+  *at_block = block4_at(g.p, x, 0, slot);
+  *in = slot & 15;
 }
 
 // A block takes a few tokens of all heads; a lane 8 channels of the keys or values of a (token,
@@ -56,7 +62,8 @@ constexpr int kRows = 4;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
   __shared__ float2 s_cs[kCosSin];
-  __shared__ int s_page[kBlockTokens], s_pos[kBlockTokens];
+  __shared__ int64_t s_at[kBlockTokens];
+  __shared__ int s_in[kBlockTokens], s_pos[kBlockTokens];
   const int tid = threadIdx.x, dim = g.p.dim, tb = g.tokens_per_block;
   const int t0 = g.first_token + blockIdx.x * tb;
   const int nt = min(tb, g.a.n_tokens - t0);
@@ -93,7 +100,7 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
     }
   };
   load(row0);
-  for (int t = tid; t < nt; t += kThreads) find_token(g, t0 + t, &s_page[t], &s_pos[t]);
+  for (int t = tid; t < nt; t += kThreads) find_token(g, t0 + t, &s_at[t], &s_in[t], &s_pos[t]);
   __syncthreads();
   if (rt.pairs) {
     for (int i = tid; i < nt * rt.pairs; i += kThreads) {
@@ -103,6 +110,7 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
     __syncthreads();
   }
   char *pool = static_cast<char *>(value ? g.p.v_pages : g.p.k_pages);
+  const int head_bytes = g.p.page_size / 16 * block4_bytes(dim);
   // (the four lanes of a scale have the same rows)
   for (int r0 = row0; r0 < rows; r0 += kRows * per) {
 #pragma unroll
@@ -114,10 +122,10 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
                 [&](int pair) { return s_cs[t * rt.pairs + pair]; });
       int byte;
       const uint32_t codes = encode4(x[j], &byte);
-      if (s_page[t] < 0) continue;
-      const int slot = s_pos[t] % g.p.page_size;
-      store4(pool + block4_at(g.p, s_page[t], head[j], slot), slot & 15, chunk, codes, byte, value,
-             dim);
+      const int64_t at = s_at[t];
+      if (at < 0) continue;
+      store4(pool + at + (uint64_t)(uint32_t)head[j] * (uint32_t)head_bytes, s_in[t], chunk, codes,
+             byte, value, dim);
     }
     load(r0 + kRows * per);
   }
@@ -125,14 +133,16 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(const Args g) {
 
 // The same way back, a lane 4 channels so that a wave writes whole lines.
 __global__ __launch_bounds__(kThreads) void read4_kernel(const Args g) {
-  __shared__ int s_page[kBlockTokens], s_pos[kBlockTokens];
+  __shared__ int64_t s_at[kBlockTokens];
+  __shared__ int s_in[kBlockTokens], s_pos[kBlockTokens];
   const int tid = threadIdx.x, dim = g.p.dim, tb = g.tokens_per_block;
   const int t0 = g.first_token + blockIdx.x * tb;
   const int nt = min(tb, g.a.n_tokens - t0);
-  for (int t = tid; t < nt; t += kThreads) find_token(g, t0 + t, &s_page[t], &s_pos[t]);
+  for (int t = tid; t < nt; t += kThreads) find_token(g, t0 + t, &s_at[t], &s_in[t], &s_pos[t]);
   __syncthreads();
   const int lanes = dim / 4, rows = g.p.n_heads * tb;
   const int per = max(kThreads / (2 * lanes), 1);
+  const int head_bytes = g.p.page_size / 16 * block4_bytes(dim);
   for (int item = tid; item < per * 2 * lanes; item += kThreads) {
     const int row0 = item / (2 * lanes), c = item - row0 * 2 * lanes;
     const bool value = c >= lanes;
@@ -152,10 +162,10 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(const Args g) {
         to[j] = -1;
         if (r >= rows || t >= nt) continue;
         to[j] = ((int64_t)t * g.p.n_heads + head) * dim;
-        if (s_page[t] < 0) continue;
-        const int slot = s_pos[t] % g.p.page_size;
-        codes[j] = load4(pool + block4_at(g.p, s_page[t], head, slot), slot & 15, d, value, dim,
-                         &byte[j]);
+        const int64_t at = s_at[t];
+        if (at < 0) continue;
+        codes[j] = load4(pool + at + (uint64_t)(uint32_t)head * (uint32_t)head_bytes, s_in[t], d,
+                         value, dim, &byte[j]);
       }
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {

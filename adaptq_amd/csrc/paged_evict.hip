@@ -17,6 +17,8 @@ namespace {
 constexpr int kSelect = 1024;
 constexpr int kSelectWaves = kSelect / 64;
 constexpr int kBatch = 16;  // weights that a thread has under way
+constexpr int kAtOnce = 4;  // keys that it reads before it counts them
+constexpr int kHeld = 1 << 15;  // keys in LDS: 128 KB
 constexpr int kMove = 256;
 constexpr int kInFlight = 8;  // rows of 16 bytes that a thread has under way
 
@@ -30,6 +32,7 @@ struct Args {
   int row_bytes;
   int slices;     // in place: parts of a row that a block takes, keys and values apart
   int chunks;     // into other pages: blocks of a (sequence, key head)
+  int held;       // keys that LDS holds
   int64_t first_block;
 };
 
@@ -45,6 +48,7 @@ __device__ __forceinline__ int tokens_of(const Args &g, int seq) {
 }
 
 __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
+  extern __shared__ uint32_t s_key[];
   __shared__ int s_count[256];
   __shared__ int s_gt[kSelectWaves], s_eq[kSelectWaves];
   __shared__ uint32_t s_digit;
@@ -62,35 +66,41 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   const float *w = g.e.weights + seq * g.e.nb[1] + head * g.e.nb[0];
   const int old = n - g.e.recent;  // tokens before the newest, which stay
   int room = keep - g.e.recent;    // of those, so many stay
+  // the keys of the first kHeld tokens stay in LDS, the others' are read again
+  const int held = min(old, g.held);
+  const auto key_at = [&](int t) { return t < held ? s_key[t] : key_of(w[t]); };
+  for (int t0 = 0; room > 0 && t0 < held; t0 += kBatch * kSelect) {
+    float x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = w[min(t0 + j * kSelect + tid, held - 1)];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (t0 + j * kSelect + tid < held) s_key[t0 + j * kSelect + tid] = key_of(x[j]);
+  }
   // the key of the last one that stays, digit by digit; `room` becomes how many of that key
   uint32_t prefix = 0;
   for (int shift = 24; room > 0 && shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += kSelect) s_count[i] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < old; t0 += kBatch * kSelect) {
-      float x[kBatch];
+    for (int t0 = 0; t0 < old; t0 += kAtOnce * kSelect) {
+      uint32_t key[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) x[j] = w[min(t0 + j * kSelect + tid, old - 1)];
+      for (int j = 0; j < kAtOnce; ++j) key[j] = key_at(min(t0 + j * kSelect + tid, old - 1));
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (t0 + j * kSelect >= old) break;  // (uniform)
-        const uint32_t key = key_of(x[j]), digit = key >> shift & 255;
+      for (int j = 0; j < kAtOnce; ++j) {
         bool counts = t0 + j * kSelect + tid < old &&
-                      (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8));
-        // equal digits of a wave are counted together, two of them at the most (tokens without
-        // any weight are many, and one counter takes one lane at a time)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint64_t there = __ballot(counts);
-          if (!there) break;
-          const uint32_t of =
-              __builtin_amdgcn_readlane(digit, __ffsll((unsigned long long)there) - 1);
-          const uint64_t same = __ballot(counts && digit == of);
-          if (counts && digit == of) {
-            if (lane == __ffsll((unsigned long long)same) - 1)
-              atomicAdd(&s_count[of], __popcll(same));
-            counts = false;
-          }
+                      (shift == 24 || key[j] >> (shift + 8) == prefix >> (shift + 8));
+        // digits that equal the first lane's are counted together (tokens without any weight are
+        // many, and one counter takes one lane at a time)
+        const uint64_t there = __ballot(counts);
+        if (!there) continue;
+        const uint32_t digit = key[j] >> shift & 255;
+        const uint32_t of =
+            __builtin_amdgcn_readlane(digit, __ffsll((unsigned long long)there) - 1);
+        const uint64_t same = __ballot(counts && digit == of);
+        if (counts && digit == of) {
+          if (lane == __ffsll((unsigned long long)same) - 1) atomicAdd(&s_count[of], __popcll(same));
+          counts = false;
         }
         if (counts) atomicAdd(&s_count[digit], 1);
       }
@@ -133,17 +143,11 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   const int t0 = min(wave * per, old), t1 = min(t0 + per, old);
   const bool none = keep == g.e.recent;
   int gt = 0, eq = 0;
-  for (int u0 = t0; !none && u0 < t1; u0 += kBatch * 64) {
-    float x[kBatch];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = w[min(u0 + j * 64 + lane, t1 - 1)];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const bool in = u0 + j * 64 + lane < t1;
-      const uint32_t key = key_of(x[j]);
-      gt += __popcll(__ballot(in && key > prefix));
-      eq += __popcll(__ballot(in && key == prefix));
-    }
+  for (int u0 = t0; !none && u0 < t1; u0 += 64) {
+    const int t = u0 + lane;
+    const uint32_t key = t < t1 ? key_at(t) : 0;
+    gt += __popcll(__ballot(t < t1 && key > prefix));
+    eq += __popcll(__ballot(t < t1 && key == prefix));
   }
   if (lane == 0) {
     s_gt[wave] = gt;
@@ -156,22 +160,16 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
     ties += s_eq[k];
   }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int u0 = t0; !none && u0 < t1; u0 += kBatch * 64) {
-    float x[kBatch];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = w[min(u0 + j * 64 + lane, t1 - 1)];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int t = u0 + j * 64 + lane;
-      const uint32_t key = key_of(x[j]);
-      const bool tie = t < t1 && key == prefix;
-      const uint64_t tied = __ballot(tie);
-      const bool stays = (t < t1 && key > prefix) || (tie && ties + __popcll(tied & below) < room);
-      const uint64_t all = __ballot(stays);
-      if (stays) kept[at + __popcll(all & below)] = t;
-      at += __popcll(all);
-      ties += __popcll(tied);
-    }
+  for (int u0 = t0; !none && u0 < t1; u0 += 64) {
+    const int t = u0 + lane;
+    const uint32_t key = t < t1 ? key_at(t) : 0;
+    const bool tie = t < t1 && key == prefix;
+    const uint64_t tied = __ballot(tie);
+    const bool stays = (t < t1 && key > prefix) || (tie && ties + __popcll(tied & below) < room);
+    const uint64_t all = __ballot(stays);
+    if (stays) kept[at + __popcll(all & below)] = t;
+    at += __popcll(all);
+    ties += __popcll(tied);
   }
   for (int j = tid; j < g.e.recent; j += kSelect) kept[keep - g.e.recent + j] = old + j;
 }
@@ -334,8 +332,13 @@ hipError_t launch_paged_evict(const PagedShape &p, const PagedSeqs &q, const Pag
   g.cap = std::min((int64_t)q.width * p.page_size, (int64_t)kMaxTokens);
   g.row_bytes = p.dim * (p.io == IoType::F32 ? 4 : 2);
   const int64_t rows = (int64_t)q.n_seqs * p.n_heads;
-  hipError_t r = over_blocks(g, rows, kSelect,
-                             [&](int blocks) { select_kernel<<<blocks, kSelect, 0, s>>>(g); });
+  g.held = (int)std::min<int64_t>(g.cap, kHeld);
+  hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void *>(select_kernel),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kHeld);
+  if (r != hipSuccess) return r;
+  r = over_blocks(g, rows, kSelect, [&](int blocks) {
+    select_kernel<<<blocks, kSelect, 4 * g.held, s>>>(g);
+  });
   if (r != hipSuccess) return r;
   if (e.into) {
     g.chunks = (e.keep + kRun - 1) / kRun + 1;
