@@ -2,7 +2,7 @@
 // stay, and their rows to the front of its pages or into other pages.
 //
 // Two launches.  select_kernel finds, per (sequence, key head), the smallest weight that stays
-// by its bits from the highest on (a count of each digit's values, four times 8 bits), and
+// by its bits from the highest on (a count of each digit's values, three times), and
 // writes the indexes that stay in their order.  move_kernel copies rows by that list.  Bound:
 // the rows that stay, read and written once, and the weights.
 #include <algorithm>
@@ -17,8 +17,11 @@ namespace {
 constexpr int kSelect = 1024;
 constexpr int kSelectWaves = kSelect / 64;
 constexpr int kBatch = 16;  // weights that a thread has under way
-constexpr int kAtOnce = 4;  // keys that it reads before it counts them
+constexpr uint32_t kZero = 0x80000000u;  // the key of a weight of 0
 constexpr int kHeld = 1 << 15;  // keys in LDS: 128 KB
+// Digits of 11, 11 and 10 bits: the first holds sign, exponent and two bits more, so that even
+// weights of like size spread over many counters (a counter takes one lane at a time).
+constexpr int kBins = 1 << 11;
 constexpr int kMove = 256;
 constexpr int kInFlight = 8;  // rows of 16 bytes that a thread has under way
 
@@ -42,14 +45,17 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// 32 neighbouring digits, which one lane adds up, 64 counters apart.
+__device__ __forceinline__ int counter_of(int digit) { return (digit & 31) << 6 | digit >> 5; }
+
 __device__ __forceinline__ int tokens_of(const Args &g, int seq) {
   const int64_t n = max(g.q.lengths[seq], 0);
   return (int)min(n, g.cap);
 }
 
 __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
-  extern __shared__ uint32_t s_key[];
-  __shared__ int s_count[256];
+  extern __shared__ __align__(16) uint32_t s_key[];
+  __shared__ int s_count[kBins];  // of digit d at counter_of(d)
   __shared__ int s_gt[kSelectWaves], s_eq[kSelectWaves];
   __shared__ uint32_t s_digit;
   __shared__ int s_above;
@@ -68,7 +74,6 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   int room = keep - g.e.recent;    // of those, so many stay
   // the keys of the first kHeld tokens stay in LDS, the others' are read again
   const int held = min(old, g.held);
-  const auto key_at = [&](int t) { return t < held ? s_key[t] : key_of(w[t]); };
   for (int t0 = 0; room > 0 && t0 < held; t0 += kBatch * kSelect) {
     float x[kBatch];
 #pragma unroll
@@ -79,40 +84,42 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   }
   // the key of the last one that stays, digit by digit; `room` becomes how many of that key
   uint32_t prefix = 0;
-  for (int shift = 24; room > 0 && shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelect) s_count[i] = 0;
+  for (int top = 32; room > 0 && top > 0;) {
+    const int shift = max(top - 11, 0), bins = 1 << (top - shift);
+    const uint32_t beyond = top == 32 ? 0 : 1u << top;
+    for (int i = tid; i < kBins; i += kSelect) s_count[i] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < old; t0 += kAtOnce * kSelect) {
-      uint32_t key[kAtOnce];
+    const auto count = [&](uint32_t key, bool there) {
+      there = there && ((key ^ prefix) < beyond || beyond == 0);
+      // tokens without any weight are many, and counted together
+      const bool zero = there && key == kZero;
+      const uint64_t zeros = __ballot(zero);
+      if (zeros && lane == 0)
+        atomicAdd(&s_count[counter_of(kZero >> shift & (bins - 1))], __popcll(zeros));
+      if (there && !zero) atomicAdd(&s_count[counter_of(key >> shift & (bins - 1))], 1);
+    };
+    for (int t0 = 0; t0 < held; t0 += 4 * kSelect) {
+      const int t = t0 + 4 * tid;  // (LDS has room for whole fours)
+      const u32x4 key = *reinterpret_cast<const u32x4 *>(s_key + min(t, g.held - 4));
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) key[j] = key_at(min(t0 + j * kSelect + tid, old - 1));
+      for (int j = 0; j < 4; ++j) count(key[j], t + j < held);
+    }
+    for (int t0 = held; t0 < old; t0 += kBatch * kSelect) {
+      float x[kBatch];
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        bool counts = t0 + j * kSelect + tid < old &&
-                      (shift == 24 || key[j] >> (shift + 8) == prefix >> (shift + 8));
-        // digits that equal the first lane's are counted together (tokens without any weight are
-        // many, and one counter takes one lane at a time)
-        const uint64_t there = __ballot(counts);
-        if (!there) continue;
-        const uint32_t digit = key[j] >> shift & 255;
-        const uint32_t of =
-            __builtin_amdgcn_readlane(digit, __ffsll((unsigned long long)there) - 1);
-        const uint64_t same = __ballot(counts && digit == of);
-        if (counts && digit == of) {
-          if (lane == __ffsll((unsigned long long)same) - 1) atomicAdd(&s_count[of], __popcll(same));
-          counts = false;
-        }
-        if (counts) atomicAdd(&s_count[digit], 1);
-      }
+      for (int j = 0; j < kBatch; ++j) x[j] = w[min(t0 + j * kSelect + tid, old - 1)];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) count(key_of(x[j]), t0 + j * kSelect + tid < old);
     }
     __syncthreads();
     if (wave == 0) {  // the digit at which `room` values from the top are reached
-      int c[4], sum = 0;
+      constexpr int kEach = kBins / 64;
+      const int first = kBins - 1 - kEach * lane;  // from the largest digit on
+      int c[kEach], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = s_count[255 - (4 * lane + i)];
-        sum += c[i];
-      }
+      for (int i = 0; i < kEach; ++i) c[i] = s_count[counter_of(first - i)];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += c[i];
       int end = sum;
 #pragma unroll
       for (int k = 1; k < 64; k <<= 1) {
@@ -121,20 +128,23 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
       }
       int above = end - sum;
       if (above < room && end >= room) {
+        int digit = 0, before = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (above < room && above + c[i] >= room) {
-            s_digit = 255 - (4 * lane + i);
-            s_above = above;
-            break;
+        for (int i = 0; i < kEach; ++i) {
+          if (above < room) {  // (the last time that this holds, above + c[i] is enough)
+            digit = first - i;
+            before = above;
           }
           above += c[i];
         }
+        s_digit = digit;
+        s_above = before;
       }
     }
     __syncthreads();
     prefix |= s_digit << shift;
     room -= s_above;
+    top = shift;
     __syncthreads();
   }
   // each wave's run of the older tokens: how many stay, and of those with the last key the first
@@ -143,11 +153,23 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   const int t0 = min(wave * per, old), t1 = min(t0 + per, old);
   const bool none = keep == g.e.recent;
   int gt = 0, eq = 0;
-  for (int u0 = t0; !none && u0 < t1; u0 += 64) {
-    const int t = u0 + lane;
-    const uint32_t key = t < t1 ? key_at(t) : 0;
-    gt += __popcll(__ballot(t < t1 && key > prefix));
-    eq += __popcll(__ballot(t < t1 && key == prefix));
+  // of 4 x 64 tokens from u0 on the lane's, 64 apart
+  const auto keys_at = [&](int u0, uint32_t (&key)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = min(u0 + 64 * j + lane, t1 - 1);
+      key[j] = u0 + 256 <= held ? s_key[t] : t < held ? s_key[t] : key_of(w[t]);
+    }
+  };
+  for (int u0 = t0; !none && u0 < t1; u0 += 256) {
+    uint32_t key[4];
+    keys_at(u0, key);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = u0 + 64 * j + lane < t1;
+      gt += __popcll(__ballot(in && key[j] > prefix));
+      eq += __popcll(__ballot(in && key[j] == prefix));
+    }
   }
   if (lane == 0) {
     s_gt[wave] = gt;
@@ -160,16 +182,21 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
     ties += s_eq[k];
   }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int u0 = t0; !none && u0 < t1; u0 += 64) {
-    const int t = u0 + lane;
-    const uint32_t key = t < t1 ? key_at(t) : 0;
-    const bool tie = t < t1 && key == prefix;
-    const uint64_t tied = __ballot(tie);
-    const bool stays = (t < t1 && key > prefix) || (tie && ties + __popcll(tied & below) < room);
-    const uint64_t all = __ballot(stays);
-    if (stays) kept[at + __popcll(all & below)] = t;
-    at += __popcll(all);
-    ties += __popcll(tied);
+  for (int u0 = t0; !none && u0 < t1; u0 += 256) {
+    uint32_t key[4];
+    keys_at(u0, key);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = u0 + 64 * j + lane;
+      const bool tie = t < t1 && key[j] == prefix;
+      const uint64_t tied = __ballot(tie);
+      const bool stays =
+          (t < t1 && key[j] > prefix) || (tie && ties + __popcll(tied & below) < room);
+      const uint64_t all = __ballot(stays);
+      if (stays) kept[at + __popcll(all & below)] = t;
+      at += __popcll(all);
+      ties += __popcll(tied);
+    }
   }
   for (int j = tid; j < g.e.recent; j += kSelect) kept[keep - g.e.recent + j] = old + j;
 }
@@ -332,7 +359,7 @@ hipError_t launch_paged_evict(const PagedShape &p, const PagedSeqs &q, const Pag
   g.cap = std::min((int64_t)q.width * p.page_size, (int64_t)kMaxTokens);
   g.row_bytes = p.dim * (p.io == IoType::F32 ? 4 : 2);
   const int64_t rows = (int64_t)q.n_seqs * p.n_heads;
-  g.held = (int)std::min<int64_t>(g.cap, kHeld);
+  g.held = (int)std::max<int64_t>(4, std::min<int64_t>(g.cap, kHeld));  // (a multiple of 4)
   hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void *>(select_kernel),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kHeld);
   if (r != hipSuccess) return r;
