@@ -212,15 +212,15 @@ bool attend_ok(const Paged *p, const void *q, const void *out, int q_heads, int 
          rows_ok(p, out, "d_out", q_heads, n_seqs, nb[2], nb[3], true, fn);
 }
 
-bool scores_ok(const adaptq_scores_t *s, aq::PagedScores *to, const char *fn) {
+bool scores_ok(const adaptq_scores_t *s, float scale, aq::PagedScores *to, const char *fn) {
   *to = aq::PagedScores{};
   if (!s) return true;
   if (!(s->softcap >= 0.0f && std::isfinite(s->softcap * 1.5f))) {  // (times log2(e) in the kernel)
     set_errorf(fn, "softcap must not be negative, up to 2.2e38");
     return false;
   }
-  if (s->softcap > 0.0f && s->softcap < 0x1p-100f) {
-    set_errorf(fn, "softcap must be 0 or at least 2^-100");
+  if (s->softcap > 0.0f && (s->softcap < 0x1p-100f || !std::isfinite(scale / s->softcap))) {
+    set_errorf(fn, "softcap must be 0 or at least 2^-100, and scale / softcap finite");
     return false;
   }
   if (s->window < 0) {
@@ -454,7 +454,7 @@ int paged_scored(Paged *p, const Token &t, const aq::PagedSeqs &q, const adaptq_
   aq::PagedScores sc;
   aq::PagedWeights w;
   if (q.n_seqs < 0 || q.width < 0) return paged_token(p, t, q, nullptr, nullptr, stream, fn);
-  if (!scores_ok(scores, &sc, fn) || !weights_ok(p, d_weights, w_nb1, w_nb2, q, &w, fn)) return -1;
+  if (!scores_ok(scores, scale_of(p, t.scale), &sc, fn) || !weights_ok(p, d_weights, w_nb1, w_nb2, q, &w, fn)) return -1;
   if (w.weights) {
     if (t.q_heads <= 0 || t.q_heads % p->shape.n_heads || (long long)q.n_seqs * t.q_heads > INT_MAX)
       return paged_token(p, t, q, nullptr, nullptr, stream, fn);  // (refuses)
@@ -896,7 +896,7 @@ int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, i
   aq::PagedPrompt a{};
   if (!seqs_ok(d_table, table_width, table_stride, d_lengths, n_seqs, fn) ||
       !attend_ok(p, d_q, d_out, n_q_heads, n_tokens, nb, scale, 0, fn) ||
-      !scores_ok(scores, &a.scores, fn))
+      !scores_ok(scores, scale_of(p, scale), &a.scores, fn))
     return -1;
   if (n_tokens == 0 || n_seqs == 0) {
     aq::clear_error();

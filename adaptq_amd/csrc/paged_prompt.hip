@@ -291,9 +291,10 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   // [w, e), and what all of them see: [w_all, e_all)
   const bool pre = see.pe > see.a;
   const int wave_lo = wave_min(pre ? see.a : see.w), wave_e = wave_max(see.e);
+  const int wave_w_all = wave_max(live ? see.w : 0), wave_e_all = wave_min(live ? see.e : INT_MAX);
+  const bool wave_pre = __any(pre);
   const int red[6] = {wave_min(pre ? see.a : INT_MAX), wave_max(pre ? see.pe : 0),
-                      wave_min(see.w), wave_e, wave_max(live ? see.w : 0),
-                      wave_min(live ? see.e : INT_MAX)};
+                      wave_min(see.w), wave_e, wave_w_all, wave_e_all};
   if (lane < 6) {
     int x = red[0];
 #pragma unroll
@@ -453,8 +454,8 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     const int tokens = (tile.r0 + tile.rows - 1) / g.group - token0 + 1;
     for (int i = tid; i < tokens * rt.pairs; i += kThreads) {
       const int t = i / rt.pairs;
-      s_cs[i] = rotary_cos_sin(rt.steps[i - t * rt.pairs], length - tile.count + token0 + t,
-                               rt.amplitude);
+      s_cs[i] = rotary_cos_sin(rt.steps[i - t * rt.pairs],
+                               (int)((int64_t)length - tile.count + token0 + t), rt.amplitude);
     }
     __syncthreads();
   }
@@ -576,7 +577,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     const uint32_t there_are = *reinterpret_cast<const uint32_t *>(s_page[buffer]);
     const uint32_t pages = __builtin_amdgcn_readfirstlane(there_are);
     constexpr uint32_t kAll = K::kBlocks == 4 ? 0x01010101u : 0x0101u;
-    const bool full = all_seen(t0) && (pages & kAll) == kAll;
+    const bool full = t0 >= wave_w_all && t0 + K::kKeys <= wave_e_all && (pages & kAll) == kAll;
     const int t1 = t0 + 4 * half;
     float scale2 = g.scale2;
     if constexpr (SHAPED) {
@@ -603,14 +604,18 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     }
     float top = -INFINITY;
     if (!full) {
+      // t is in [w, e) if t - w is below e - w as a number without sign; likewise [a, pe)
       bool any = false;
+      const uint32_t in_w = t1 - see.w, in_a = t1 - see.a;
+      const uint32_t size_w = max(see.e - see.w, 0), size_a = max(see.pe - see.a, 0);
 #pragma unroll
       for (int i = 0; i < K::kSubs; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const int t = t1 + 32 * i + 8 * (j / 4) + j % 4;
-          const bool there = (pages >> 8 * (2 * i + j / 8) & 1) &&
-                             ((t >= see.w && t < see.e) || (t >= see.a && t < see.pe));
+          const int d = 32 * i + 8 * (j / 4) + j % 4;
+          bool there = in_w + d < size_w;
+          if (wave_pre) there = there || in_a + d < size_a;
+          there = there && (pages >> 8 * (2 * i + j / 8) & 1);
           any = any || there;
           s[i][j] = there ? s[i][j] : -INFINITY;
         }

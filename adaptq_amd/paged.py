@@ -1,5 +1,5 @@
-"""``PagedCache``: exact keys and values in pages that sequences share
-(adaptq_paged_* of adaptq.h).
+"""``PagedCache``: exact keys and values in pages that sequences share, and ``PagedCache4``,
+the same in 4 bits (adaptq_paged_* and adaptq_paged4_* of adaptq.h).
 
     cache = PagedCache.allocate(pages, heads=8, page_size=64, dim=128, rotary=Rotary(128))
     cache.append(k, v, table, lengths, offsets)   # prompts: rotated keys and values into pages
@@ -9,7 +9,8 @@
 Sequence b's token p lies in page ``table[b, p // page_size]``, slot ``p % page_size``;
 ``lengths[b]`` is what it holds before the call.  All tensors are on the GPU, the table,
 lengths and offsets int32; calls run on torch's current stream, allocate only their
-output, never wait, and may be captured into a graph, which the cache has to outlive.
+output (and, where prompts are short or weights are asked for, a workspace), never wait, and
+may be captured into a graph, which the cache has to outlive.
 Inference only: no gradients, and tracing (torch.jit.trace, make_fx, torch.export) is
 refused.
 Calls on one cache from different streams wait for each other (they share its workspace as
@@ -212,7 +213,8 @@ class PagedCache(_Pages):
 
         With offsets, of several: q [tokens, q_heads, dim], tokens offsets[b] to
         offsets[b + 1] - 1 the last ones of sequence b, whose lengths[b] counts them (a prompt
-        after its append); rows outside the offsets are left as ``out`` has them.
+        after its append); rows outside the offsets are left as ``out`` has them (without it
+        they hold anything).
 
         For the query at position p and token t: scores become softcap * tanh(score / softcap),
         then lose slopes[q_head] * |p - t| (float32); t is seen where first <= t and

@@ -486,7 +486,8 @@ int adaptq_paged_step_device(adaptq_paged_t cache, const void *d_k, const void *
  * window 0: all tokens up to p.  first and prefix are of the query's own, d_first and
  * d_prefix one int a query (a token of the call), NULL: 0.  So a document of a packed row
  * is seen from its first token on, a prefix is seen from both sides, and a window keeps its
- * first tokens.  A query that sees nothing gets zeros.  softcap not negative. */
+ * first tokens.  A query that sees nothing gets zeros.  softcap 0 or at least 2^-100, and
+ * scale / softcap finite. */
 typedef struct {
   float softcap;
   int window;
