@@ -368,7 +368,7 @@ __device__ __forceinline__ void shape_scores(const Args &g, f32x4 (&s)[SUBS], fl
 #pragma unroll
     for (int i = 0; i < SUBS; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = g.cap2 * tanh_of<true>(s[i][j]);
+      for (int j = 0; j < 4; ++j) s[i][j] = capped<true>(s[i][j], 1.0f, g.cap2);
   if (g.sc.slopes)
 #pragma unroll
     for (int i = 0; i < SUBS; ++i)

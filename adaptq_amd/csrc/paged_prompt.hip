@@ -587,7 +587,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
 #pragma unroll
         for (int i = 0; i < K::kSubs; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) s[i][j] = cap2 * tanh_of<!K::kHalf>(s[i][j] * cap_in);
+          for (int j = 0; j < 16; ++j) s[i][j] = capped<!K::kHalf>(s[i][j], cap_in, cap2);
       } else {
 #pragma unroll
         for (int i = 0; i < K::kSubs; ++i) s[i] *= scale2;

@@ -8,17 +8,18 @@ namespace aq {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// tanh: with u = exp(-2|z|), (1 - u) / (1 + u).  1 - u keeps 2^-24 of 1, so below 0.6 of z
-// the error would grow against the value: EXACT takes z times a polynomial of z^2 there
-// (fitted at Chebyshev points, 2^-26 of the value), 2^-22 of the value above.  Without EXACT
-// the error is 2^-23 of the cap everywhere, a thousandth of what scores of half-precision
-// rows and weights are rounded by.
+// cap * tanh(s / cap) to base 2: in is 1 / cap (of a product), cap2 the cap to base 2.  With
+// u = exp(-2|z|), tanh is (1 - u) / (1 + u).  1 - u keeps 2^-24 of 1, so below 0.6 of z the error
+// would grow against the value: EXACT takes z times a polynomial of z^2 there (fitted at
+// Chebyshev points, 2^-26 of the value), 2^-21 of the value above (the reciprocal is within one
+// step, as the exponential is).  Without EXACT the error is 2^-22 of the cap everywhere, a
+// thousandth of what scores of half-precision rows and weights are rounded by.
 template <bool EXACT>
-__device__ __forceinline__ float tanh_of(float z) {
+__device__ __forceinline__ float capped(float s, float in, float cap2) {
+  const float z = s * in;
   const float u = __builtin_amdgcn_exp2f(fabsf(z) * (-2.0f * kLog2e));
-  float y;
+  float y = copysignf((1.0f - u) * __builtin_amdgcn_rcpf(1.0f + u), z);
   if constexpr (EXACT) {
-    y = copysignf((1.0f - u) / (1.0f + u), z);
     const float z2 = z * z;
     float c = -0.0062691197f;
     c = fmaf(c, z2, 0.02111096f);
@@ -26,10 +27,8 @@ __device__ __forceinline__ float tanh_of(float z) {
     c = fmaf(c, z2, 0.13332915f);
     c = fmaf(c, z2, -0.3333333f);
     y = fabsf(z) < 0.6f ? fmaf(z * z2, c, z) : y;
-  } else {
-    y = copysignf((1.0f - u) * __builtin_amdgcn_rcpf(1.0f + u), z);
   }
-  return y;
+  return y * cap2;
 }
 
 }  // namespace aq
