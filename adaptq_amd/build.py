@@ -48,7 +48,7 @@ HIP_FLAGS = [
 ]
 
 SOURCES = ["append.hip", "decode.hip", "mirror_step.hip", "mquery.hip", "sparse.hip", "layout.hip",
-           "kbackend.hip", "rotary.hip", "paged.hip", "paged_attend.hip", "paged_shaped.hip",
+           "kbackend.hip", "rotary.hip", "paged.hip", "paged_attend.hip", "paged_shaped.hip", "paged_few.hip",
            "paged_prompt.hip", "paged_evict.hip", "paged4.hip", "paged4_attend.hip",
            "c_api.cpp", "paged_api.cpp", "vtable.cpp"]
 PROBE_SOURCES = ["probe_rows.hip", "probe_chain.hip"]

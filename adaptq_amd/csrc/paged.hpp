@@ -114,6 +114,10 @@ size_t paged_prompt_workspace(const PagedShape &p, int q_heads, int n_tokens, in
                               int table_width);
 hipError_t launch_paged_prompt(const PagedShape &p, const PagedSeqs &q, const PagedPrompt &a,
                                void *workspace, hipStream_t s);
+// The same for a few queries a sequence, without first tokens, and with a window or prefixes but
+// not both; workspace is the handle's.
+hipError_t launch_paged_few(const PagedShape &p, const PagedSeqs &q, const PagedPrompt &a,
+                            void *workspace, hipStream_t s);
 
 // Bytes of workspace an attention of this shape may need, zeroed once when it is made.
 size_t paged_workspace_bytes(const PagedShape &p);

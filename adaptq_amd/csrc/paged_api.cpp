@@ -430,6 +430,19 @@ int paged_token(Paged *p, const Token &t, const aq::PagedSeqs &q, const aq::Page
   return 0;
 }
 
+// Whether a prompt goes through the single-token kernel: its queries make one tile of 16 rows a
+// key head and sequence on the average, and it takes the masks.  One such tile costs what one
+// query does (32 sequences of up to 4,000 tokens, 8 heads, 4 queries of 4 heads each 71.5 us,
+// through a prompt's tiles 111; 8 of 8,192, fp32, 8 queries of 2, a window of 1,000 34.5 and 51;
+// one of 16,000, 4 queries of 4, 43.2 and 44.8), two read all rows twice (8 of up to 1,500, 6
+// queries of 4, 35.4 and 33.9; four tiles, 16 of up to 4,000, 87 and 63).
+constexpr int kFewRows = 16;
+bool few_queries(const Paged *p, const aq::PagedPrompt &a, int n_seqs) {
+  const long long rows = (long long)a.n_tokens * (a.q_heads / p->shape.n_heads);
+  return rows <= kFewRows * (long long)n_seqs && !a.scores.first &&
+         !(a.scores.prefix && a.scores.window > 0);
+}
+
 // Weights [n_seqs][n_heads][tokens] of a call, and the memory their scores take meanwhile.
 bool weights_ok(const Paged *p, float *w, size_t nb1, size_t nb2, const aq::PagedSeqs &q,
                 aq::PagedWeights *to, const char *fn) {
@@ -921,8 +934,10 @@ int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, i
   a.offsets = d_offsets;
   a.scale = scale_of(p, scale);
   DeviceGuard g(p->device);
-  if (hip_fail(aq::launch_paged_prompt(p->shape, q, a, d_workspace,
-                                       static_cast<hipStream_t>(stream)),
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool few = few_queries(p, a, n_seqs);
+  if (hip_fail(few ? aq::launch_paged_few(p->shape, q, a, p->ws, s)
+                   : aq::launch_paged_prompt(p->shape, q, a, d_workspace, s),
                fn))
     return -1;
   aq::clear_error();

@@ -1,5 +1,6 @@
 // paged_attend.hpp -- attention of one new token per sequence over its pages (the kernel;
-// paged_attend.hip, paged_shaped.hip and paged4_attend.hip hold its variants).
+// paged_attend.hip, paged_shaped.hip, paged_few.hip (of a few) and paged4_attend.hip hold its
+// variants).
 //
 // For the g query heads of a key head and the tokens t of [lo, n):
 //   s_t = scale <q, k_t>,  o = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),
@@ -32,6 +33,7 @@
 #pragma once
 
 #include <float.h>
+#include <limits.h>
 
 #include <algorithm>
 
@@ -83,6 +85,9 @@ struct Args {
   float *scores;    // [n_seqs][q_heads][score_stride]: to base 2, or null
   float2 *stats;    // [n_seqs][q_heads]: maximum, to base 2, and sum
   int64_t score_stride;
+  // several queries a sequence: its last offsets[b + 1] - offsets[b] tokens of n_tokens
+  const int *offsets;
+  int n_tokens;
   float *partial;
   int *counters;        // [kMaxBlocks]: parts there of the segment cut first by a block
   int *group_counters;  // [2 * kMaxBlocks]: pieces there of the group that a slot begins
@@ -337,26 +342,62 @@ struct ShapedSpan : SeenSpan {
   }
   __device__ __forceinline__ int units_end(int unit) const { return (n + unit - 1) / unit - gap; }
 };
-template <bool SHAPED>
+// Several queries a sequence: what any of them sees, and of a tile of them what all see.
+struct ManySpan : TokenSpan {
+  int first_query, queries;  // of the call's tokens
+  int w_all, e_all;
+  __device__ __forceinline__ int real(int unit) const { return unit; }
+  __device__ __forceinline__ bool all_seen(int t0, int t1) const {
+    return t0 >= w_all && t1 <= e_all;
+  }
+  __device__ __forceinline__ bool any_seen(int t0, int t1) const { return t1 > lo; }
+  __device__ __forceinline__ int units_end(int unit) const { return (n + unit - 1) / unit; }
+};
+
+constexpr int kPlain = 0, kShaped = 1, kMany = 2;  // spans
+template <int KIND>
 struct SpanOf {
   typedef Span type;
 };
 template <>
-struct SpanOf<true> {
+struct SpanOf<kShaped> {
   typedef ShapedSpan type;
 };
+template <>
+struct SpanOf<kMany> {
+  typedef ManySpan type;
+};
 
-template <bool SHAPED>
-__device__ __forceinline__ typename SpanOf<SHAPED>::type span_of(const Args &g, int seq, int length,
-                                                                 int unit) {
-  typename SpanOf<SHAPED>::type s;
-  if constexpr (SHAPED)
+__device__ __forceinline__ void queries_of(const Args &g, int seq, int *first, int *count) {
+  *first = min(max(g.offsets[seq], 0), g.n_tokens);
+  *count = min(max(g.offsets[seq + 1], *first), g.n_tokens) - *first;
+}
+
+template <int KIND>
+__device__ __forceinline__ typename SpanOf<KIND>::type span_of(const Args &g, int seq, int length,
+                                                               int unit) {
+  typename SpanOf<KIND>::type s;
+  if constexpr (KIND == kShaped) {
     static_cast<SeenSpan &>(s) =
         seen_span(length, g.a.extra, g.a.window, g.cap, unit, kMinUnits,
                   g.sc.first ? g.sc.first[seq] : 0, g.sc.prefix ? g.sc.prefix[seq] : 0);
-  else
+  } else if constexpr (KIND == kMany) {
+    queries_of(g, seq, &s.first_query, &s.queries);
+    // the window of the first query on
+    const int64_t window = g.a.window > 0 ? (int64_t)g.a.window + max(s.queries - 1, 0) : 0;
+    static_cast<TokenSpan &>(s) =
+        token_span(length, 0, window < INT_MAX ? (int)window : 0, g.cap, unit, kMinUnits);
+  } else {
     static_cast<TokenSpan &>(s) = token_span(length, g.a.extra, g.a.window, g.cap, unit, kMinUnits);
+  }
   return s;
+}
+
+// Tiles of 16 rows of a sequence and key head, a row a query head (of a query).
+template <int KIND>
+__device__ __forceinline__ int tiles_of(const Args &g, const typename SpanOf<KIND>::type &s) {
+  if constexpr (KIND == kMany) return (s.queries * g.group + kTile - 1) / kTile;
+  return g.q_tiles;
 }
 
 // Scores, to base 2 (over the cap where there is one), of tokens 16 i + j from `distance` behind
@@ -389,12 +430,15 @@ __device__ __forceinline__ void keep_scores(float *row, const f32x4 (&s)[SUBS],
 
 // DP: dim padded to 64, 128 or 256; EXACT: dim is DP; ONCE: one tile of query heads reads a row.
 // SHAPED: with scores of its own (PagedScores).
-template <typename T_, int DP_, bool EXACT, bool ONCE, bool STEP, bool SHAPED_>
+// MANY: several queries a sequence (then shaped too, without first tokens, and with a window or
+// a prefix but not both): a row of a tile is a (query, query head) and sees what its query does.
+template <typename T_, int DP_, bool EXACT, bool ONCE, bool STEP, bool SHAPED_, bool MANY = false>
 struct Attend {
   typedef T_ T;
   typedef T_ Product;  // of the products' operands
   static constexpr int DP = DP_;
   static constexpr bool kStep = STEP, SHAPED = SHAPED_;
+  static constexpr int kSpan = MANY ? kMany : SHAPED ? kShaped : kPlain;
   typedef Kind<T, DP> K;
   typedef aq::Rows<T, DP> Rows;
   typedef aq::Where<K::kSubs> Where;
@@ -407,9 +451,11 @@ struct Attend {
   const Args &g;
   const int lane, row16, group4;
   int k_off[EXACT ? 1 : K::kChunks], v_off[EXACT ? 1 : 4 * K::kVChunks];  // bytes in 16 rows
-  typename SpanOf<SHAPED>::type span;
+  typename SpanOf<kSpan>::type span;
   const int *table;
   int head, u_end;
+  int row_w = 0, row_e = 0;        // MANY: the tokens that this lane's row sees
+  bool wild_values = false;        // MANY: infinities or NaN among tokens that not all rows see
   float slope2 = 0.0f;             // of this lane's query head
   float *score_row = nullptr;      // where its scores go
   int64_t query_at = 0;            // its position
@@ -440,6 +486,13 @@ struct Attend {
 
   __device__ float query(const char *row, int d) const {
     return row_get(reinterpret_cast<const T *>(row)[d]);
+  }
+  // Several queries are rounded to the type when they are rotated, as Rotary's are.
+  __device__ float turned(float x) const {
+    if constexpr (!MANY) return x;
+    T y;
+    row_put(y, x);
+    return row_get(y);
   }
   __device__ void output(char *row, int d, f32x4 y) const {
     T *o = reinterpret_cast<T *>(row) + d;
@@ -550,7 +603,66 @@ struct Attend {
     }
   }
 
-  __device__ void use(State<DP> &st, Rows &r, const Where &w, int unit) const {
+  // MANY: an infinity or NaN of a token that some row does not see must not meet its weight of 0:
+  // zeros take its place here, and mend() adds it for the rows that do see it.
+  __device__ void tame(Rows &r) {
+    constexpr uint32_t top =
+        __is_same(T, float) ? 0x7F800000u : __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
+    constexpr bool two = sizeof(T) == 2;
+    constexpr int words = K::kVVec * (int)sizeof(T) / 4;
+    const auto wild = [&](uint32_t x) {
+      return (x & top) == top || (two && (x & top << 16) == top << 16);
+    };
+    bool some = false;
+#pragma unroll
+    for (int j = 0; j < K::kVRows; ++j)
+#pragma unroll
+      for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < words; ++i) some = some || wild(r.v[j][c][i]);
+    if (!__any(some)) return;
+    wild_values = true;
+#pragma unroll
+    for (int j = 0; j < K::kVRows; ++j)
+#pragma unroll
+      for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < words; ++i) {
+          const uint32_t x = r.v[j][c][i];
+          const uint32_t lo = two ? x & 0xFFFFu : x, hi = two ? x & 0xFFFF0000u : 0;
+          r.v[j][c][i] = ((lo & top) == top ? 0 : lo) |
+                         (two && (hi & top << 16) == top << 16 ? 0 : hi);
+        }
+  }
+  __device__ void mend(State<DP> &st, int unit) {
+    for (; unit < u_end; unit += kWaves) {
+      const int t0 = unit * K::kUnit;
+      if (span.all_seen(t0, t0 + K::kUnit)) continue;
+      for (int t = t0; t < min(t0 + K::kUnit, span.n); ++t) {
+        const int col = page_column(g.page_of, t >> 4);
+        const int page = ((cint *)(uint64_t)table)[col];
+        if (page < 0 || page >= g.p.n_pages || t < span.lo) continue;
+        const T *v = reinterpret_cast<const T *>(
+            static_cast<const char *>(g.p.v_pages) +
+            (((int64_t)page * g.p.n_heads + head) * g.p.page_size + (t - col * g.p.page_size)) *
+                g.row_bytes);
+#pragma unroll
+        for (int c = 0; c < K::kVChunks; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < K::kVVec; ++i) {
+              const int d = K::kVVec * (16 * c + 4 * group4 + k) + i;
+              const float x = d < g.p.dim ? row_get(v[d]) : 0.0f;
+              if (t >= row_w && t < row_e && !(fabsf(x) <= FLT_MAX))
+                st.acc[c * K::kVVec + i][k] += x;
+            }
+      }
+    }
+    wild_values = false;
+  }
+
+  __device__ void use(State<DP> &st, Rows &r, const Where &w, int unit) {
     const int t0 = span.real(unit) * K::kUnit;
     bool full = span.all_seen(t0, t0 + K::kUnit), any = false;
 #pragma unroll
@@ -598,7 +710,22 @@ struct Attend {
         s[i] *= scale2;
       }
     if constexpr (SHAPED) shape_scores(g, s, slope2, (float)(query_at - (t0 + 4 * group4)));
-    if (!full) {
+    bool row_any = true;  // whether this lane's row sees a token here
+    if constexpr (MANY) {
+      if (!span.all_seen(t0, t0 + K::kUnit)) tame(r);
+      if (!full) {
+        row_any = false;
+#pragma unroll
+        for (int i = 0; i < K::kSubs; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = t0 + 16 * i + 4 * group4 + j;
+            const bool there = w.page[i] >= 0 && t >= row_w && t < row_e;
+            row_any = row_any || there;
+            s[i][j] = there ? s[i][j] : -INFINITY;
+          }
+      }
+    } else if (!full) {
 #pragma unroll
       for (int i = 0; i < K::kSubs; ++i)
 #pragma unroll
@@ -611,23 +738,25 @@ struct Attend {
             for (int c = 0; c < K::kVChunks; ++c) r.v[4 * i + j][c] = typename Rows::V(0u);
         }
     }
-    if constexpr (SHAPED) keep_scores<K::kSubs>(score_row, s, w.page, t0 + 4 * group4);
-    // at least one token is here, so the maximum is finite from now on
-    float top = fmaxf(st.m, -FLT_MAX);
+    if constexpr (SHAPED && !MANY) keep_scores<K::kSubs>(score_row, s, w.page, t0 + 4 * group4);
+    // at least one token is here, so the maximum is finite from now on (MANY: where the row sees
+    // one)
+    float top = MANY ? st.m : fmaxf(st.m, -FLT_MAX);
     {
-      float x = -INFINITY;
+      float x = MANY && row_any ? -FLT_MAX : -INFINITY;
 #pragma unroll
       for (int i = 0; i < K::kSubs; ++i)
         x = fmaxf(x, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
       top = fmaxf(top, cross_max(x));
     }
     if (__any(top > st.m)) {
-      const float keep = __builtin_amdgcn_exp2f(st.m - top);
+      const float keep = MANY && top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - top);
       st.l *= keep;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) st.acc[i] *= keep;
       st.m = top;
     }
+    if constexpr (MANY) top = fmaxf(top, -FLT_MAX);
     float p[K::kUnit / 4];
 #pragma unroll
     for (int i = 0; i < K::kSubs; ++i)
@@ -676,14 +805,16 @@ struct Ends {
   int64_t end, units;
 };
 
-template <bool SHAPED>
+template <int KIND>
 __device__ __forceinline__ Ends ends_of(const Args &g, int lane, int unit, int b0) {
   const int b = b0 + lane;
   Ends e;
   e.length = g.q.lengths[min(b, g.q.n_seqs - 1)];
   e.units = 0;
-  if (b < g.q.n_seqs)
-    e.units = (int64_t)span_of<SHAPED>(g, b, e.length, unit).units * g.segs;
+  if (b < g.q.n_seqs) {
+    const auto span = span_of<KIND>(g, b, e.length, unit);
+    e.units = (int64_t)span.units * (KIND == kMany ? g.p.n_heads * tiles_of<KIND>(g, span) : g.segs);
+  }
   e.end = e.units;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
@@ -705,6 +836,8 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
   typedef typename A::K K;
   constexpr int DP = A::DP, S = DP + 4;
   constexpr bool STEP = A::kStep, SHAPED = A::SHAPED;
+  constexpr int kSpan = A::kSpan;
+  constexpr bool MANY = kSpan == kMany;
   constexpr bool kHalfProduct = __is_same(typename A::Product, _Float16);
   __shared__ __align__(16) float s_acc[kWaves][kTile][S];  // first: the queries, in [0]
   __shared__ __align__(16) u32x4 s_q[K::kHalf ? (K::kTerms - 1) * K::kChunks * 64 : 1];
@@ -715,11 +848,11 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
   const int dim = g.p.dim;
 
   // the block's share of the units, and the sequence that it begins in
-  Ends e = ends_of<SHAPED>(g, lane, K::kUnit, 0);
+  Ends e = ends_of<kSpan>(g, lane, K::kUnit, 0);
   const int n_seqs = g.q.n_seqs;
   int64_t total = uniform(e.end, min(n_seqs, 64) - 1);
   for (int b0 = 64; b0 < n_seqs; b0 += 64)
-    total += uniform(ends_of<SHAPED>(g, lane, K::kUnit, b0).end, min(n_seqs - b0, 64) - 1);
+    total += uniform(ends_of<kSpan>(g, lane, K::kUnit, b0).end, min(n_seqs - b0, 64) - 1);
   const int64_t share = share_of(total, (int)gridDim.x, kWaves);
   const int64_t start = blockIdx.x * share, end = min(start + share, total);
   if (start >= end) return;
@@ -729,7 +862,7 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
   while (!past && seq + 64 < n_seqs) {
     base += uniform(e.end, 63);
     seq += 64;
-    e = ends_of<SHAPED>(g, lane, K::kUnit, seq);
+    e = ends_of<kSpan>(g, lane, K::kUnit, seq);
     past = __ballot(base + e.end > start && seq + lane < n_seqs);
   }
   if (!past) return;  // (only if the lengths changed under the call)
@@ -748,18 +881,28 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
   const uint64_t step = turns ? rt.steps[pair] : 0;
 
   A w(g, lane, s_q);
-  int seg = -1, u0 = 0;
+  int seg = -1, u0 = 0, segs = g.segs;
   const auto next = [&](const Piece &pc) {
     at += pc.u1 - u0;
     u0 = 0;
-    if (++seg == g.segs) {
+    if (++seg == segs) {
       seg = 0;
+      if constexpr (MANY) {  // (sequences without queries have no segments)
+        int q, count;
+        while (seq + 1 < n_seqs && (queries_of(g, seq + 1, &q, &count), count == 0)) ++seq;
+      }
       if (++seq < n_seqs) length = ((cint *)(uint64_t)g.q.lengths)[seq];
       else at = end;
     }
   };
   while (at < end) {
-    w.span = span_of<SHAPED>(g, seq, length, K::kUnit);
+    w.span = span_of<kSpan>(g, seq, length, K::kUnit);
+    int q_tiles = g.q_tiles;
+    if constexpr (MANY) {
+      q_tiles = __builtin_amdgcn_readfirstlane(tiles_of<kSpan>(g, w.span));
+      segs = g.p.n_heads * q_tiles;
+      if (q_tiles == 0) break;  // (only if the offsets changed under the call)
+    }
     if (seg < 0) {
       const Start s = start_at(at, base, w.span.units);
       seg = __builtin_amdgcn_readfirstlane(s.seg);
@@ -771,15 +914,45 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
       next(pc);
       continue;
     }
-    const int head = __builtin_amdgcn_readfirstlane(seg / g.q_tiles);
-    const int q0 = (seg - head * g.q_tiles) * kTile;
-    const int rows = min(kTile, g.group - q0);
+    const int head = __builtin_amdgcn_readfirstlane(seg / q_tiles);
+    const int q0 = (seg - head * q_tiles) * kTile;
+    int rows = min(kTile, g.group - q0);
+    if constexpr (MANY) rows = min(kTile, w.span.queries * g.group - q0);
     const int64_t qh0 = (int64_t)head * g.group + q0;
+    // a row's place among the call's queries, and MANY: which of the sequence's it is
+    struct Place {
+      int64_t token, q_head;
+      int number;
+    };
+    const auto place = [&](int row) {
+      if constexpr (MANY) {
+        const int number = (q0 + row) / g.group;
+        return Place{w.span.first_query + number,
+                     (int64_t)head * g.group + (q0 + row - number * g.group), number};
+      } else {
+        return Place{seq, qh0 + row, 0};
+      }
+    };
     w.head = head;
     w.table = g.q.table + (int64_t)seq * g.q.stride;
     // (a short segment counts for more units than it has)
     w.u_end = min(w.span.first_unit + pc.u1, w.span.units_end(K::kUnit));
-    if constexpr (SHAPED) {
+    if constexpr (MANY) {
+      const auto own = place(min(w.row16, rows - 1));
+      const int64_t at0 = (int64_t)length - w.span.queries;  // position of the first query
+      w.query_at = at0 + own.number;
+      if (g.sc.slopes) w.slope2 = g.sc.slopes[own.q_head] * kLog2e;
+      const int pre = g.sc.prefix ? g.sc.prefix[own.token] : 0;
+      const int64_t back = g.a.window > 0 ? w.query_at - g.a.window + 1 : 0;
+      w.row_w = (int)max(back, (int64_t)0);
+      w.row_e = max((int)min(max(w.query_at + 1, (int64_t)0), (int64_t)w.span.n),
+                    min(pre, w.span.n));
+      const int64_t last = at0 + place(rows - 1).number - g.a.window + 1;
+      w.span.w_all =
+          __builtin_amdgcn_readfirstlane(g.a.window > 0 ? (int)max(last, (int64_t)0) : 0);
+      w.span.e_all = __builtin_amdgcn_readfirstlane(
+          (int)min(max(at0 + place(0).number + 1, (int64_t)0), (int64_t)w.span.n));
+    } else if constexpr (SHAPED) {
       const int64_t qh = qh0 + min(w.query_row(), rows - 1);
       if (g.sc.slopes) w.slope2 = g.sc.slopes[qh] * kLog2e;
       w.query_at = (int64_t)length + (g.a.extra - 1);
@@ -793,7 +966,7 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
       // the token goes into its page by the wave whose units hold it
       int last = length / K::kUnit, off = last - (w.span.first_unit + u0);
       bool mine = last < w.u_end && off >= 0 && off % kWaves == wave;
-      if constexpr (SHAPED) {
+      if constexpr (SHAPED && !MANY) {
         last -= w.span.gap;
         off -= w.span.gap;
         mine = last < w.u_end && off >= 0 && off % kWaves == wave;
@@ -813,12 +986,21 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
                        qh0 * (int64_t)g.a.q_nb[0];
     {
       float2 cs = make_float2(1.0f, 0.0f);
-      if (turns) cs = rotary_cos_sin(step, length < 0 ? 0 : length + (g.a.extra - 1), rt.amplitude);
+      if (turns && !MANY)
+        cs = rotary_cos_sin(step, length < 0 ? 0 : length + (g.a.extra - 1), rt.amplitude);
       for (int row = tid / (DP / 2); row < rows; row += 2 * kThreads / DP) {
         const char *q = q_at + row * (int64_t)g.a.q_nb[0];
+        if constexpr (MANY) {
+          const auto own = place(row);
+          q = static_cast<const char *>(g.a.q) + own.token * (int64_t)g.a.q_nb[1] +
+              own.q_head * (int64_t)g.a.q_nb[0];
+          if (turns)
+            cs = rotary_cos_sin(step, (int)((int64_t)length - w.span.queries + own.number),
+                                rt.amplitude);
+        }
         const float x = c0 < dim ? w.query(q, c0) : 0.0f, y = c1 < dim ? w.query(q, c1) : 0.0f;
-        s_acc[0][row][c0] = turns ? fmaf(x, cs.x, -(y * cs.y)) : x;
-        s_acc[0][row][c1] = turns ? fmaf(y, cs.x, x * cs.y) : y;
+        s_acc[0][row][c0] = turns ? w.turned(fmaf(x, cs.x, -(y * cs.y))) : x;
+        s_acc[0][row][c1] = turns ? w.turned(fmaf(y, cs.x, x * cs.y)) : y;
       }
     }
     __syncthreads();
@@ -886,6 +1068,9 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
       w1 = next;
     }
 
+    if constexpr (MANY)
+      if (w.wild_values) w.mend(st, w.span.first_unit + u0 + wave);
+
     // the waves' parts together
     st.l = cross_sum(st.l);
     if constexpr (A::kPacked) {
@@ -918,7 +1103,14 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
               make_float2(m, __builtin_amdgcn_ldexpf(l, -(int)A::kLift));
       if (d >= dim) return;
       y = m == -INFINITY ? f32x4{0, 0, 0, 0} : y / l;  // no tokens: zeros
-      w.output(o_at + (qh0 + row) * (int64_t)g.a.out_nb[0], d, y);
+      if constexpr (MANY) {
+        const auto own = place(row);
+        w.output(static_cast<char *>(g.a.out) + own.token * (int64_t)g.a.out_nb[1] +
+                     own.q_head * (int64_t)g.a.out_nb[0],
+                 d, y);
+      } else {
+        w.output(o_at + (qh0 + row) * (int64_t)g.a.out_nb[0], d, y);
+      }
     };
     constexpr int kPart = part_floats(DP);
     int slot = 2 * blockIdx.x + pc.slot;  // where this block's part of a cut segment goes

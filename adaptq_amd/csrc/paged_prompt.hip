@@ -95,8 +95,9 @@ struct Kind {
   // at one place and 4 of values at two pairs of places, lie in different banks
   static constexpr int key_turn(int row) { return DP == 64 ? row >> 1 & 7 : row & 15; }
   static constexpr int value_turn(int row) { return DP == 64 ? 4 * (row >> 1 & 1) : 4 * (row & 3); }
-  // waves of a SIMD: at 64 channels a third one hides more than its registers would hold (fp16,
-  // biased scores, 14 query heads on 2: 50.4 us, with two 57.5; with four, which spill, 89)
+  // waves of a SIMD: at 64 channels there is room for three, which hide each other's exponentials
+  // (2 prompts of 4,096, bf16, 16 query heads on 4, capped: 377 us, with two 391; as they are or
+  // biased the same within 1; packed documents, fp16, 42.6, with four, which spill, 54)
   static constexpr int kResident = DP == 256 ? 1 : DP == 128 ? 2 : 3;
   // fp16 weights are taken times 2^7 (so is their sum): small ones stay normal numbers, and with
   // kLazy the largest stay below 2^15
@@ -820,7 +821,7 @@ struct Cut {
 // Tiles (a bound: the offsets are on the device), and into how many pieces each is cut: until
 // there are two blocks a CU, of fp32, where a pass takes the matrix cores sixteen times as long
 // and a piece more is cheap beside it, four (3 prompts of 1,277 tokens, 4 heads of 96, window 500:
-// 164 -> 138 us); pieces of at least four passes.
+// 140 -> 132 us); pieces of at least four passes.
 Cut cut_of(const PagedShape &p, int q_heads, int n_tokens, int n_seqs, int64_t cap) {
   const int64_t rows = (int64_t)n_tokens * (q_heads / p.n_heads);
   const bool half = p.io != IoType::F32;

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(const WeightArgs x) {
   const int chunk = (int)(block % x.chunks);
   const int64_t rest = block / x.chunks;
   const int head = (int)(rest % g.p.n_heads), seq = (int)(rest / g.p.n_heads);
-  const ShapedSpan span = span_of<true>(g, seq, g.q.lengths[seq], 16);
+  const ShapedSpan span = span_of<kShaped>(g, seq, g.q.lengths[seq], 16);
   const int t = chunk * kChunk + 4 * (int)threadIdx.x;
   if (t >= span.n || t + 4 <= span.lo) return;
   const int col = page_column(g.page_of, t >> 4);

@@ -499,8 +499,8 @@ typedef struct {
  * tokens d_offsets[b] to d_offsets[b + 1] - 1 are the last ones of sequence b, whose
  * d_lengths[b] counts them (append them first).  Tokens outside the offsets are left as they
  * were.  Query heads, pages and d_out as in attend; scores NULL: every token up to its own.
- * Half types: rotated queries and the softmax's weights are rounded to the type before
- * the products, the rest is fp32.  n_tokens * n_q_heads up to 2^31 - 1.  d_workspace:
+ * Half types: rotated queries are rounded to the type before the products, the softmax's
+ * weights enter as two numbers of it or more, the rest is fp32.  n_tokens * n_q_heads up to 2^31 - 1.  d_workspace:
  * device memory of adaptq_paged_prompt_workspace bytes (0 for many tokens), 16-byte
  * aligned, this call's alone until it is done.  Returns 0/-1. */
 size_t adaptq_paged_prompt_workspace(adaptq_paged_t cache, int n_q_heads, int n_tokens,
