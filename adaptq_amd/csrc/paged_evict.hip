@@ -16,12 +16,17 @@ namespace {
 
 constexpr int kSelect = 1024;
 constexpr int kSelectWaves = kSelect / 64;
-constexpr int kBatch = 16;  // weights that a thread has under way
 constexpr uint32_t kZero = 0x80000000u;  // the key of a weight of 0
-constexpr int kHeld = 1 << 15;  // keys in LDS: 128 KB
+// Weights that a thread holds: those of so many tokens are read once, longer sequences' in
+// stretches of as many, for each of the three digits and for the list (32,768 tokens, 8 heads,
+// both launches: 56 us; from LDS, and one counter a digit, 65).
+constexpr int kHeld = 32;
+constexpr int kStretch = kHeld * kSelect;
 // Digits of 11, 11 and 10 bits: the first holds sign, exponent and two bits more, so that even
-// weights of like size spread over many counters (a counter takes one lane at a time).
+// weights of like size spread over many counters.  A counter takes one lane at a time, so there
+// are some of each digit, side by side.
 constexpr int kBins = 1 << 11;
+constexpr int kCopies = 4;
 constexpr int kMove = 256;
 constexpr int kInFlight = 8;  // rows of 16 bytes that a thread has under way
 
@@ -35,7 +40,6 @@ struct Args {
   int row_bytes;
   int slices;     // in place: parts of a row that a block takes, keys and values apart
   int chunks;     // into other pages: blocks of a (sequence, key head)
-  int held;       // keys that LDS holds
   int64_t first_block;
 };
 
@@ -45,17 +49,13 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// 32 neighbouring digits, which one lane adds up, 64 counters apart.
-__device__ __forceinline__ int counter_of(int digit) { return (digit & 31) << 6 | digit >> 5; }
-
 __device__ __forceinline__ int tokens_of(const Args &g, int seq) {
   const int64_t n = max(g.q.lengths[seq], 0);
   return (int)min(n, g.cap);
 }
 
 __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
-  extern __shared__ __align__(16) uint32_t s_key[];
-  __shared__ int s_count[kBins];  // of digit d at counter_of(d)
+  __shared__ __align__(16) int s_count[kBins * kCopies];
   __shared__ int s_gt[kSelectWaves], s_eq[kSelectWaves];
   __shared__ uint32_t s_digit;
   __shared__ int s_above;
@@ -72,131 +72,129 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   const float *w = g.e.weights + seq * g.e.nb[1] + head * g.e.nb[0];
   const int old = n - g.e.recent;  // tokens before the newest, which stay
   int room = keep - g.e.recent;    // of those, so many stay
-  // the keys of the first kHeld tokens stay in LDS, the others' are read again
-  const int held = min(old, g.held);
-  for (int t0 = 0; room > 0 && t0 < held; t0 += kBatch * kSelect) {
-    float x[kBatch];
+  // The keys of a stretch: each wave a run of its tokens, 64 neighbours a step.
+  uint32_t key[kHeld];
+  int t0 = 0, count = 0, steps = 0;  // the run, the same `steps` for all waves
+  const auto hold = [&](int64_t from) {
+    const int m = (int)min((int64_t)kStretch, old - from);
+    const int per = ((m + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
+    steps = per / 64;
+    t0 = (int)min(from + wave * per, (int64_t)old - 1);
+    count = min(max(m - wave * per, 0), per);
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = w[min(t0 + j * kSelect + tid, held - 1)];
+    for (int j0 = 0; j0 < kHeld; j0 += 8) {
+      if (j0 >= steps) break;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (t0 + j * kSelect + tid < held) s_key[t0 + j * kSelect + tid] = key_of(x[j]);
-  }
+      for (int j = j0; j < j0 + 8; ++j)
+        key[j] = __float_as_uint(w[min((int64_t)t0 + 64 * j + lane, (int64_t)old - 1)]);
+    }
+#pragma unroll
+    for (int j0 = 0; j0 < kHeld; j0 += 8) {
+      if (j0 >= steps) break;
+#pragma unroll
+      for (int j = j0; j < j0 + 8; ++j) key[j] = key_of(__uint_as_float(key[j]));
+    }
+  };
+  const auto each_key = [&](auto use) {  // use(key, step, whether the lane has one)
+#pragma unroll
+    for (int j0 = 0; j0 < kHeld; j0 += 4) {
+      if (j0 >= steps) break;
+#pragma unroll
+      for (int j = j0; j < j0 + 4; ++j) use(key[j], j, 64 * j + lane < count);
+    }
+  };
+  const bool once = old <= kStretch;
+  if (room > 0 && once) hold(0);
   // the key of the last one that stays, digit by digit; `room` becomes how many of that key
+  const bool none = room <= 0;
   uint32_t prefix = 0;
-  for (int top = 32; room > 0 && top > 0;) {
+  for (int top = 32; !none && top > 0;) {
     const int shift = max(top - 11, 0), bins = 1 << (top - shift);
     const uint32_t beyond = top == 32 ? 0 : 1u << top;
-    for (int i = tid; i < kBins; i += kSelect) s_count[i] = 0;
+    for (int i = 4 * tid; i < kBins * kCopies; i += 4 * kSelect)
+      *reinterpret_cast<u32x4 *>(s_count + i) = u32x4{0, 0, 0, 0};
     __syncthreads();
-    const auto count = [&](uint32_t key, bool there) {
-      there = there && ((key ^ prefix) < beyond || beyond == 0);
-      // tokens without any weight are many, and counted together
-      const bool zero = there && key == kZero;
-      const uint64_t zeros = __ballot(zero);
-      if (zeros && lane == 0)
-        atomicAdd(&s_count[counter_of(kZero >> shift & (bins - 1))], __popcll(zeros));
-      if (there && !zero) atomicAdd(&s_count[counter_of(key >> shift & (bins - 1))], 1);
-    };
-    for (int t0 = 0; t0 < held; t0 += 4 * kSelect) {
-      const int t = t0 + 4 * tid;  // (LDS has room for whole fours)
-      const u32x4 key = *reinterpret_cast<const u32x4 *>(s_key + min(t, g.held - 4));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) count(key[j], t + j < held);
-    }
-    for (int t0 = held; t0 < old; t0 += kBatch * kSelect) {
-      float x[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) x[j] = w[min(t0 + j * kSelect + tid, old - 1)];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) count(key_of(x[j]), t0 + j * kSelect + tid < old);
+    for (int64_t from = 0; from < old; from += kStretch) {
+      if (!once) hold(from);
+      each_key([&](uint32_t k, int, bool there) {
+        there = there && ((k ^ prefix) < beyond || beyond == 0);
+        if (!__any(there)) return;
+        // tokens without any weight are many, and counted together
+        const bool zero = there && k == kZero;
+        const uint64_t zeros = __ballot(zero);
+        if (zeros && lane == 0)
+          atomicAdd(&s_count[(kZero >> shift & (bins - 1)) * kCopies], __popcll(zeros));
+        if (there && !zero)
+          atomicAdd(&s_count[(k >> shift & (bins - 1)) * kCopies + lane % kCopies], 1);
+      });
     }
     __syncthreads();
-    if (wave == 0) {  // the digit at which `room` values from the top are reached
-      constexpr int kEach = kBins / 64;
-      const int first = kBins - 1 - kEach * lane;  // from the largest digit on
-      int c[kEach], sum = 0;
+    // the digit at which `room` values from the top are reached: two digits a thread, the
+    // largest first
+    static_assert(kBins == 2 * kSelect, "two digits a thread");
+    const int digit = kBins - 1 - 2 * tid;
+    int c[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) c[i] = s_count[counter_of(first - i)];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) sum += c[i];
-      int end = sum;
+      for (int k = 0; k < kCopies; ++k) c[i] += s_count[(digit - i) * kCopies + k];
+    const int sum = c[0] + c[1];
+    int end = sum;
 #pragma unroll
-      for (int k = 1; k < 64; k <<= 1) {
-        const int y = __shfl_up(end, k, 64);
-        if (lane >= k) end += y;
-      }
-      int above = end - sum;
-      if (above < room && end >= room) {
-        int digit = 0, before = 0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          if (above < room) {  // (the last time that this holds, above + c[i] is enough)
-            digit = first - i;
-            before = above;
-          }
-          above += c[i];
-        }
-        s_digit = digit;
-        s_above = before;
-      }
+    for (int k = 1; k < 64; k <<= 1) {
+      const int y = __shfl_up(end, k, 64);
+      if (lane >= k) end += y;
+    }
+    if (lane == 63) s_gt[wave] = end;
+    __syncthreads();
+    int above = end - sum;
+    for (int k = 0; k < wave; ++k) above += s_gt[k];
+    if (above < room && above + sum >= room) {
+      const bool second = above + c[0] < room;
+      s_digit = digit - second;
+      s_above = above + (second ? c[0] : 0);
     }
     __syncthreads();
     prefix |= s_digit << shift;
     room -= s_above;
     top = shift;
-    __syncthreads();
   }
   // each wave's run of the older tokens: how many stay, and of those with the last key the first
   // `room`; then the indexes in order
-  const int per = ((old + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
-  const int t0 = min(wave * per, old), t1 = min(t0 + per, old);
-  const bool none = keep == g.e.recent;
-  int gt = 0, eq = 0;
-  // of 4 x 64 tokens from u0 on the lane's, 64 apart
-  const auto keys_at = [&](int u0, uint32_t (&key)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = min(u0 + 64 * j + lane, t1 - 1);
-      key[j] = u0 + 256 <= held ? s_key[t] : t < held ? s_key[t] : key_of(w[t]);
-    }
-  };
-  for (int u0 = t0; !none && u0 < t1; u0 += 256) {
-    uint32_t key[4];
-    keys_at(u0, key);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool in = u0 + 64 * j + lane < t1;
-      gt += __popcll(__ballot(in && key[j] > prefix));
-      eq += __popcll(__ballot(in && key[j] == prefix));
-    }
-  }
-  if (lane == 0) {
-    s_gt[wave] = gt;
-    s_eq[wave] = eq;
-  }
-  __syncthreads();
   int at = 0, ties = 0;
-  for (int k = 0; k < wave; ++k) {
-    at += s_gt[k] + min(s_eq[k], max(room - ties, 0));
-    ties += s_eq[k];
-  }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int u0 = t0; !none && u0 < t1; u0 += 256) {
-    uint32_t key[4];
-    keys_at(u0, key);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = u0 + 64 * j + lane;
-      const bool tie = t < t1 && key[j] == prefix;
+  for (int64_t from = 0; !none && from < old; from += kStretch) {
+    if (!once) hold(from);
+    int gt = 0, eq = 0;
+    each_key([&](uint32_t k, int, bool there) {
+      gt += __popcll(__ballot(there && k > prefix));
+      eq += __popcll(__ballot(there && k == prefix));
+    });
+    __syncthreads();
+    if (lane == 0) {
+      s_gt[wave] = gt;
+      s_eq[wave] = eq;
+    }
+    __syncthreads();
+    int to = 0, tied_before = 0;  // of this wave
+    for (int k = 0; k < kSelectWaves; ++k) {
+      if (k == wave) {
+        to = at;
+        tied_before = ties;
+      }
+      at += s_gt[k] + min(s_eq[k], max(room - ties, 0));
+      ties += s_eq[k];
+    }
+    each_key([&](uint32_t k, int j, bool there) {
+      const bool tie = there && k == prefix;
       const uint64_t tied = __ballot(tie);
       const bool stays =
-          (t < t1 && key[j] > prefix) || (tie && ties + __popcll(tied & below) < room);
+          (there && k > prefix) || (tie && tied_before + __popcll(tied & below) < room);
       const uint64_t all = __ballot(stays);
-      if (stays) kept[at + __popcll(all & below)] = t;
-      at += __popcll(all);
-      ties += __popcll(tied);
-    }
+      if (stays) kept[to + __popcll(all & below)] = t0 + 64 * j + lane;
+      to += __popcll(all);
+      tied_before += __popcll(tied);
+    });
   }
   for (int j = tid; j < g.e.recent; j += kSelect) kept[keep - g.e.recent + j] = old + j;
 }
@@ -359,13 +357,8 @@ hipError_t launch_paged_evict(const PagedShape &p, const PagedSeqs &q, const Pag
   g.cap = std::min((int64_t)q.width * p.page_size, (int64_t)kMaxTokens);
   g.row_bytes = p.dim * (p.io == IoType::F32 ? 4 : 2);
   const int64_t rows = (int64_t)q.n_seqs * p.n_heads;
-  g.held = (int)std::max<int64_t>(4, std::min<int64_t>(g.cap, kHeld));  // (a multiple of 4)
-  hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void *>(select_kernel),
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kHeld);
-  if (r != hipSuccess) return r;
-  r = over_blocks(g, rows, kSelect, [&](int blocks) {
-    select_kernel<<<blocks, kSelect, 4 * g.held, s>>>(g);
-  });
+  const hipError_t r = over_blocks(
+      g, rows, kSelect, [&](int blocks) { select_kernel<<<blocks, kSelect, 0, s>>>(g); });
   if (r != hipSuccess) return r;
   if (e.into) {
     g.chunks = (e.keep + kRun - 1) / kRun + 1;
