@@ -42,7 +42,13 @@ def attend(q, k, v, seen, at, scale, dtype, *, softcap=None, slopes=None, q_err=
     over its sum.  Exponential, product, quotient and joins round a few times each (32), the sum
     over n tokens as a random walk (4 sqrt(n)).  Weights and queries enter half-precision products
     as two numbers at the least: 2^-16 of the value (bf16), 2^-20 (fp16).  Then the rounding to
-    the type."""
+    the type.
+
+    A weight exp(s - m) below 2^-126, fp32's smallest normal number, is 0, and so is what a
+    number of a weight, or a product of one and a value, has below it: with up to three numbers a
+    weight, that is up to 2^-126 (1 + 3 |v|) of each token's part, over a sum of 1 or more.  It
+    shows where everything else of an output is 0: one token of value 0 beside others of weight
+    1e-40 gave 0 for -2e-40."""
     m, hq, d = q.shape
     h, n = k.shape[:2]
     g = hq // h
@@ -74,7 +80,8 @@ def attend(q, k, v, seen, at, scale, dtype, *, softcap=None, slopes=None, q_err=
         ds = (ds * (w > 1e-12)).amax(1, keepdim=True)
         rel = 2 * ds + U32 * (32 + 4 * math.sqrt(n)) + split
         out[:, j] = w @ vj
-        tol[:, j] = rel * (w @ vj.abs()) + R.u(dtype) * out[:, j].abs() + R._tiny(dtype)
+        lost = 2.0 ** -126 * (seen.double() @ (1 + 3 * vj.abs()))
+        tol[:, j] = rel * (w @ vj.abs()) + lost + R.u(dtype) * out[:, j].abs() + R._tiny(dtype)
         mass[j // g] += w.sum(0)
         mass_tol[j // g] += (w * rel).sum(0) + 1e-12
     return out, tol, mass, mass_tol

@@ -261,6 +261,18 @@ def test_masks_caps_and_biases(dtype, group, window):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [3, 6])
+@pytest.mark.parametrize("slope", [0.03, 0.045, 0.052])
+def test_weights_at_the_end_of_fp32(dtype, group, slope):
+    """A token of its own, whose values are 0 in some channels, and a prefix 1,900 tokens away: e^-57
+    to e^-104 of the weight."""
+    lengths = [2000, 1950]
+    c = Case(lengths, 2, group, 64, 16, dtype)
+    c.check(window=1, prefix=torch.full((2,), 70, dtype=torch.int32),
+            slopes=slope * torch.linspace(1, 1.05, 2 * group))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rotated_queries(dtype):
     Case([1, 50, 700, 0], 2, 4, 128, 16, dtype, rot=128).check()
 
