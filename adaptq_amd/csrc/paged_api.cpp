@@ -157,6 +157,14 @@ bool seqs_ok(const int *table, int width, int stride, const int *lengths, int n_
   return aligned_to(table, 4, fn) && aligned_to(lengths, 4, fn);
 }
 
+bool over_pages(const Paged *p, const Span &x) {
+  for (const void *q : {p->shape.k_pages, p->shape.v_pages}) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
+    if (x.lo < lo + p->pool && lo < x.hi) return true;
+  }
+  return false;
+}
+
 // Rows of a call against the cache: strides, alignment, and the pages' own memory.
 bool rows_ok(const Paged *p, const void *rows, const char *name, int heads, int n, size_t nb1,
              size_t nb2, bool written, const char *fn) {
@@ -171,14 +179,9 @@ bool rows_ok(const Paged *p, const void *rows, const char *name, int heads, int 
     set_errorf(fn, "output rows overlap");
     return false;
   }
-  const Span x = span_of(rows, row, counts, nb, 2);
-  const size_t pool = p->pool;
-  for (const void *q : {s.k_pages, s.v_pages}) {
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
-    if (x.lo < lo + pool && lo < x.hi) {
-      set_errorf(fn, "rows overlap the pages");
-      return false;
-    }
+  if (over_pages(p, span_of(rows, row, counts, nb, 2))) {
+    set_errorf(fn, "rows overlap the pages");
+    return false;
   }
   return true;
 }
@@ -451,8 +454,13 @@ bool weights_ok(const Paged *p, float *w, size_t nb1, size_t nb2, const aq::Page
   const size_t nb[2] = {nb1, nb2};
   const int n[2] = {p->shape.n_heads, q.n_seqs};
   if (!aligned_to(w, 4, fn) || !strides_ok(4, n, nb, 2, fn)) return false;
-  if (!rows_apart((size_t)q.width * p->shape.page_size * 4, n, nb, 2)) {
+  const size_t row = (size_t)q.width * p->shape.page_size * 4;
+  if (!rows_apart(row, n, nb, 2)) {
     set_errorf(fn, "d_weights has rows of fewer than table_width * page_size values");
+    return false;
+  }
+  if (q.n_seqs > 0 && over_pages(p, span_of(w, row, n, nb, 2))) {
+    set_errorf(fn, "d_weights overlaps the pages");
     return false;
   }
   to->weights = w;
@@ -467,7 +475,9 @@ int paged_scored(Paged *p, const Token &t, const aq::PagedSeqs &q, const adaptq_
   aq::PagedScores sc;
   aq::PagedWeights w;
   if (q.n_seqs < 0 || q.width < 0) return paged_token(p, t, q, nullptr, nullptr, stream, fn);
-  if (!scores_ok(scores, scale_of(p, t.scale), &sc, fn) || !weights_ok(p, d_weights, w_nb1, w_nb2, q, &w, fn)) return -1;
+  if (!scores_ok(scores, scale_of(p, t.scale), &sc, fn) ||
+      !weights_ok(p, d_weights, w_nb1, w_nb2, q, &w, fn))
+    return -1;
   if (w.weights) {
     if (t.q_heads <= 0 || t.q_heads % p->shape.n_heads || (long long)q.n_seqs * t.q_heads > INT_MAX)
       return paged_token(p, t, q, nullptr, nullptr, stream, fn);  // (refuses)
@@ -475,6 +485,20 @@ int paged_scored(Paged *p, const Token &t, const aq::PagedSeqs &q, const adaptq_
                       aq::paged_weights_workspace(p->shape, t.q_heads, q.n_seqs, q.width), fn))
       return -1;
     w.workspace = ws;
+    // the sums against the rows of the call, each from its first byte to its last
+    const size_t row = size_of((int)p->shape.io) * p->shape.dim, w_nb[2] = {w_nb1, w_nb2};
+    const int nw[2] = {p->shape.n_heads, q.n_seqs}, nq[2] = {t.q_heads, q.n_seqs};
+    const Span x = span_of(w.weights, (size_t)q.width * p->shape.page_size * 4, nw, w_nb, 2);
+    const auto meets = [&](const void *rows, const int *n, const size_t *nb) {
+      if (!rows || q.n_seqs == 0) return false;
+      const Span y = span_of(rows, row, n, nb, 2);
+      return x.lo < y.hi && y.lo < x.hi;
+    };
+    if (meets(t.q, nq, t.q_nb) || meets(t.out, nq, t.q_nb + 2) || meets(t.k, nw, t.kv_nb) ||
+        meets(t.v, nw, t.kv_nb + 2)) {
+      set_errorf(fn, "d_weights overlaps rows of the call");
+      return -1;
+    }
   }
   Token to = t;
   to.window = sc.window;

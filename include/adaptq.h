@@ -516,7 +516,8 @@ int adaptq_paged_prompt_device(adaptq_paged_t cache, const void *d_q, void *d_ou
  * n - 1 (of the n tokens it then holds).  d_weights, NULL or fp32 [n_seqs][n_heads] rows of at
  * least table_width * page_size values, w_nb1 and w_nb2 bytes apart: to each token that is
  * seen, the sum of its weights in the softmaxes of its key head's query heads is added (in
- * their order; one more launch).  d_workspace: then device memory of
+ * their order; one more launch); over the pages or the call's rows they are refused.
+ * d_workspace: then device memory of
  * adaptq_paged_weights_workspace bytes (4 a column of the table, slot and query head),
  * 16-byte aligned, this call's alone until it is done.  Returns 0/-1. */
 size_t adaptq_paged_weights_workspace(adaptq_paged_t cache, int n_q_heads, int n_seqs,

@@ -255,6 +255,9 @@ def test_refusals():
     for bad in (w[:1], w.half(), w.cpu(), w[:, :, 1:]):
         with pytest.raises(ValueError):
             c.cache.evict(bad, t, n, 10)
+    pages = c.p.v_pages.flatten().view(torch.float32)[:w.numel()].view(w.shape)
+    with pytest.raises(RuntimeError, match="overlap"):
+        c.cache.evict(pages, t, n, 10)
     rotates = PagedCache(c.p.k_pages, c.p.v_pages, rotary=Rotary(64))
     with pytest.raises(ValueError):
         rotates.evict(w, t, n, 10)

@@ -273,6 +273,15 @@ def test_refusals():
             c.cache.attend(c.q, c.p.table, c.p.lengths, weights=w)
     with pytest.raises(RuntimeError):  # rows over each other
         c.cache.attend(c.q, c.p.table, c.p.lengths, weights=good[:, :1].expand(2, 2, tokens))
+    pages = c.p.k_pages.flatten().view(torch.float32)[:4 * tokens].view(2, 2, tokens)
+    room = torch.zeros(2 ** 12, device="cuda")
+    over = room[:4 * tokens].view(2, 2, tokens)
+    rows = room.view(torch.float16)[128:640].view(2, 4, 64)
+    for w, q, out in ((pages, c.q, None), (over, rows, None), (over, c.q, rows)):  # over the rows
+        with pytest.raises(RuntimeError, match="overlap"):
+            c.cache.attend(q, c.p.table, c.p.lengths, weights=w, out=out)
+    with pytest.raises(RuntimeError, match="overlap"):
+        c.cache.step(c.q, rows[:, :2], c.q[:, 2:], c.p.table, c.p.lengths, weights=over)
     for kw in (dict(softcap=0.0), dict(slopes=torch.zeros(5, device="cuda")),
                dict(first=torch.zeros(2, device="cuda")),
                dict(prefix=torch.zeros(3, dtype=torch.int32, device="cuda"))):
