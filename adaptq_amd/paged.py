@@ -378,7 +378,8 @@ class PagedCache4(_Pages):
             at = offsets.data_ptr()
         elif tokens != lengths.shape[0]:
             raise ValueError("without offsets, one token a sequence is read")
-        k, v = (torch.empty(tokens, self.heads, self.dim, device=self.device) for _ in range(2))
+        k, v = (torch.empty(tokens, self.heads, self.dim, dtype=torch.float32, device=self.device)
+                for _ in range(2))
         if tokens and not seqs[4]:
             return k.zero_(), v.zero_()
         if tokens:
