@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
   const int n = tokens_of(g, seq), keep = g.e.keep;
   int *kept = g.e.kept + block * keep;
   if (n <= keep) {
-    for (int j = tid; j < keep; j += kSelect) kept[j] = j < n ? j : -1;
+    for (int64_t j = tid; j < keep; j += kSelect) kept[j] = j < n ? (int)j : -1;
     return;
   }
   const float *w = g.e.weights + seq * g.e.nb[1] + head * g.e.nb[0];
@@ -196,7 +196,8 @@ __global__ __launch_bounds__(kSelect) void select_kernel(const Args g) {
       tied_before += __popcll(tied);
     });
   }
-  for (int j = tid; j < g.e.recent; j += kSelect) kept[keep - g.e.recent + j] = old + j;
+  for (int64_t j = tid; j < g.e.recent; j += kSelect)
+    kept[keep - g.e.recent + j] = old + (int)j;
 }
 
 // Where token t of a sequence lies: row in the pages, or -1.
@@ -214,23 +215,23 @@ __device__ __forceinline__ int64_t row_of(const Args &g, const int *table, int w
 __device__ __forceinline__ void move_weights(const Args &g, float *w, const int *kept, int n,
                                              int tid) {
   const int keep = g.e.keep;
-  for (int j0 = 0; j0 < keep; j0 += kInFlight * kMove) {
+  for (int64_t j0 = 0; j0 < keep; j0 += kInFlight * kMove) {
     float x[kInFlight];
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      const int j = j0 + i * kMove + tid;
+      const int64_t j = j0 + i * kMove + tid;
       if (j < keep) x[i] = w[kept[j]];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      const int j = j0 + i * kMove + tid;
+      const int64_t j = j0 + i * kMove + tid;
       if (j < keep) w[j] = x[i];
     }
   }
   __syncthreads();  // (the last ones read lie behind)
-  for (int j = keep + tid; j < n; j += kMove) w[j] = 0.0f;
+  for (int64_t j = (int64_t)keep + tid; j < n; j += kMove) w[j] = 0.0f;
 }
 
 // In place: token kept[j] >= j goes to j, with j ascending, so a chunk's rows may be written once
@@ -258,19 +259,19 @@ __global__ __launch_bounds__(kMove) void move_kernel(const Args g) {
   const int part = tid % parts, row0 = tid / parts;
   const int *table = g.q.table + (int64_t)seq * g.q.stride;
   const int chunk = per * kInFlight;
-  for (int j0 = 0; j0 < keep; j0 += chunk) {
-    const int last = min(j0 + chunk, keep) - 1;
+  for (int64_t j0 = 0; j0 < keep; j0 += chunk) {
+    const int last = (int)min(j0 + chunk, (int64_t)keep) - 1;
     if (kept[last] == last) continue;  // all of them stay where they are
     u32x4 x[kInFlight];
     int64_t to[kInFlight];
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      const int j = j0 + i * per + row0;
+      const int64_t j = j0 + i * per + row0;
       to[i] = -1;
       if (row0 < per && j <= last) {
         const int64_t from = row_of(g, table, g.q.width, head, kept[j]);
         if (from >= 0) {
-          to[i] = row_of(g, table, g.q.width, head, j);
+          to[i] = row_of(g, table, g.q.width, head, (int)j);
           x[i] = *reinterpret_cast<const u32x4 *>(pool + from * g.row_bytes + 16 * part);
         }
       }
@@ -361,7 +362,8 @@ hipError_t launch_paged_evict(const PagedShape &p, const PagedSeqs &q, const Pag
       g, rows, kSelect, [&](int blocks) { select_kernel<<<blocks, kSelect, 0, s>>>(g); });
   if (r != hipSuccess) return r;
   if (e.into) {
-    g.chunks = (e.keep + kRun - 1) / kRun + 1;
+    // (of the tokens that a sequence can hold: keep may be up to the last int)
+    g.chunks = (int)((std::min((int64_t)e.keep, g.cap) + kRun - 1) / kRun) + 1;
     return over_blocks(g, rows * g.chunks, kMove,
                        [&](int blocks) { copy_kernel<<<blocks, kMove, 0, s>>>(g); });
   }
