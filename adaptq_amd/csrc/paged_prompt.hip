@@ -62,6 +62,7 @@ struct Args {
   PagedPrompt a;
   float scale2;        // of the scores, to base 2, positive
   float cap_in, cap2;  // 1 / cap of a score, cap to base 2
+  bool cap_rough;      // (scores.hpp)
   bool flip;           // a negative scale: the queries change sign
   int group;           // query heads of a key head
   int64_t cap;         // tokens that the table has columns for
@@ -584,11 +585,16 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     if constexpr (SHAPED) {
       const PagedScores &sc = g.a.scores;
       const float cap_in = g.cap_in, cap2 = g.cap2;
-      if (sc.softcap > 0.0f) {
+      if (K::kHalf && g.cap_rough) {
 #pragma unroll
         for (int i = 0; i < K::kSubs; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) s[i][j] = capped<!K::kHalf>(s[i][j], cap_in, cap2);
+          for (int j = 0; j < 16; ++j) s[i][j] = capped<false>(s[i][j], cap_in, cap2);
+      } else if (sc.softcap > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < K::kSubs; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[i][j] = capped<true>(s[i][j], cap_in, cap2);
       } else {
 #pragma unroll
         for (int i = 0; i < K::kSubs; ++i) s[i] *= scale2;
@@ -899,6 +905,7 @@ hipError_t launch_paged_prompt(const PagedShape &p, const PagedSeqs &q, const Pa
   if (a.scores.softcap > 0) {
     g.cap_in = scale / a.scores.softcap;
     g.cap2 = a.scores.softcap * kLog2e;
+    g.cap_rough = a.scores.softcap <= kRoughCap;
   }
   g.group = a.q_heads / p.n_heads;
   g.cap = cap_of(p, q.width);

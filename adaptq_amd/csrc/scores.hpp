@@ -12,8 +12,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // u = exp(-2|z|), tanh is (1 - u) / (1 + u).  1 - u keeps 2^-24 of 1, so below 0.6 of z the error
 // would grow against the value: EXACT takes z times a polynomial of z^2 there (fitted at
 // Chebyshev points, 2^-26 of the value), 2^-21 of the value above (the reciprocal is within one
-// step, as the exponential is).  Without EXACT the error is 2^-22 of the cap everywhere, a
-// thousandth of what scores of half-precision rows and weights are rounded by.
+// step, as the exponential is).  Without EXACT the error is 2^-22 of the cap everywhere, whatever
+// the score: for half-precision rows and caps up to kRoughCap alone, where it is 2^-16 of a unit,
+// as much as their weights are rounded by.
+constexpr float kRoughCap = 64.0f;
+
 template <bool EXACT>
 __device__ __forceinline__ float capped(float s, float in, float cap2) {
   const float z = s * in;
