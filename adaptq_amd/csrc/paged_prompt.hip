@@ -319,24 +319,8 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   w = __builtin_amdgcn_readfirstlane(w), e = __builtin_amdgcn_readfirstlane(e);
   w_all = __builtin_amdgcn_readfirstlane(w_all), e_all = __builtin_amdgcn_readfirstlane(e_all);
 
-  // the passes: units of kKeys tokens, in one run or two
-  int u_first = w / K::kKeys, u_end = (e + K::kKeys - 1) / K::kKeys, gap_at = INT_MAX, gap = 0;
-  if (w >= e) u_first = u_end = 0;
-  if (lo < pe) {
-    const int p0 = lo / K::kKeys, p1 = (pe + K::kKeys - 1) / K::kKeys;
-    if (u_first >= u_end) {
-      u_first = p0;
-      u_end = p1;
-    } else {
-      if (u_first > p1) {
-        gap_at = p1;
-        gap = u_first - p1;
-      }
-      u_end = max(u_end, p1) - gap;
-      u_first = min(p0, u_first);
-    }
-  }
-  const int units = u_end - u_first;
+  const Passes passes = passes_of(lo, pe, w, e, K::kKeys);
+  const int units = passes.count;
   const int i0 = (int)((int64_t)units * split / g.splits),
             i1 = (int)((int64_t)units * (split + 1) / g.splits);
 
@@ -358,10 +342,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
   u32x4 k_in[K::kHalf ? 1 : K::kPasses], v_in[K::kHalf ? 1 : K::kPasses];
 
-  const auto real = [&](int i) {  // unit of pass i
-    const int u = u_first + i;
-    return u >= gap_at ? u + gap : u;
-  };
+  const auto real = [&](int i) { return unit_of(passes, i); };
   // Where the wave's tokens of 64 passes lie, a pass a lane: the offset of their block's rows in
   // the pools, and how many bytes of it are there (0: no page, or no tokens).
   uint64_t at64 = 0;
@@ -406,7 +387,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     }
     if (lane == 0 && wave_row % 16 == 0) s_page[buffer][wave_row / 16] = bytes > 0;
   };
-  const auto all_seen = [&](int t0) { return t0 >= w_all && t0 + K::kKeys <= e_all; };
+  const auto all_seen = [&](int t0) { return unit_within(t0, K::kKeys, w_all, e_all); };
   // The loads of pass i are in LDS (of this wave).  An infinity or NaN among the values of a token
   // that some query does not see must not meet its weight of 0: zeros take its place, and at the
   // end it is added for the queries that do see it.
@@ -579,7 +560,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     const uint32_t there_are = *reinterpret_cast<const uint32_t *>(s_page[buffer]);
     const uint32_t pages = __builtin_amdgcn_readfirstlane(there_are);
     constexpr uint32_t kAll = K::kBlocks == 4 ? 0x01010101u : 0x0101u;
-    const bool full = t0 >= wave_w_all && t0 + K::kKeys <= wave_e_all && (pages & kAll) == kAll;
+    const bool full = unit_within(t0, K::kKeys, wave_w_all, wave_e_all) && (pages & kAll) == kAll;
     const int t1 = t0 + 4 * half;
     float scale2 = g.scale2;
     if constexpr (SHAPED) {
@@ -691,7 +672,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     __syncthreads();  // pass i is there, and the buffer of pass i - 1 free
     if (i + 1 < i1) load(i + 1);
     const int t0 = real(i) * K::kKeys;
-    if (t0 < wave_e && t0 + K::kKeys > wave_lo) {
+    if (unit_meets(t0, K::kKeys, wave_lo, wave_e)) {
       Scores s;
       products(s, (i - i0) & 1);
       weigh(s, (i - i0) & 1, t0);
@@ -704,7 +685,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     for (int i = i0; i < i1; ++i) {
       const int t0 = real(i) * K::kKeys;
       if (all_seen(t0)) continue;
-      for (int t = t0; t < min(t0 + K::kKeys, n); ++t) {
+      for (int t = t0, end = unit_end(t0, K::kKeys, n); t < end; ++t) {
         const int c = page_column(g.page_of, t >> 4);
         const int page = ((cint *)(uint64_t)table)[c];
         if (page < 0 || page >= g.p.n_pages) continue;

@@ -125,6 +125,51 @@ AQ_SPLIT_HD int real_unit(const SeenSpan &s, int unit) {
   return unit >= s.gap_at ? unit + s.gap : unit;
 }
 
+// The passes of a prompt's tile: the units of `keys` tokens that hold tokens of the runs [lo, pe)
+// and [w, e), either of which may be empty.  Pass i is unit first + i, or, behind what lies
+// between the runs, first + i + gap.  Tokens end at kMaxTokens, a unit of 64 may end beyond an
+// int: its first token and the runs' ends are what is compared.
+struct Passes {
+  int first, count;
+  int gap_at, gap;
+};
+
+AQ_SPLIT_HD Passes passes_of(int lo, int pe, int w, int e, int keys) {
+  Passes p = {0, 0, 0x7FFFFFFF, 0};
+  int end = 0;
+  if (w < e) {
+    p.first = w / keys;
+    end = (e - 1) / keys + 1;
+  }
+  if (lo < pe) {
+    const int p0 = lo / keys, p1 = (pe - 1) / keys + 1;
+    if (p.first >= end) {
+      p.first = p0;
+      end = p1;
+    } else {
+      if (p.first > p1) {
+        p.gap_at = p1;
+        p.gap = p.first - p1;
+      }
+      end = (end > p1 ? end : p1) - p.gap;
+      p.first = p0 < p.first ? p0 : p.first;
+    }
+  }
+  p.count = end - p.first;
+  return p;
+}
+
+AQ_SPLIT_HD int unit_of(const Passes &p, int pass) {
+  const int u = p.first + pass;
+  return u >= p.gap_at ? u + p.gap : u;
+}
+
+// Whether the unit's tokens from t0 on all lie in [a, b); whether some do (a and b not negative);
+// and where they end among n > t0 tokens.
+AQ_SPLIT_HD bool unit_within(int t0, int keys, int a, int b) { return t0 >= a && t0 <= b - keys; }
+AQ_SPLIT_HD bool unit_meets(int t0, int keys, int a, int b) { return t0 < b && t0 > a - keys; }
+AQ_SPLIT_HD int unit_end(int t0, int keys, int n) { return n - t0 < keys ? n : t0 + keys; }
+
 // Units of a block: an equal share of the total, in whole passes of the block's waves.
 AQ_SPLIT_HD int64_t share_of(int64_t total, int blocks, int waves) {
   const int64_t s = ((total + blocks - 1) / blocks + waves - 1) / waves * waves;
