@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   extern __shared__ __align__(16) char lds[];
   __shared__ int s_red[kWaves][8];
   __shared__ __align__(4) uint8_t s_page[2][4];  // whether a block of 16 tokens has a page
-  __shared__ int s_wild;
+  __shared__ int s_wild[2];  // the first and the last pass with an infinity or NaN among its values
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int dim = g.p.dim, heads = g.p.n_heads;
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
     for (int i = 1; i < 6; ++i) x = lane == i ? red[i] : x;
     s_red[wave][lane] = x;
   }
-  if (tid == 0) s_wild = 0;
+  if (tid == 0) s_wild[0] = INT_MAX, s_wild[1] = -1;
   __syncthreads();
   int lo = INT_MAX, pe = 0, w = INT_MAX, e = 0, w_all = 0, e_all = INT_MAX;
 #pragma unroll
@@ -390,11 +390,20 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   const auto all_seen = [&](int t0) { return unit_within(t0, K::kKeys, w_all, e_all); };
   // The loads of pass i are in LDS (of this wave).  An infinity or NaN among the values of a token
   // that some query does not see must not meet its weight of 0: zeros take its place, and at the
-  // end it is added for the queries that do see it.
+  // end it is added for the queries that do see it.  A weight's second number may be 0 too, or a
+  // weight below the smallest number: where that shows, the passes that all queries see are gone
+  // over in the same way (tame_all).
+  bool tame_all = false;
+  const auto found = [&](int i) {
+    if (lane == 0) {
+      atomicMin(&s_wild[0], i);
+      atomicMax(&s_wild[1], i);
+    }
+  };
   const auto arrive = [&](int i) {
     char *to = lds + ((i - i0) & 1) * K::kBuffer;
     char *v_to = to + K::kKeys * K::kKStride;
-    const bool whole = all_seen(real(i) * K::kKeys);
+    const bool whole = !tame_all && all_seen(real(i) * K::kKeys);
     if constexpr (K::kHalf) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (whole) return;
@@ -403,7 +412,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
         u32x4 *at = reinterpret_cast<u32x4 *>(v_to + wave_row * K::kVStride + p * 1024 + lane * 16);
         const u32x4 y = *at;
         if (!__any(wild4<T>(y))) continue;
-        s_wild = 1;
+        found(i);
         *at = tamed4<T>(y);
       }
     } else {
@@ -412,7 +421,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
         const int row = wave_row + p * K::kRowsAPass + l_row;
         u32x4 y = v_in[p];
         if (!whole && __any(wild4<T>(y))) {
-          s_wild = 1;
+          found(i);
           y = tamed4<T>(y);
         }
         *reinterpret_cast<u32x4 *>(to + row * K::kKStride + l_chunk * 16) = k_in[p];
@@ -667,24 +676,42 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   };
 
   if (!early && i0 < i1) load(i0);
-  for (int i = i0; i < i1; ++i) {
-    arrive(i);
-    __syncthreads();  // pass i is there, and the buffer of pass i - 1 free
-    if (i + 1 < i1) load(i + 1);
-    const int t0 = real(i) * K::kKeys;
-    if (unit_meets(t0, K::kKeys, wave_lo, wave_e)) {
-      Scores s;
-      products(s, (i - i0) & 1);
-      weigh(s, (i - i0) & 1, t0);
-    }
-  }
-  __syncthreads();
-
-  if (s_wild) {
-    // the tokens of the passes that not every query sees whole, one by one
+#pragma clang loop unroll(disable)
+  for (;;) {
     for (int i = i0; i < i1; ++i) {
+      arrive(i);
+      __syncthreads();  // pass i is there, and the buffer of pass i - 1 free
+      if (i + 1 < i1) load(i + 1);
       const int t0 = real(i) * K::kKeys;
-      if (all_seen(t0)) continue;
+      if (unit_meets(t0, K::kKeys, wave_lo, wave_e)) {
+        Scores s;
+        products(s, (i - i0) & 1);
+        weigh(s, (i - i0) & 1, t0);
+      }
+    }
+    // a sum that is not finite, of weights that are numbers: once more, without the values that
+    // make it so
+    float zero = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DC / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) zero = fmaf(acc[i][j], 0.0f, zero);
+    const bool weighed = half_sum(l) <= FLT_MAX;  // (not NaN)
+    const bool odd = live && weighed && zero != 0.0f;
+    if (!__syncthreads_or(odd) || tame_all) break;
+    tame_all = true;
+    m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DC / 32; ++i) acc[i] = f32x16{0};
+    locate(i0);
+    if (i0 < i1) load(i0);
+  }
+
+  if (s_wild[1] >= 0) {
+    // the tokens of the passes that not every query sees whole, one by one
+    for (int i = s_wild[0]; i <= s_wild[1]; ++i) {
+      const int t0 = real(i) * K::kKeys;
+      if (!tame_all && all_seen(t0)) continue;
       for (int t = t0, end = unit_end(t0, K::kKeys, n); t < end; ++t) {
         const int c = page_column(g.page_of, t >> 4);
         const int page = ((cint *)(uint64_t)table)[c];
