@@ -44,8 +44,9 @@ constexpr int kRows = 32 * kWaves;  // of a tile
 constexpr int kBeyond = 1 << 30;
 constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
 // A maximum is followed only when it grows by more than this (in powers of two): weights
-// are then up to 2^8 of what they would be, which no sum or type minds, and most passes
-// leave the sums as they are.
+// are then up to 2^8 of what they would be, and most passes leave the sums as they are.  A sum
+// of values of 2^119 and more may pass fp32's end by that; such a tile is gone over again with
+// the maximum followed always.  (Sums of weights up to 1 still end where fp32 does.)
 constexpr float kLazy = 8.0f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -394,6 +395,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
   // weight below the smallest number: where that shows, the passes that all queries see are gone
   // over in the same way (tame_all).
   bool tame_all = false;
+  float lazy = kLazy;
   const auto found = [&](int i) {
     if (lane == 0) {
       atomicMin(&s_wild[0], i);
@@ -628,7 +630,7 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
         for (int j = 0; j < 16; ++j) y = fmaxf(y, s[i][j]);
       top = half_max(fmaxf(top, y * scale2));
     }
-    if (__any(top > m + kLazy)) {  // (m is minus infinity at first)
+    if (__any(top > m + lazy)) {  // (m is minus infinity at first)
       const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
       l *= keep;
 #pragma unroll
@@ -689,8 +691,8 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
         weigh(s, (i - i0) & 1, t0);
       }
     }
-    // a sum that is not finite, of weights that are numbers: once more, without the values that
-    // make it so
+    // a sum that is not finite, of weights that are numbers: once more without the values that
+    // make it so, and if it is too large by itself, with smaller weights
     float zero = 0.0f;
 #pragma unroll
     for (int i = 0; i < DC / 32; ++i)
@@ -698,7 +700,8 @@ __global__ __launch_bounds__(kThreads, (Kind<T, DP>::kResident)) void prompt_ker
       for (int j = 0; j < 16; ++j) zero = fmaf(acc[i][j], 0.0f, zero);
     const bool weighed = half_sum(l) <= FLT_MAX;  // (not NaN)
     const bool odd = live && weighed && zero != 0.0f;
-    if (!__syncthreads_or(odd) || tame_all) break;
+    if (!__syncthreads_or(odd) || lazy == 0.0f) break;
+    if (tame_all) lazy = 0.0f;
     tame_all = true;
     m = -INFINITY, l = 0.0f;
 #pragma unroll

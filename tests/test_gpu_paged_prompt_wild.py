@@ -1,5 +1,5 @@
 """Infinities and NaN among the values that every query of a prompt's tile sees, at every weight
-that a token can have."""
+that a token can have; values near the end of fp32's range."""
 import math
 
 import pytest
@@ -67,6 +67,25 @@ def test_of_any_weight(dtype, n, new):
     rest = [i for i in range(40, 64) if i not in (50, 60)]
     R.check(got[:, :, rest], *(x[:, :, rest] for x in c.want()))
     assert torch.equal(c.run().nan_to_num(7.0), got.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,new", [(500, 30), (6000, 20)])
+def test_values_near_the_end_of_fp32(dtype, n, new):
+    """A maximum that grows by less than 2^8 a pass, and a value of 2^126 at its top: the formula
+    is finite, so is the output."""
+    c = P.Case([n], [new], 1, 2, 64, 16, dtype)
+    at = torch.arange(n) % 128  # (where the pieces of a cut tile begin, of four passes or more)
+    scores = (at >= 32) * 2.0 + (at >= 64) * 2.0
+    scores[456] = 5.0
+    rising(c, scores)
+    c.p.v[0].zero_()
+    c.p.v[0][456, 0, 5] = 2.0 ** 126
+    c.p.v[0][457, 0, 6] = -2.0 ** 126
+    c.p.put(0)
+    want, tol = c.want()
+    assert want.abs().max() > 2.0 ** 110
+    R.check(c.run(), want, tol)
 
 
 def test_prompts_of_all_types_of_trouble_in_one_batch():
