@@ -48,6 +48,9 @@ constexpr int kBatch = 8;  // pieces of a join whose loads are in flight at once
 // of values of 2^119 and more may pass fp32's end by that; such a tile is gone over again with
 // the maximum followed always.  (Sums of weights up to 1 still end where fp32 does.)
 constexpr float kLazy = 8.0f;
+// A piece's weight in a join at the least, fp32's smallest number: infinities of a piece of no
+// weight stay what they are, and finite values stay below 2^-21.
+constexpr float kLeast = 0x1p-149f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -806,14 +809,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Args g) {
         to = fmaxf(to, ml[k].x);
       }
       if (to == -INFINITY) continue;
-      const float keep = __builtin_amdgcn_exp2f(m - to);
+      const float keep = fmaxf(__builtin_amdgcn_exp2f(m - to), kLeast);
       l *= keep;
       y *= keep;
       m = to;
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         if (ml[k].x == -INFINITY) continue;
-        const float e = __builtin_amdgcn_exp2f(ml[k].x - to);
+        const float e = fmaxf(__builtin_amdgcn_exp2f(ml[k].x - to), kLeast);
         l = fmaf(e, ml[k].y, l);
         y += e * f32x4{a[k].x, a[k].y, b[k].x, b[k].y};
       }

@@ -69,6 +69,27 @@ def test_of_any_weight(dtype, n, new):
     assert torch.equal(c.run().nan_to_num(7.0), got.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("dtype", P.DTYPES)
+def test_in_a_piece_of_no_weight(dtype):
+    """A tile that is cut: all of the first piece's tokens weigh e^-100 beside the others', and one
+    of them is infinite."""
+    c = P.Case([6000], [20], 1, 2, 64, 16, dtype)
+    scores = torch.zeros(6000)
+    scores[:3000] = -100.0
+    rising(c, scores)
+    c.p.put(0)
+    clean = c.check()
+    c.p.v[0][40, 0, 3] = float("inf")
+    c.p.v[0][2990, 0, 4] = -float("inf")
+    c.p.v[0][1500, 0, 5] = float("nan")
+    c.p.put(0)
+    got = c.run()
+    assert (got[:, :, 3] == float("inf")).all() and (got[:, :, 4] == -float("inf")).all()
+    assert torch.isnan(got[:, :, 5]).all()
+    rest = [0, 1, 2, *range(6, 64)]
+    assert torch.equal(got[:, :, rest], clean[:, :, rest])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,new", [(500, 30), (6000, 20)])
 def test_values_near_the_end_of_fp32(dtype, n, new):
