@@ -235,10 +235,20 @@ __device__ __forceinline__ int piece_slot(int first, int k) {
   return k == 0 ? 2 * first + 1 : 2 * (first + k);
 }
 
+// A part's weight beside others, of the difference of their maxima.  MANY: at the least fp32's
+// smallest number, so that an infinity that mend() added to a part of no weight stays one (finite
+// values come to less than 2^-21).
+template <bool MANY>
+__device__ __forceinline__ float weight_of(float x) {
+  const float e = __builtin_amdgcn_exp2f(x);
+  return MANY ? fmaxf(e, 0x1p-149f) : e;
+}
+
 // Pieces k0, k0 + step, ... (n of them) of a segment together, in their order, by the block
 // that finished last.  Threads beyond one per 4 channels of a row share the pieces; a thread
 // has the loads of kBatch pieces in flight at once.  put(row, channel, sums, max, sum).
-template <int DP, typename Put>
+// MANY: what weight_of says.
+template <int DP, bool MANY, typename Put>
 __device__ __forceinline__ void join(const Args &g, int first, int piece0, int step, int n,
                                      int rows, int tid, float *lds, Put put) {
   constexpr int kPart = part_floats(DP);
@@ -268,14 +278,14 @@ __device__ __forceinline__ void join(const Args &g, int first, int piece0, int s
           top = fmaxf(top, ml[j].x);
         }
         if (top == -INFINITY) continue;
-        const float keep = __builtin_amdgcn_exp2f(m - top);
+        const float keep = weight_of<MANY>(m - top);
         l *= keep;
         y *= keep;
         m = top;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
           if (ml[j].x == -INFINITY) continue;
-          const float e = __builtin_amdgcn_exp2f(ml[j].x - top);
+          const float e = weight_of<MANY>(ml[j].x - top);
           l = fmaf(e, ml[j].y, l);
           y += e * x[j];
         }
@@ -292,13 +302,13 @@ __device__ __forceinline__ void join(const Args &g, int first, int piece0, int s
         float top = m;
         for (int k = 1; k < parts; ++k) top = fmaxf(top, at[8 * k * items + 4]);
         if (top != -INFINITY) {
-          const float keep = __builtin_amdgcn_exp2f(m - top);
+          const float keep = weight_of<MANY>(m - top);
           l *= keep;
           y *= keep;
           for (int k = 1; k < parts; ++k) {
             const float *from = at + 8 * k * items;
             if (from[4] == -INFINITY) continue;
-            const float e = __builtin_amdgcn_exp2f(from[4] - top);
+            const float e = weight_of<MANY>(from[4] - top);
             l = fmaf(e, from[5], l);
             y += e * *reinterpret_cast<const f32x4 *>(from);
           }
@@ -455,7 +465,8 @@ struct Attend {
   const int *table;
   int head, u_end;
   int row_w = 0, row_e = 0;        // MANY: the tokens that this lane's row sees
-  bool wild_values = false;        // MANY: infinities or NaN among tokens that not all rows see
+  bool wild_values = false;        // MANY: infinities or NaN among the values that were tamed
+  bool tame_all = false;           // MANY: of all tokens, not of those alone that some do not see
   float slope2 = 0.0f;             // of this lane's query head
   float *score_row = nullptr;      // where its scores go
   int64_t query_at = 0;            // its position
@@ -604,7 +615,9 @@ struct Attend {
   }
 
   // MANY: an infinity or NaN of a token that some row does not see must not meet its weight of 0:
-  // zeros take its place here, and mend() adds it for the rows that do see it.
+  // zeros take its place here, and mend() adds it for the rows that do see it.  Where all see it
+  // its weight may still be below the smallest number, or a number of the weight may: a wave whose
+  // sums show that goes over its units again with tame_all.
   __device__ void tame(Rows &r) {
     constexpr uint32_t top =
         __is_same(T, float) ? 0x7F800000u : __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
@@ -637,7 +650,7 @@ struct Attend {
   __device__ void mend(State<DP> &st, int unit) {
     for (; unit < u_end; unit += kWaves) {
       const int t0 = unit * K::kUnit;
-      if (span.all_seen(t0, t0 + K::kUnit)) continue;
+      if (!tame_all && span.all_seen(t0, t0 + K::kUnit)) continue;
       for (int t = t0; t < min(t0 + K::kUnit, span.n); ++t) {
         const int col = page_column(g.page_of, t >> 4);
         const int page = ((cint *)(uint64_t)table)[col];
@@ -712,7 +725,7 @@ struct Attend {
     if constexpr (SHAPED) shape_scores(g, s, slope2, (float)(query_at - (t0 + 4 * group4)));
     bool row_any = true;  // whether this lane's row sees a token here
     if constexpr (MANY) {
-      if (!span.all_seen(t0, t0 + K::kUnit)) tame(r);
+      if (tame_all || !span.all_seen(t0, t0 + K::kUnit)) tame(r);
       if (!full) {
         row_any = false;
 #pragma unroll
@@ -1072,8 +1085,29 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
       w1 = next;
     }
 
-    if constexpr (MANY)
+    if constexpr (MANY) {
+      // sums that are not finite, of weights that are numbers
+      float zero = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) zero = fmaf(st.acc[i][j], 0.0f, zero);
+      const bool weighed = cross_sum(st.l) <= FLT_MAX;
+      if (__any(w.row16 < rows && weighed && zero != 0.0f)) {
+        w.tame_all = true;
+        st.m = -INFINITY;
+        st.l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) st.acc[i] = f32x4{0, 0, 0, 0};
+        for (u = w.span.first_unit + u0 + wave; u < w.u_end; u += kWaves) {
+          w0 = w.locate(u);
+          w.load(r0, w0, u);
+          w.use(st, r0, w0, u);
+        }
+      }
       if (w.wild_values) w.mend(st, w.span.first_unit + u0 + wave);
+      w.tame_all = false;
+    }
 
     // the waves' parts together
     st.l = cross_sum(st.l);
@@ -1135,7 +1169,7 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
       if (m != -INFINITY) {
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-          const float e = __builtin_amdgcn_exp2f(s_m[k][row] - m);
+          const float e = weight_of<MANY>(s_m[k][row] - m);
           l = fmaf(e, s_l[k][row], l);
           y += e * *reinterpret_cast<const f32x4 *>(&s_acc[k][row][d]);
         }
@@ -1169,7 +1203,7 @@ __global__ __launch_bounds__(kThreads, A::DP == 256 ? 1 : 2) void attend_kernel(
         if (tid == 0)  // for the next call
           __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         slot = piece_slot(pc.first, piece0);
-        join<DP>(g, pc.first, piece0, step, n, rows, tid, &s_acc[0][0][0],
+        join<DP, MANY>(g, pc.first, piece0, step, n, rows, tid, &s_acc[0][0][0],
                  [&](int row, int d, f32x4 y, float m, float l) {
                    if (last) {
                      put(row, d, y, m, l);
