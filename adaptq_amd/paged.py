@@ -137,8 +137,8 @@ class _Pages:
 
     def _scores(self, n, q_heads, softcap, slopes, prefix, first):
         """What attention with scores of its own takes: (softcap, slopes, prefix, first)."""
-        if softcap is not None and not softcap > 0:
-            raise ValueError(f"softcap must be positive, got {softcap}")
+        if softcap is not None and not softcap >= 2.0 ** -100:  # 0 in fp32 would mean none
+            raise ValueError(f"softcap must be positive, 2^-100 or more, got {softcap}")
         at = []
         for name, x, dtype, size in (("slopes", slopes, torch.float32, q_heads),
                                      ("prefix", prefix, torch.int32, n),
