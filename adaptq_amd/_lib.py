@@ -107,6 +107,7 @@ SIGNATURES = {
     "adaptq_paged_step_device": (_i, [_v, _v, _v, _z, _z, _z, _z, _v, _v, _i, _z, _z, _z, _z, _v,
                                       _i, _i, _v, _i, C.c_float, _i, _v]),
     "adaptq_paged_prompt_workspace": (_z, [_v, _i, _i, _i, _i]),
+    "adaptq_paged_prompt_scores_workspace": (_z, [_v, _i, _i, _i, _i, C.POINTER(Scores)]),
     "adaptq_paged_prompt_device": (_i, [_v, _v, _v, _i, _i, _z, _z, _z, _z, _v, _i, _i, _v, _i, _v,
                                         C.c_float, C.POINTER(Scores), _v, _z, _v]),
     "adaptq_paged_weights_workspace": (_z, [_v, _i, _i, _i]),

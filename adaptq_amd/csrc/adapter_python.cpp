@@ -175,8 +175,10 @@ class PyPagedCache {
                                      width, stride, ints(lengths), n_seqs, scale, window,
                                      ptr(stream)));
   }
-  size_t prompt_workspace(int q_heads, int n_tokens, int n_seqs, int width) {
-    return adaptq_paged_prompt_workspace(h_, q_heads, n_tokens, n_seqs, width);
+  size_t prompt_workspace(int q_heads, int n_tokens, int n_seqs, int width, int window, addr prefix,
+                          addr first) {
+    const adaptq_scores_t s = {0, window, nullptr, ints(prefix), ints(first)};
+    return adaptq_paged_prompt_scores_workspace(h_, q_heads, n_tokens, n_seqs, width, &s);
   }
   void prompt(addr q, addr out, int q_heads, size_t q1, size_t q2, size_t o1, size_t o2,
               int n_tokens, addr table, int width, int stride, addr lengths, int n_seqs,

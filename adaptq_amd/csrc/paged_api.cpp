@@ -915,6 +915,20 @@ size_t adaptq_paged_prompt_workspace(adaptq_paged_t h, int n_q_heads, int n_toke
   return aq::paged_prompt_workspace(p->shape, n_q_heads, n_tokens, n_seqs, table_width);
 }
 
+size_t adaptq_paged_prompt_scores_workspace(adaptq_paged_t h, int n_q_heads, int n_tokens,
+                                            int n_seqs, int table_width,
+                                            const adaptq_scores_t *scores) {
+  if (!h || n_q_heads <= 0 || n_tokens <= 0 || n_seqs <= 0 || table_width < 0) return 0;
+  const Paged *p = static_cast<Paged *>(h);
+  if (n_q_heads % p->shape.n_heads) return 0;
+  aq::PagedPrompt a{};
+  a.q_heads = n_q_heads;
+  a.n_tokens = n_tokens;
+  if (scores) a.scores = {0.0f, scores->window, nullptr, scores->d_prefix, scores->d_first};
+  if (few_queries(p, a, n_seqs)) return 0;
+  return aq::paged_prompt_workspace(p->shape, n_q_heads, n_tokens, n_seqs, table_width);
+}
+
 int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, int n_q_heads,
                                int n_tokens, size_t q_nb1, size_t q_nb2, size_t out_nb1,
                                size_t out_nb2, const int *d_table, int table_width,
@@ -941,10 +955,7 @@ int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, i
   }
   if (!require_pointer(d_offsets, fn, "d_offsets") || !aligned_to(d_offsets, 4, fn) ||
       !out_apart(p, d_out, n_q_heads, out_nb1, out_nb2, d_q, n_q_heads, q_nb1, q_nb2, n_tokens,
-                 fn) ||
-      !workspace_ok(d_workspace, workspace_bytes,
-                    aq::paged_prompt_workspace(p->shape, n_q_heads, n_tokens, n_seqs, table_width),
-                    fn))
+                 fn))
     return -1;
   const aq::PagedSeqs q{d_table, table_width, table_stride, d_lengths, n_seqs};
   a.q = d_q;
@@ -957,9 +968,14 @@ int adaptq_paged_prompt_device(adaptq_paged_t h, const void *d_q, void *d_out, i
   a.n_tokens = n_tokens;
   a.offsets = d_offsets;
   a.scale = scale_of(p, scale);
+  const bool few = few_queries(p, a, n_seqs);
+  if (!few && !workspace_ok(d_workspace, workspace_bytes,
+                            aq::paged_prompt_workspace(p->shape, n_q_heads, n_tokens, n_seqs,
+                                                       table_width),
+                            fn))
+    return -1;
   DeviceGuard g(p->device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool few = few_queries(p, a, n_seqs);
   if (hip_fail(few ? aq::launch_paged_few(p->shape, q, a, p->ws, s)
                    : aq::launch_paged_prompt(p->shape, q, a, d_workspace, s),
                fn))

@@ -232,7 +232,8 @@ class PagedCache(_Pages):
             n = q.shape[0]
             if n and seqs[4]:
                 shape = self._scores(n, q.shape[1], softcap, slopes, prefix, first)
-                need = self._handle.prompt_workspace(q.shape[1], n, seqs[4], seqs[1])
+                need = self._handle.prompt_workspace(q.shape[1], n, seqs[4], seqs[1], args[1][1],
+                                                     *shape[2:])
                 space = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
                 self._handle.prompt(*args[0], n, *seqs, offsets.data_ptr(), *args[1], *shape,
                                     0 if space is None else space.data_ptr(), need,

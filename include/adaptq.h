@@ -500,9 +500,17 @@ typedef struct {
  * d_lengths[b] counts them (append them first).  Tokens outside the offsets are left as they
  * were.  Query heads, pages and d_out as in attend; scores NULL: every token up to its own.
  * Half types: rotated queries are rounded to the type before the products, the softmax's
- * weights enter as two numbers of it or more, the rest is fp32.  n_tokens * n_q_heads up to 2^31 - 1.  d_workspace:
- * device memory of adaptq_paged_prompt_workspace bytes (0 for many tokens), 16-byte
- * aligned, this call's alone until it is done.  Returns 0/-1. */
+ * weights enter as two numbers of it or more, the rest is fp32.
+ * n_tokens * n_q_heads up to 2^31 - 1.  d_workspace: device memory of
+ * adaptq_paged_prompt_scores_workspace bytes (0 for many tokens, and for few rows),
+ * 16-byte aligned, this call's alone until it is done; adaptq_paged_prompt_workspace: as many
+ * as the call takes whatever its scores.  Prompts of up to 16 rows a key head and sequence on
+ * the average (tokens times query heads of a key head), without d_first and without a window
+ * and prefixes at once, are attended like single tokens and use the cache's own workspace, so
+ * they need the same order among calls on one cache.  Returns 0/-1. */
+size_t adaptq_paged_prompt_scores_workspace(adaptq_paged_t cache, int n_q_heads, int n_tokens,
+                                            int n_seqs, int table_width,
+                                            const adaptq_scores_t *scores);
 size_t adaptq_paged_prompt_workspace(adaptq_paged_t cache, int n_q_heads, int n_tokens,
                                      int n_seqs, int table_width);
 int adaptq_paged_prompt_device(adaptq_paged_t cache, const void *d_q, void *d_out, int n_q_heads,
