@@ -1,8 +1,10 @@
 // paged_api.cpp -- the C ABI of the rotary positions and of the paged cache
 // (include/adaptq.h, part 3): argument checks, handles, launches.
 //
-// Nothing here synchronises or allocates after a handle's creation: every call is
-// one launch on the caller's stream and may be captured into a graph.
+// Nothing here synchronises or allocates after a handle's creation: a call is one
+// launch on the caller's stream, or a few in a row (prompts whose tiles are cut, the
+// weights of tokens, eviction, more blocks than a launch takes), and may be captured
+// into a graph.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -438,7 +440,10 @@ int paged_token(Paged *p, const Token &t, const aq::PagedSeqs &q, const aq::Page
 // query does (32 sequences of up to 4,000 tokens, 8 heads, 4 queries of 4 heads each 71.5 us,
 // through a prompt's tiles 111; 8 of 8,192, fp32, 8 queries of 2, a window of 1,000 34.5 and 51;
 // one of 16,000, 4 queries of 4, 43.2 and 44.8), two read all rows twice (8 of up to 1,500, 6
-// queries of 4, 35.4 and 33.9; four tiles, 16 of up to 4,000, 87 and 63).
+// queries of 4, 35.4 and 33.9; four tiles, 16 of up to 4,000, 87 and 63).  The average decides, for
+// the offsets are on the device; a chunk among single tokens is no slower by it (4 query heads of
+// 8, 63 single tokens and a chunk of 190 over 4,096 tokens each: 280 us, through a prompt's tiles
+// 317; the chunk over 16,384, the others over 1,024: 468 and 570).
 constexpr int kFewRows = 16;
 bool few_queries(const Paged *p, const aq::PagedPrompt &a, int n_seqs) {
   const long long rows = (long long)a.n_tokens * (a.q_heads / p->shape.n_heads);

@@ -283,7 +283,8 @@ class PagedCache(_Pages):
         pages to move to, with nothing of the sequences in them (sequences of up to keep tokens
         are copied whole); without it a page may be no second sequence's.  Returns where the
         tokens lay, int32 [sequences, heads, keep], -1 where there are none.  Refused where the
-        cache rotates: positions come from lengths then."""
+        cache rotates: positions come from lengths then.  Later calls' slopes, window, first and
+        prefix count the places that are left, not the tokens that were there."""
         seqs = self._sequences(table, lengths)
         if self._rotates:
             raise ValueError("a cache with a rotary takes positions from its lengths, which "

@@ -555,7 +555,9 @@ int adaptq_paged_step_scores_device(adaptq_paged_t cache, const void *d_k, const
  * that the sequences hold), where sequences of up to `keep` tokens are copied whole.  Their
  * weights move likewise within d_weights, with zeros behind (of sequences over `keep`).
  * d_kept [n_seqs][n_heads][keep]: where each place's token lay, -1 where there is none.
- * d_lengths is read alone: the caller lowers it to at most keep after the call.  Rows without
+ * d_lengths is read alone: the caller lowers it to at most keep after the call.  From then on a
+ * token's position is its place: d_slopes, windows, d_first and d_prefix of later calls count the
+ * places that are left, not the tokens that were there, and each key head keeps others.  Rows without
  * a page, or without one to go to, are not moved.  A page that several of the call's
  * sequences hold may not be evicted in place.  Caches with a rotary are refused.  Returns 0/-1. */
 int adaptq_paged_evict_device(adaptq_paged_t cache, float *d_weights, size_t w_nb1, size_t w_nb2,
